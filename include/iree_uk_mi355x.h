@@ -83,6 +83,47 @@ typedef long long iree_uk_index_t;
 #define IREE_UK_FLAG_QUERY_TILE_SIZES_OPERATION_MATMUL_BF16BF16F32 0x0500
 #define IREE_UK_FLAG_QUERY_TILE_SIZES_OPERATION_MATMUL_BF16BF16BF16 0x0600
 
+/* Flag values of the microscaled operators and of the norm (no counterpart in
+ * the reference). Type flags name the input's type, then the output's; of
+ * products the lhs, the rhs and the result. E2M1 and E4M3 are the 4-bit and
+ * 8-bit floats of the OCP microscaling formats, always with E8M0 scales. */
+#define IREE_UK_MI355X_FLAG_MX_PACK_TYPE_MASK 0xFF
+#define IREE_UK_MI355X_FLAG_MX_PACK_TYPE_F32E2M1 0x01
+#define IREE_UK_MI355X_FLAG_MX_PACK_TYPE_F16E2M1 0x02
+#define IREE_UK_MI355X_FLAG_MX_PACK_TYPE_BF16E2M1 0x03
+#define IREE_UK_MI355X_FLAG_MX_PACK_TYPE_F32E4M3 0x04
+#define IREE_UK_MI355X_FLAG_MX_PACK_TYPE_F16E4M3 0x05
+#define IREE_UK_MI355X_FLAG_MX_PACK_TYPE_BF16E4M3 0x06
+
+#define IREE_UK_MI355X_FLAG_MX_UNPACK_TYPE_MASK 0xFF
+#define IREE_UK_MI355X_FLAG_MX_UNPACK_TYPE_E2M1F32 0x01
+#define IREE_UK_MI355X_FLAG_MX_UNPACK_TYPE_E2M1F16 0x02
+#define IREE_UK_MI355X_FLAG_MX_UNPACK_TYPE_E2M1BF16 0x03
+#define IREE_UK_MI355X_FLAG_MX_UNPACK_TYPE_E4M3F32 0x04
+#define IREE_UK_MI355X_FLAG_MX_UNPACK_TYPE_E4M3F16 0x05
+#define IREE_UK_MI355X_FLAG_MX_UNPACK_TYPE_E4M3BF16 0x06
+
+#define IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_MASK 0xFF
+#define IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_E2M1E2M1F32 0x01
+#define IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_E2M1E2M1F16 0x02
+#define IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_E2M1E2M1BF16 0x03
+#define IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_E4M3E2M1F32 0x04
+#define IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_E4M3E2M1F16 0x05
+#define IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_E4M3E2M1BF16 0x06
+#define IREE_UK_MI355X_FLAG_MX_MMT4D_ACCUMULATE 0x100
+
+#define IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_MASK 0xFF
+#define IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_F32S8 0x01
+#define IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_F16S8 0x02
+#define IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_BF16S8 0x03
+#define IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_F32E4M3 0x04
+#define IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_F16E4M3 0x05
+#define IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_BF16E4M3 0x06
+#define IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_F32E2M1 0x07
+#define IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_F16E2M1 0x08
+#define IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_BF16E2M1 0x09
+#define IREE_UK_MI355X_FLAG_RMS_NORM_WEIGHT_F32 0x100
+
 /*===--------------------------------------------------------------------===*/
 /* Parameter structs (field order and types are ABI).                         */
 /*===--------------------------------------------------------------------===*/
@@ -163,6 +204,100 @@ typedef struct iree_uk_query_tile_sizes_2d_out_params_t {
   iree_uk_index_t tile_size0;
   iree_uk_index_t tile_size1;
 } iree_uk_query_tile_sizes_2d_out_params_t;
+
+/* Parameters of the operators without a counterpart in the reference, in the
+ * same manner: offsets and strides count ELEMENTS of the buffer's type (4-bit
+ * elements included; a scale is an element of one byte), only the outermost
+ * dimension of tiled operands is strided. */
+typedef struct iree_uk_mi355x_mx_pack_params_t {
+  const void* in_buffer;
+  iree_uk_index_t in_offset;
+  iree_uk_index_t in_stride0;
+  iree_uk_index_t in_stride1;
+  void* out_buffer;
+  iree_uk_index_t out_offset;
+  iree_uk_index_t out_stride0;
+  void* scales_buffer;
+  iree_uk_index_t scales_offset;
+  iree_uk_index_t scales_stride0;
+  iree_uk_index_t in_size0;
+  iree_uk_index_t in_size1;
+  iree_uk_index_t out_size0;
+  iree_uk_index_t out_size1;
+  iree_uk_index_t out_size2;
+  iree_uk_index_t out_size3;
+  uint32_t flags;
+} iree_uk_mi355x_mx_pack_params_t;
+
+typedef struct iree_uk_mi355x_mx_unpack_params_t {
+  const void* in_buffer;
+  iree_uk_index_t in_offset;
+  iree_uk_index_t in_stride0;
+  const void* scales_buffer;
+  iree_uk_index_t scales_offset;
+  iree_uk_index_t scales_stride0;
+  void* out_buffer;
+  iree_uk_index_t out_offset;
+  iree_uk_index_t out_stride0;
+  iree_uk_index_t out_stride1;
+  iree_uk_index_t in_size0;
+  iree_uk_index_t in_size1;
+  iree_uk_index_t in_size2;
+  iree_uk_index_t in_size3;
+  iree_uk_index_t out_size0;
+  iree_uk_index_t out_size1;
+  uint32_t flags;
+} iree_uk_mi355x_mx_unpack_params_t;
+
+typedef struct iree_uk_mi355x_mx_mmt4d_params_t {
+  const void* lhs_buffer;
+  iree_uk_index_t lhs_offset;
+  iree_uk_index_t lhs_stride0;
+  const void* lhs_scales_buffer;
+  iree_uk_index_t lhs_scales_offset;
+  iree_uk_index_t lhs_scales_stride0;
+  const void* rhs_buffer;
+  iree_uk_index_t rhs_offset;
+  iree_uk_index_t rhs_stride0;
+  const void* rhs_scales_buffer;
+  iree_uk_index_t rhs_scales_offset;
+  iree_uk_index_t rhs_scales_stride0;
+  void* out_buffer;
+  iree_uk_index_t out_offset;
+  iree_uk_index_t out_stride0;
+  iree_uk_index_t M;
+  iree_uk_index_t N;
+  iree_uk_index_t K;
+  int32_t M0;
+  int32_t N0;
+  int32_t K0;
+  uint32_t flags;
+} iree_uk_mi355x_mx_mmt4d_params_t;
+
+typedef struct iree_uk_mi355x_rms_norm_params_t {
+  const void* in_buffer;
+  iree_uk_index_t in_offset;
+  iree_uk_index_t in_stride0;
+  const void* residual_buffer; /* NULL: nothing is added */
+  iree_uk_index_t residual_offset;
+  iree_uk_index_t residual_stride0;
+  void* sum_buffer; /* NULL: the sum is not stored */
+  iree_uk_index_t sum_offset;
+  iree_uk_index_t sum_stride0;
+  const void* weight_buffer; /* NULL: ones */
+  iree_uk_index_t weight_offset;
+  void* out_buffer;
+  iree_uk_index_t out_offset;
+  iree_uk_index_t out_stride0;
+  void* scales_buffer;
+  iree_uk_index_t scales_offset;
+  iree_uk_index_t scales_stride0;
+  iree_uk_index_t size0;
+  iree_uk_index_t size1;
+  iree_uk_index_t out_size1;
+  float epsilon;
+  uint32_t flags;
+} iree_uk_mi355x_rms_norm_params_t;
 
 /*===--------------------------------------------------------------------===*/
 /* Entry points shared with the reference.                                    */
@@ -259,6 +394,65 @@ int iree_uk_mi355x_multi_mma_i32_16x16x64_i8(const void* a, const void* b, void*
                                              long long outer_n, int32_t k_size, int32_t intrinsics_m,
                                              int32_t subgroups_m, int32_t intrinsics_n, int32_t subgroups_n,
                                              int32_t intrinsics_k);
+
+/* Quantises a matrix into microscaled tiles: in[in_size0][in_size1] of f32,
+ * f16 or bf16, element (i, k) at i * in_stride0 + k * in_stride1, into codes
+ * out[out_size0][out_size1][out_size2][out_size3] as iree_uk_pack tiles them
+ * and one scale byte for each 32 consecutive values of a tile's row,
+ * scales[out_size0][out_size1][out_size2][out_size3 / 32]. out_size3 is a
+ * multiple of 32. A 4-bit code with an even index lies in the low half of its
+ * byte. Strides in_stride0 = 1, in_stride1 = pitch read a transposed matrix.
+ * Tiles one row tall (out_size2 = 1, out_size3 = out_stride0 = the padded
+ * row) are the row-major form.
+ *   For a block with the largest magnitude a, all finite:
+ *     scale byte b = max(floor(log2 a) + 127 - e, 0), e = 2 (E2M1) or 8 (E4M3),
+ *     code = the element nearest to x / 2^(b - 127), ties to the even code, the
+ *     largest element (6 or 448) beyond it; a = 0 gives b = 0 and zero codes.
+ *   A block that holds an infinity or a NaN: scale byte 255 (NaN), zero codes.
+ *   What pads the matrix to whole tiles counts as zero.
+ * The outputs may not overlap each other, an input or, row for row,
+ * themselves. */
+void iree_uk_mi355x_mx_pack_p(const iree_uk_mi355x_mx_pack_params_t* params);
+
+/* The inverse: code * 2^(scale - 127), rounded to nearest even in the output's
+ * type (infinity beyond its range; scale byte 255 and the NaN codes of E4M3 are
+ * NaN). Writes only the out_size0 x out_size1 logical region, element (i, k) at
+ * i * out_stride0 + k * out_stride1. */
+void iree_uk_mi355x_mx_unpack_p(const iree_uk_mi355x_mx_unpack_params_t* params);
+
+/* iree_uk_mmt4d of microscaled operands: out[M,N,M0,N0] (+)= lhs * rhs^T with
+ * lhs[M,K,M0,K0] of E2M1 or E4M3 and rhs[N,K,N0,K0] of E2M1, their scales
+ * [M,K,M0,K0/32] and [N,K,N0,K0/32] as iree_uk_mi355x_mx_pack_p writes them.
+ * K0 is a multiple of 32. Sums are in f32; the result is rounded once to f16 or
+ * bf16 where that is its type (with IREE_UK_MI355X_FLAG_MX_MMT4D_ACCUMULATE the
+ * destination's value is added before that rounding). A scale byte of 255 makes
+ * every result that its block takes part in NaN, zero codes or not. Products
+ * and sums below the smallest normal f32 may come out as zero. The order of
+ * summation is fixed for a call's parameters: the same call gives the same bits.
+ * The fast kernels take operands whose K0 is 128 or whose tiles are one row
+ * tall (a row-major matrix with row-major scales) and whose buffers and
+ * strides are multiples of 16 bytes (scales: of 4); rhs tiles of 16 x 128 suit
+ * them best. Others run on a kernel with one thread for each result. */
+void iree_uk_mi355x_mx_mmt4d_p(const iree_uk_mi355x_mx_mmt4d_params_t* params);
+
+/* Root-mean-square norm of the rows of a matrix, with the residual's addition,
+ * into rows that a product reads as its lhs with tiles one row tall. For each
+ * of size0 rows of size1 values:
+ *   s = in + residual, rounded to their type; stored in `sum` if there is one
+ *       (which may be `in` or `residual` itself)
+ *   r = 1 / sqrt(mean(s^2) + epsilon), summed in f64, rounded once to f32
+ *   y = (s * r) * weight in f32 (weight: the type of `in`, or f32 with
+ *       IREE_UK_MI355X_FLAG_RMS_NORM_WEIGHT_F32)
+ * and the row of out_size1 >= size1 values, zeros behind the size1 ones, is
+ *   S8: q = y * (1 / scale) rounded to nearest even, for iree_uk_mmt4d's S8S8S32
+ *       and S8S4S32; scales: one f32 a row, scale = max(max|y| / 127, 2^-126).
+ *       A row with a y that is not finite: scale NaN, all q zero.
+ *   E4M3, E2M1: codes and scale bytes as iree_uk_mi355x_mx_pack_p makes them of
+ *       y, [size0][out_size1 / 32] bytes, rows scales_stride0 apart.
+ *       out_size1 is a multiple of 32.
+ * `sum` needs a residual. The outputs may not overlap each other or an input,
+ * but for a `sum` at exactly the place of `in` or `residual`. */
+void iree_uk_mi355x_rms_norm_p(const iree_uk_mi355x_rms_norm_params_t* params);
 
 /* iree_uk_mmt4d_p for callers that cannot allocate. It has no counterpart in
  * the reference (whose microkernels never allocate, being CPU code); it is for

@@ -54,6 +54,37 @@ QTS_OP_MATMUL_F16F16F16 = 0x0400
 QTS_OP_MATMUL_BF16BF16F32 = 0x0500
 QTS_OP_MATMUL_BF16BF16BF16 = 0x0600
 
+# --- microscaled operators and the norm (no counterpart in the reference) ----
+MX_PACK_TYPE_F32E2M1 = 0x01
+MX_PACK_TYPE_F16E2M1 = 0x02
+MX_PACK_TYPE_BF16E2M1 = 0x03
+MX_PACK_TYPE_F32E4M3 = 0x04
+MX_PACK_TYPE_F16E4M3 = 0x05
+MX_PACK_TYPE_BF16E4M3 = 0x06
+MX_UNPACK_TYPE_E2M1F32 = 0x01
+MX_UNPACK_TYPE_E2M1F16 = 0x02
+MX_UNPACK_TYPE_E2M1BF16 = 0x03
+MX_UNPACK_TYPE_E4M3F32 = 0x04
+MX_UNPACK_TYPE_E4M3F16 = 0x05
+MX_UNPACK_TYPE_E4M3BF16 = 0x06
+MX_MMT4D_TYPE_E2M1E2M1F32 = 0x01
+MX_MMT4D_TYPE_E2M1E2M1F16 = 0x02
+MX_MMT4D_TYPE_E2M1E2M1BF16 = 0x03
+MX_MMT4D_TYPE_E4M3E2M1F32 = 0x04
+MX_MMT4D_TYPE_E4M3E2M1F16 = 0x05
+MX_MMT4D_TYPE_E4M3E2M1BF16 = 0x06
+MX_MMT4D_ACCUMULATE = 0x100
+RMS_NORM_TYPE_F32S8 = 0x01
+RMS_NORM_TYPE_F16S8 = 0x02
+RMS_NORM_TYPE_BF16S8 = 0x03
+RMS_NORM_TYPE_F32E4M3 = 0x04
+RMS_NORM_TYPE_F16E4M3 = 0x05
+RMS_NORM_TYPE_BF16E4M3 = 0x06
+RMS_NORM_TYPE_F32E2M1 = 0x07
+RMS_NORM_TYPE_F16E2M1 = 0x08
+RMS_NORM_TYPE_BF16E2M1 = 0x09
+RMS_NORM_WEIGHT_F32 = 0x100
+
 # (lhs bits, rhs bits, out bits) per mmt4d type flag.
 MMT4D_BITS = {
     MMT4D_TYPE_F32F32F32: (32, 32, 32),
@@ -125,6 +156,58 @@ class QueryTileSizes2dParams(C.Structure):
 
 class QueryTileSizes2dOutParams(C.Structure):
     _fields_ = [("tile_size0", index_t), ("tile_size1", index_t)]
+
+
+class MxPackParams(C.Structure):
+    _fields_ = [
+        ("in_buffer", C.c_void_p), ("in_offset", index_t),
+        ("in_stride0", index_t), ("in_stride1", index_t),
+        ("out_buffer", C.c_void_p), ("out_offset", index_t), ("out_stride0", index_t),
+        ("scales_buffer", C.c_void_p), ("scales_offset", index_t), ("scales_stride0", index_t),
+        ("in_size0", index_t), ("in_size1", index_t),
+        ("out_size0", index_t), ("out_size1", index_t),
+        ("out_size2", index_t), ("out_size3", index_t),
+        ("flags", C.c_uint32),
+    ]
+
+
+class MxUnpackParams(C.Structure):
+    _fields_ = [
+        ("in_buffer", C.c_void_p), ("in_offset", index_t), ("in_stride0", index_t),
+        ("scales_buffer", C.c_void_p), ("scales_offset", index_t), ("scales_stride0", index_t),
+        ("out_buffer", C.c_void_p), ("out_offset", index_t),
+        ("out_stride0", index_t), ("out_stride1", index_t),
+        ("in_size0", index_t), ("in_size1", index_t),
+        ("in_size2", index_t), ("in_size3", index_t),
+        ("out_size0", index_t), ("out_size1", index_t),
+        ("flags", C.c_uint32),
+    ]
+
+
+class MxMmt4dParams(C.Structure):
+    _fields_ = [
+        ("lhs_buffer", C.c_void_p), ("lhs_offset", index_t), ("lhs_stride0", index_t),
+        ("lhs_scales_buffer", C.c_void_p), ("lhs_scales_offset", index_t), ("lhs_scales_stride0", index_t),
+        ("rhs_buffer", C.c_void_p), ("rhs_offset", index_t), ("rhs_stride0", index_t),
+        ("rhs_scales_buffer", C.c_void_p), ("rhs_scales_offset", index_t), ("rhs_scales_stride0", index_t),
+        ("out_buffer", C.c_void_p), ("out_offset", index_t), ("out_stride0", index_t),
+        ("M", index_t), ("N", index_t), ("K", index_t),
+        ("M0", C.c_int32), ("N0", C.c_int32), ("K0", C.c_int32),
+        ("flags", C.c_uint32),
+    ]
+
+
+class RmsNormParams(C.Structure):
+    _fields_ = [
+        ("in_buffer", C.c_void_p), ("in_offset", index_t), ("in_stride0", index_t),
+        ("residual_buffer", C.c_void_p), ("residual_offset", index_t), ("residual_stride0", index_t),
+        ("sum_buffer", C.c_void_p), ("sum_offset", index_t), ("sum_stride0", index_t),
+        ("weight_buffer", C.c_void_p), ("weight_offset", index_t),
+        ("out_buffer", C.c_void_p), ("out_offset", index_t), ("out_stride0", index_t),
+        ("scales_buffer", C.c_void_p), ("scales_offset", index_t), ("scales_stride0", index_t),
+        ("size0", index_t), ("size1", index_t), ("out_size1", index_t),
+        ("epsilon", C.c_float), ("flags", C.c_uint32),
+    ]
 
 
 def mmt4d_spans(p):

@@ -476,8 +476,9 @@ bool pipe_down(const Stager& stager, void* host, const void* dev, size_t bytes, 
 }
 
 // Makes the operands of a call reachable from the device.
+constexpr int kMostOperands = 6;
 bool stage_operands(Stager& stager, Operand* const* ops, int count, hipStream_t stream) {
-  Operand* mirrored[3];
+  Operand* mirrored[kMostOperands];
   int mirrors = 0, piped = 0;
   for (int i = 0; i < count; ++i) {
     Operand& o = *ops[i];
@@ -981,6 +982,351 @@ UK_API void iree_uk_query_tile_sizes_2d(const iree_uk_query_tile_sizes_2d_params
     case IREE_UK_FLAG_QUERY_TILE_SIZES_OPERAND_ROLE_RESULT: o->tile_size0 = M0; o->tile_size1 = N0; break;
     default: UK_REQUIRE(!"unknown operand role");
   }
+}
+
+//===----------------------------------------------------------------------===//
+// Microscaled operators and the norm (no counterpart in the reference)
+//===----------------------------------------------------------------------===//
+
+namespace {
+
+// Whether an operand that is written shares bytes with another one. Rows that interleave at the same pitch (column ranges
+// of one wider matrix) do not; any other two spans that cross are taken to.
+bool overlap(const Operand& a, const Operand& b) {
+  if (a.region.span == 0 || b.region.span == 0) return false;
+  const uintptr_t x = (uintptr_t)a.ptr, y = (uintptr_t)b.ptr;
+  if (x + (uintptr_t)a.region.span <= y || y + (uintptr_t)b.region.span <= x) return false;
+  const int64_t pitch = a.region.pitch;
+  if (pitch != b.region.pitch || a.region.rows == 1 || b.region.rows == 1) return true;
+  const int64_t between = x <= y ? (int64_t)((y - x) % (uintptr_t)pitch) : (pitch - (int64_t)((x - y) % (uintptr_t)pitch)) % pitch;
+  return between < a.region.width || between + b.region.width > pitch;
+}
+
+// Whether an operand that a call touches has an address.
+bool given(const Operand& o) { return o.region.span == 0 || o.ptr != nullptr; }
+
+bool same_place(const Operand& a, const Operand& b) {
+  return a.ptr == b.ptr && (a.region.rows == 1 || a.region.pitch == b.region.pitch);
+}
+
+// Rows that are written concurrently lie apart.
+bool rows_apart(const RowRegion& r) { return r.rows <= 1 || r.pitch >= r.width; }
+
+RowRegion as_copied(const RowRegion& r) { return r.rows > 1 && r.pitch < r.width ? as_one_span(r) : r; }
+
+// Ends a call with several results: every one of them back where the caller has it.
+bool finish(const Stager& stager, hipStream_t stream, const Operand* const* outs, int count) {
+  for (int i = 0; i < count; ++i) {
+    if (outs[i]->host && !finish(stager, stream, *outs[i])) return false;
+  }
+  if (!tl_async) UK_HIP_OK(hipStreamSynchronize(stream));
+  return true;
+}
+
+// Type flags of these operators number the float types 1 to 3, once for each other type of the call.
+uk::Float float_of(uint32_t type) { return (uk::Float)((type - 1) % 3); }
+
+}  // namespace
+
+UK_API void iree_uk_mi355x_mx_pack_p(const iree_uk_mi355x_mx_pack_params_t* p) {
+  tl_last_kernel = "";
+  UK_REQUIRE(p != nullptr);
+  UK_REQUIRE(!(p->flags & ~(uint32_t)IREE_UK_MI355X_FLAG_MX_PACK_TYPE_MASK));
+  UK_REQUIRE(p->flags >= IREE_UK_MI355X_FLAG_MX_PACK_TYPE_F32E2M1 &&
+             p->flags <= IREE_UK_MI355X_FLAG_MX_PACK_TYPE_BF16E4M3);
+  const uk::Float type = float_of(p->flags);
+  const int e = uk::float_bytes(type), bits = p->flags <= IREE_UK_MI355X_FLAG_MX_PACK_TYPE_BF16E2M1 ? 4 : 8;
+  UK_REQUIRE(p->in_size0 >= 0);
+  UK_REQUIRE(p->in_size1 >= 0);
+  UK_REQUIRE(p->out_size0 >= 0);
+  UK_REQUIRE(p->out_size1 >= 0);
+  UK_REQUIRE(p->out_size2 >= 0);
+  UK_REQUIRE(p->out_size3 >= 0);
+  UK_REQUIRE(p->in_stride0 >= 0);
+  UK_REQUIRE(p->in_stride1 >= 0);
+  UK_REQUIRE(p->out_stride0 >= 0);
+  UK_REQUIRE(p->scales_stride0 >= 0);
+  UK_REQUIRE(p->out_size3 % 32 == 0);
+  UK_REQUIRE(bits == 8 || (p->out_offset % 2 == 0 && p->out_stride0 % 2 == 0));
+  UK_REQUIRE(tiles_cover(p->out_size0, p->out_size2, p->in_size0));
+  UK_REQUIRE(tiles_cover(p->out_size1, p->out_size3, p->in_size1));
+  if (p->out_size0 == 0 || p->out_size1 == 0 || p->out_size2 == 0 || p->out_size3 == 0) return;
+
+  Checked c;
+  const bool have_input = p->in_size0 > 0 && p->in_size1 > 0;
+  const RowRegion in_region =
+      make_region(c, have_input ? p->in_size0 : 0, c.mul(c.add(c.mul(p->in_size1 - 1, p->in_stride1), 1), e),
+                  c.mul(p->in_stride0, e));
+  const int64_t row = c.mul(p->out_size1, c.mul(p->out_size2, p->out_size3));
+  const RowRegion codes_region = make_region(c, p->out_size0, c.bytes(row, bits), c.bytes(p->out_stride0, bits));
+  const RowRegion scales_region = make_region(c, p->out_size0, row / 32, p->scales_stride0);
+  const int64_t in_offset_bytes = c.mul(p->in_offset, e), out_offset_bytes = c.bytes(p->out_offset, bits);
+  UK_REQUIRE(c.ok && "operand extents fit int64");
+  UK_REQUIRE(rows_apart(codes_region));
+  UK_REQUIRE(rows_apart(scales_region));
+
+  hipStream_t stream = tl_stream;
+  Stager stager;
+  Operand o_in{offset_pointer(p->in_buffer, in_offset_bytes), as_copied(in_region), true};
+  Operand o_codes{offset_pointer(p->out_buffer, out_offset_bytes), codes_region, false};
+  Operand o_scales{offset_pointer(p->scales_buffer, p->scales_offset), scales_region, false};
+  UK_REQUIRE(!overlap(o_codes, o_scales));
+  UK_REQUIRE(!overlap(o_codes, o_in));
+  UK_REQUIRE(!overlap(o_scales, o_in));
+  Operand* const operands[] = {&o_in, &o_codes, &o_scales};
+  for (const Operand* o : operands) UK_REQUIRE(given(*o));
+  if (!stage_operands(stager, operands, 3, stream)) {
+    abandon(stager, stream);
+    return;
+  }
+  uk::MxPackArgs a;
+  a.in = (const uint8_t*)o_in.dev;
+  a.codes = (uint8_t*)const_cast<void*>(o_codes.dev);
+  a.scales = (uint8_t*)const_cast<void*>(o_scales.dev);
+  a.in_stride0 = p->in_stride0; a.in_stride1 = p->in_stride1;
+  a.codes_stride0 = codes_region.pitch; a.scales_stride0 = scales_region.pitch;
+  a.in_size0 = p->in_size0; a.in_size1 = p->in_size1;
+  a.outer0 = p->out_size0; a.outer1 = p->out_size1; a.tile0 = p->out_size2; a.tile1 = p->out_size3;
+  a.type = type;
+  a.bits = bits;
+  if (!launch_ok(uk::launch_mx_pack(a, stream, &tl_last_kernel), "mx_pack")) {
+    abandon(stager, stream);
+    return;
+  }
+  const Operand* const outs[] = {&o_codes, &o_scales};
+  finish(stager, stream, outs, 2);
+}
+
+UK_API void iree_uk_mi355x_mx_unpack_p(const iree_uk_mi355x_mx_unpack_params_t* p) {
+  tl_last_kernel = "";
+  UK_REQUIRE(p != nullptr);
+  UK_REQUIRE(!(p->flags & ~(uint32_t)IREE_UK_MI355X_FLAG_MX_UNPACK_TYPE_MASK));
+  UK_REQUIRE(p->flags >= IREE_UK_MI355X_FLAG_MX_UNPACK_TYPE_E2M1F32 &&
+             p->flags <= IREE_UK_MI355X_FLAG_MX_UNPACK_TYPE_E4M3BF16);
+  const uk::Float type = float_of(p->flags);
+  const int e = uk::float_bytes(type), bits = p->flags <= IREE_UK_MI355X_FLAG_MX_UNPACK_TYPE_E2M1BF16 ? 4 : 8;
+  UK_REQUIRE(p->out_size0 >= 0);
+  UK_REQUIRE(p->out_size1 >= 0);
+  UK_REQUIRE(p->in_size0 >= 0);
+  UK_REQUIRE(p->in_size1 >= 0);
+  UK_REQUIRE(p->in_size2 >= 0);
+  UK_REQUIRE(p->in_size3 >= 0);
+  UK_REQUIRE(p->in_stride0 >= 0);
+  UK_REQUIRE(p->scales_stride0 >= 0);
+  UK_REQUIRE(p->out_stride0 >= 0);
+  UK_REQUIRE(p->out_stride1 >= 0);
+  UK_REQUIRE(p->in_size3 % 32 == 0);
+  UK_REQUIRE(bits == 8 || (p->in_offset % 2 == 0 && p->in_stride0 % 2 == 0));
+  UK_REQUIRE(tiles_cover(p->in_size0, p->in_size2, p->out_size0));
+  UK_REQUIRE(tiles_cover(p->in_size1, p->in_size3, p->out_size1));
+  if (p->out_size0 == 0 || p->out_size1 == 0) return;
+
+  Checked c;
+  const int64_t row = c.mul(p->in_size1, c.mul(p->in_size2, p->in_size3));
+  const RowRegion codes_region = make_region(c, p->in_size0, c.bytes(row, bits), c.bytes(p->in_stride0, bits));
+  const RowRegion scales_region = make_region(c, p->in_size0, row / 32, p->scales_stride0);
+  const RowRegion out_region =
+      make_region(c, p->out_size0, c.mul(c.add(c.mul(p->out_size1 - 1, p->out_stride1), 1), e), c.mul(p->out_stride0, e));
+  const int64_t in_offset_bytes = c.bytes(p->in_offset, bits), out_offset_bytes = c.mul(p->out_offset, e);
+  UK_REQUIRE(c.ok && "operand extents fit int64");
+  UK_REQUIRE(rows_apart(out_region));
+  UK_REQUIRE(p->out_size1 == 1 || p->out_stride1 >= 1);
+
+  hipStream_t stream = tl_stream;
+  Stager stager;
+  Operand o_codes{offset_pointer(p->in_buffer, in_offset_bytes), as_copied(codes_region), true};
+  Operand o_scales{offset_pointer(p->scales_buffer, p->scales_offset), as_copied(scales_region), true};
+  // (With an inner stride the bytes between elements have to survive the way through the staging memory.)
+  Operand o_out{offset_pointer(p->out_buffer, out_offset_bytes), out_region, p->out_stride1 != 1};
+  UK_REQUIRE(!overlap(o_out, o_codes));
+  UK_REQUIRE(!overlap(o_out, o_scales));
+  Operand* const operands[] = {&o_codes, &o_scales, &o_out};
+  for (const Operand* o : operands) UK_REQUIRE(given(*o));
+  if (!stage_operands(stager, operands, 3, stream)) {
+    abandon(stager, stream);
+    return;
+  }
+  uk::MxUnpackArgs a;
+  a.codes = (const uint8_t*)o_codes.dev;
+  a.scales = (const uint8_t*)o_scales.dev;
+  a.out = (uint8_t*)const_cast<void*>(o_out.dev);
+  a.codes_stride0 = codes_region.pitch; a.scales_stride0 = scales_region.pitch;
+  a.out_stride0 = p->out_stride0; a.out_stride1 = p->out_stride1;
+  a.outer0 = p->in_size0; a.outer1 = p->in_size1; a.tile0 = p->in_size2; a.tile1 = p->in_size3;
+  a.out_size0 = p->out_size0; a.out_size1 = p->out_size1;
+  a.type = type;
+  a.bits = bits;
+  if (!launch_ok(uk::launch_mx_unpack(a, stream, &tl_last_kernel), "mx_unpack")) {
+    abandon(stager, stream);
+    return;
+  }
+  finish(stager, stream, o_out);
+}
+
+UK_API void iree_uk_mi355x_mx_mmt4d_p(const iree_uk_mi355x_mx_mmt4d_params_t* p) {
+  tl_last_kernel = "";
+  UK_REQUIRE(p != nullptr);
+  const uint32_t known = IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_MASK | IREE_UK_MI355X_FLAG_MX_MMT4D_ACCUMULATE;
+  UK_REQUIRE(!(p->flags & ~known));
+  const uint32_t type = p->flags & IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_MASK;
+  UK_REQUIRE(type >= IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_E2M1E2M1F32 &&
+             type <= IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_E4M3E2M1BF16);
+  const int lb = type <= IREE_UK_MI355X_FLAG_MX_MMT4D_TYPE_E2M1E2M1BF16 ? 4 : 8;
+  const uk::Float out_type = float_of(type);
+  const int e = uk::float_bytes(out_type);
+  UK_REQUIRE(in_unsigned_range(p->M, 31));
+  UK_REQUIRE(in_unsigned_range(p->N, 31));
+  UK_REQUIRE(in_unsigned_range(p->K, 31));
+  UK_REQUIRE(in_unsigned_range(p->M0, 15));
+  UK_REQUIRE(in_unsigned_range(p->N0, 15));
+  UK_REQUIRE(in_unsigned_range(p->K0, 15));
+  UK_REQUIRE(p->K0 % 32 == 0);
+  UK_REQUIRE(lb == 8 || (p->lhs_offset % 2 == 0 && p->lhs_stride0 % 2 == 0));
+  UK_REQUIRE(p->rhs_offset % 2 == 0 && p->rhs_stride0 % 2 == 0);
+  const bool accumulate = p->flags & IREE_UK_MI355X_FLAG_MX_MMT4D_ACCUMULATE;
+  if (p->M == 0 || p->N == 0 || ((p->K == 0 || p->K0 == 0) && accumulate)) return;
+  if (p->M0 == 0 || p->N0 == 0) return;
+
+  Checked c;
+  const int64_t lhs_row = c.mul(p->K, (int64_t)p->M0 * p->K0), rhs_row = c.mul(p->K, (int64_t)p->N0 * p->K0);
+  const RowRegion lhs_region = make_region(c, p->M, c.bytes(lhs_row, lb), c.bytes(p->lhs_stride0, lb));
+  const RowRegion rhs_region = make_region(c, p->N, c.bytes(rhs_row, 4), c.bytes(p->rhs_stride0, 4));
+  const RowRegion lhs_scales_region = make_region(c, p->M, lhs_row / 32, p->lhs_scales_stride0);
+  const RowRegion rhs_scales_region = make_region(c, p->N, rhs_row / 32, p->rhs_scales_stride0);
+  const RowRegion out_region =
+      make_region(c, p->M, c.mul(c.mul(p->N, (int64_t)p->M0 * p->N0), e), c.mul(p->out_stride0, e));
+  const int64_t lhs_offset_bytes = c.bytes(p->lhs_offset, lb), rhs_offset_bytes = c.bytes(p->rhs_offset, 4),
+                out_offset_bytes = c.mul(p->out_offset, e);
+  UK_REQUIRE(c.ok && "operand extents fit int64");
+  // Panels of the operands may coincide or overlap (they are only read); see iree_uk_mmt4d.
+  UK_REQUIRE(p->M == 1 || (p->lhs_stride0 >= 0 && p->lhs_scales_stride0 >= 0));
+  UK_REQUIRE(p->N == 1 || (p->rhs_stride0 >= 0 && p->rhs_scales_stride0 >= 0));
+  UK_REQUIRE(rows_apart(out_region));
+
+  hipStream_t stream = tl_stream;
+  Stager stager;
+  Operand o_lhs{offset_pointer(p->lhs_buffer, lhs_offset_bytes), as_copied(lhs_region), true};
+  Operand o_lhs_scales{offset_pointer(p->lhs_scales_buffer, p->lhs_scales_offset), as_copied(lhs_scales_region), true};
+  Operand o_rhs{offset_pointer(p->rhs_buffer, rhs_offset_bytes), as_copied(rhs_region), true};
+  Operand o_rhs_scales{offset_pointer(p->rhs_scales_buffer, p->rhs_scales_offset), as_copied(rhs_scales_region), true};
+  Operand o_out{offset_pointer(p->out_buffer, out_offset_bytes), out_region, accumulate};
+  Operand* const operands[] = {&o_lhs, &o_lhs_scales, &o_rhs, &o_rhs_scales, &o_out};
+  for (const Operand* o : operands) UK_REQUIRE(given(*o));
+  for (int i = 0; i < 4; ++i) UK_REQUIRE(!overlap(o_out, *operands[i]));
+  if (!stage_operands(stager, operands, 5, stream)) {
+    abandon(stager, stream);
+    return;
+  }
+  uk::MxMmt4dArgs a;
+  a.lhs = (const uint8_t*)o_lhs.dev;
+  a.lhs_scales = (const uint8_t*)o_lhs_scales.dev;
+  a.rhs = (const uint8_t*)o_rhs.dev;
+  a.rhs_scales = (const uint8_t*)o_rhs_scales.dev;
+  a.out = (uint8_t*)const_cast<void*>(o_out.dev);
+  a.lhs_stride0 = lhs_region.pitch; a.lhs_scales_stride0 = lhs_scales_region.pitch;
+  a.rhs_stride0 = rhs_region.pitch; a.rhs_scales_stride0 = rhs_scales_region.pitch;
+  a.out_stride0 = p->out_stride0;
+  a.M = p->M; a.N = p->N; a.K = p->K0 == 0 ? 0 : p->K;
+  a.M0 = p->M0; a.N0 = p->N0; a.K0 = p->K0 == 0 ? 32 : p->K0;
+  a.lhs_bits = lb;
+  a.out_type = out_type;
+  a.accumulate = accumulate;
+  if (!launch_ok(uk::launch_mx_mmt4d(a, stream, &tl_last_kernel), "mx_mmt4d")) {
+    abandon(stager, stream);
+    return;
+  }
+  finish(stager, stream, o_out);
+}
+
+UK_API void iree_uk_mi355x_rms_norm_p(const iree_uk_mi355x_rms_norm_params_t* p) {
+  tl_last_kernel = "";
+  UK_REQUIRE(p != nullptr);
+  const uint32_t known = IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_MASK | IREE_UK_MI355X_FLAG_RMS_NORM_WEIGHT_F32;
+  UK_REQUIRE(!(p->flags & ~known));
+  const uint32_t flag = p->flags & IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_MASK;
+  UK_REQUIRE(flag >= IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_F32S8 && flag <= IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_BF16E2M1);
+  const uk::Float type = float_of(flag);
+  const uk::NormOut out_type = (uk::NormOut)((flag - 1) / 3);
+  const uk::Float weight_type = p->flags & IREE_UK_MI355X_FLAG_RMS_NORM_WEIGHT_F32 ? uk::Float::kF32 : type;
+  const int e = uk::float_bytes(type), bits = out_type == uk::NormOut::kE2M1 ? 4 : 8;
+  const bool rows_of_bytes = out_type != uk::NormOut::kS8;  // scales: bytes in rows, or one f32 a row
+  UK_REQUIRE(p->size0 >= 0);
+  UK_REQUIRE(p->size1 >= 0);
+  UK_REQUIRE(p->out_size1 >= p->size1);
+  UK_REQUIRE(!rows_of_bytes || p->out_size1 % 32 == 0);
+  UK_REQUIRE(p->in_stride0 >= 0);
+  UK_REQUIRE(!p->residual_buffer || p->residual_stride0 >= 0);
+  UK_REQUIRE(!p->sum_buffer || (p->residual_buffer && p->sum_stride0 >= 0));
+  UK_REQUIRE(p->out_stride0 >= 0);
+  UK_REQUIRE(p->scales_stride0 >= 0);
+  UK_REQUIRE(p->epsilon >= 0);
+  UK_REQUIRE(bits == 8 || (p->out_offset % 2 == 0 && p->out_stride0 % 2 == 0));
+  if (p->size0 == 0 || p->out_size1 == 0) return;
+
+  Checked c;
+  const int64_t width = c.mul(p->size1, e);
+  const RowRegion in_region = make_region(c, p->size0, width, c.mul(p->in_stride0, e));
+  const RowRegion residual_region =
+      make_region(c, p->residual_buffer ? p->size0 : 0, width, c.mul(p->residual_buffer ? p->residual_stride0 : 0, e));
+  const RowRegion sum_region =
+      make_region(c, p->sum_buffer ? p->size0 : 0, width, c.mul(p->sum_buffer ? p->sum_stride0 : 0, e));
+  const int weight_bytes = uk::float_bytes(weight_type);
+  const RowRegion weight_region = make_region(c, p->weight_buffer ? 1 : 0, c.mul(p->size1, weight_bytes), 0);
+  const RowRegion out_region = make_region(c, p->size0, c.bytes(p->out_size1, bits),
+                                            c.bytes(p->out_stride0, bits));
+  const int scale_bytes = rows_of_bytes ? 1 : 4;
+  const RowRegion scales_region =
+      make_region(c, p->size0, rows_of_bytes ? p->out_size1 / 32 : 4, c.mul(p->scales_stride0, scale_bytes));
+  const int64_t in_offset = c.mul(p->in_offset, e), residual_offset = c.mul(p->residual_buffer ? p->residual_offset : 0, e),
+                sum_offset = c.mul(p->sum_buffer ? p->sum_offset : 0, e),
+                weight_offset = c.mul(p->weight_buffer ? p->weight_offset : 0, weight_bytes),
+                out_offset = c.bytes(p->out_offset, bits), scales_offset = c.mul(p->scales_offset, scale_bytes);
+  UK_REQUIRE(c.ok && "operand extents fit int64");
+  UK_REQUIRE(rows_apart(sum_region));
+  UK_REQUIRE(rows_apart(out_region));
+  UK_REQUIRE(rows_apart(scales_region));
+
+  hipStream_t stream = tl_stream;
+  Stager stager;
+  Operand o_in{offset_pointer(p->in_buffer, in_offset), as_copied(in_region), true};
+  Operand o_residual{offset_pointer(p->residual_buffer, residual_offset), as_copied(residual_region), true};
+  Operand o_sum{offset_pointer(p->sum_buffer, sum_offset), sum_region, false};
+  Operand o_weight{offset_pointer(p->weight_buffer, weight_offset), weight_region, true};
+  Operand o_out{offset_pointer(p->out_buffer, out_offset), out_region, false};
+  Operand o_scales{offset_pointer(p->scales_buffer, scales_offset), scales_region, false};
+  UK_REQUIRE(same_place(o_sum, o_in) || !overlap(o_sum, o_in));
+  UK_REQUIRE(same_place(o_sum, o_residual) || !overlap(o_sum, o_residual));
+  UK_REQUIRE(!overlap(o_sum, o_weight));
+  const Operand* const inputs[] = {&o_in, &o_residual, &o_sum, &o_weight};
+  for (const Operand* i : inputs) {
+    UK_REQUIRE(!overlap(o_out, *i));
+    UK_REQUIRE(!overlap(o_scales, *i));
+  }
+  UK_REQUIRE(!overlap(o_out, o_scales));
+  Operand* const operands[] = {&o_in, &o_residual, &o_sum, &o_weight, &o_out, &o_scales};
+  for (const Operand* o : operands) UK_REQUIRE(given(*o));
+  if (!stage_operands(stager, operands, 6, stream)) {
+    abandon(stager, stream);
+    return;
+  }
+  uk::RmsNormArgs a;
+  a.in = (const uint8_t*)o_in.dev;
+  a.residual = p->residual_buffer ? (const uint8_t*)o_residual.dev : nullptr;
+  a.sum = p->sum_buffer ? (uint8_t*)const_cast<void*>(o_sum.dev) : nullptr;
+  a.weight = p->weight_buffer ? (const uint8_t*)o_weight.dev : nullptr;
+  a.out = (uint8_t*)const_cast<void*>(o_out.dev);
+  a.scales = (uint8_t*)const_cast<void*>(o_scales.dev);
+  a.in_stride0 = p->in_stride0; a.residual_stride0 = p->residual_stride0; a.sum_stride0 = p->sum_stride0;
+  a.out_stride0 = out_region.pitch; a.scales_stride0 = scales_region.pitch;
+  a.size0 = p->size0; a.size1 = p->size1; a.out_size1 = p->out_size1;
+  a.epsilon = p->epsilon;
+  a.type = type; a.weight_type = weight_type; a.out_type = out_type;
+  if (!launch_ok(uk::launch_rms_norm(a, stream, &tl_last_kernel), "rms_norm")) {
+    abandon(stager, stream);
+    return;
+  }
+  const Operand* const outs[] = {&o_sum, &o_out, &o_scales};
+  finish(stager, stream, outs, 3);
 }
 
 //===----------------------------------------------------------------------===//

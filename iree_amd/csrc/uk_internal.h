@@ -48,6 +48,67 @@ struct UnpackArgs {
   int elem_bytes;
 };
 
+// Element types of a matrix next to microscaled operands, in the order of the type flags.
+enum class Float { kF32 = 0, kF16 = 1, kBf16 = 2 };
+inline int float_bytes(Float t) { return t == Float::kF32 ? 4 : 2; }
+
+// Microscaled operands: codes of 4 or 8 bits, tiled [outer0][outer1][tile0][tile1] with panels `stride0` BYTES apart, and
+// their scales, one byte for each 32 codes of a tile's row, in panels scales_stride0 bytes apart.
+struct MxPackArgs {
+  const uint8_t* in;
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t in_stride0, in_stride1;  // elements
+  int64_t codes_stride0, scales_stride0;
+  int64_t in_size0, in_size1;
+  int64_t outer0, outer1, tile0, tile1;
+  Float type;
+  int bits;  // 4 or 8
+};
+
+struct MxUnpackArgs {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  uint8_t* out;
+  int64_t codes_stride0, scales_stride0;
+  int64_t out_stride0, out_stride1;  // elements
+  int64_t outer0, outer1, tile0, tile1;
+  int64_t out_size0, out_size1;
+  Float type;
+  int bits;
+};
+
+struct MxMmt4dArgs {
+  const uint8_t* lhs;
+  const uint8_t* lhs_scales;
+  const uint8_t* rhs;
+  const uint8_t* rhs_scales;
+  uint8_t* out;
+  int64_t lhs_stride0, lhs_scales_stride0, rhs_stride0, rhs_scales_stride0;  // bytes
+  int64_t out_stride0;                                                      // elements
+  int64_t M, N, K;
+  int32_t M0, N0, K0;
+  int lhs_bits;  // of the lhs: 4 or 8
+  Float out_type;
+  bool accumulate;
+};
+
+enum class NormOut { kS8 = 0, kE4M3 = 1, kE2M1 = 2 };
+struct RmsNormArgs {
+  const uint8_t* in;
+  const uint8_t* residual;  // or null
+  uint8_t* sum;             // or null
+  const uint8_t* weight;    // or null
+  uint8_t* out;
+  uint8_t* scales;
+  int64_t in_stride0, residual_stride0, sum_stride0;  // elements
+  int64_t out_stride0, scales_stride0;                // bytes
+  int64_t size0, size1, out_size1;
+  float epsilon;
+  Float type, weight_type;
+  NormOut out_type;
+};
+
 // Enqueues a kernel that takes one argument struct. (Half a hundred nanoseconds each of the triple-bracket form's
 // configuration stack and of hipGetLastError are left out: the call itself returns the launch's status.)
 template <typename Args>
@@ -91,6 +152,11 @@ hipError_t launch_mmt4d_generic(const Mmt4dArgs& a, hipStream_t stream, const ch
 
 hipError_t launch_pack(const PackArgs& a, hipStream_t stream, const char** name);
 hipError_t launch_unpack(const UnpackArgs& a, hipStream_t stream, const char** name);
+
+hipError_t launch_mx_pack(const MxPackArgs& a, hipStream_t stream, const char** name);
+hipError_t launch_mx_unpack(const MxUnpackArgs& a, hipStream_t stream, const char** name);
+hipError_t launch_mx_mmt4d(const MxMmt4dArgs& a, hipStream_t stream, const char** name);
+hipError_t launch_rms_norm(const RmsNormArgs& a, hipStream_t stream, const char** name);
 
 // Copies between pinned host memory and the device as kernels on the stream (host_copy.hip), 16 bytes at a time: both
 // sides are 16-byte aligned and may be touched up to the next multiple of 16 bytes. A download sets flag b to

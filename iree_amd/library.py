@@ -50,6 +50,10 @@ def load():
     l.iree_uk_query_tile_sizes_2d.argtypes = [C.POINTER(abi.QueryTileSizes2dParams),
                                               C.POINTER(abi.QueryTileSizes2dOutParams)]
     l.iree_uk_query_tile_sizes_2d.restype = None
+    for name, params in (("mx_pack", abi.MxPackParams), ("mx_unpack", abi.MxUnpackParams),
+                         ("mx_mmt4d", abi.MxMmt4dParams), ("rms_norm", abi.RmsNormParams)):
+        entry = getattr(l, "iree_uk_mi355x_%s_p" % name)
+        entry.argtypes, entry.restype = [C.POINTER(params)], None
     l.iree_uk_mi355x_version.restype = C.c_int
     l.iree_uk_mi355x_multi_mma_i32_16x16x64_i8.argtypes = [vp, vp, vp, C.c_longlong, C.c_longlong] + [C.c_int32] * 6
     l.iree_uk_mi355x_multi_mma_i32_16x16x64_i8.restype = C.c_int
