@@ -2,7 +2,7 @@
 // every tile shape, stride and alignment.
 #include <type_traits>
 
-#include "mx_device.h"
+#include "mx_mmt4d.h"
 
 namespace uk {
 namespace {
@@ -71,9 +71,47 @@ hipError_t launch_generic(const MxMmt4dArgs& a, hipStream_t stream, const char**
                          : launch_kernel(mx_mmt4d_generic<8>, grid, kThreads, 0, stream, g);
 }
 
+// Whether a row of an operand's tiles has its K in chunks of 128 that lie a tile apart.
+bool in_chunks(int32_t tile_rows, int32_t k0) { return tile_rows == 1 || k0 == 128; }
+
+bool aligned(const void* p, int64_t stride, int64_t rows, int64_t to) {
+  return (uintptr_t)p % to == 0 && (rows == 1 || stride % to == 0);
+}
+
+// The problem as the fast kernels take it; false: they do not.
+bool as_product(const MxMmt4dArgs& a, MxProduct* p) {
+  const int64_t rows = a.M * a.M0, cols = a.N * a.N0, depth = a.K * a.K0;
+  if (depth == 0 || depth % 128 != 0 || depth / 128 > 0x7FFFFFFF || !in_chunks(a.M0, a.K0) || !in_chunks(a.N0, a.K0)) return false;
+  if (rows > 0x7FFFFFFF - 256 || cols > 0x7FFFFFFF - 256) return false;
+  if (!aligned(a.lhs, a.lhs_stride0, a.M, 16) || !aligned(a.rhs, a.rhs_stride0, a.N, 16) ||
+      !aligned(a.lhs_scales, a.lhs_scales_stride0, a.M, 4) || !aligned(a.rhs_scales, a.rhs_scales_stride0, a.N, 4))
+    return false;
+  const int out_bytes = float_bytes(a.out_type);
+  p->lhs = {a.lhs, a.lhs_scales, a.lhs_stride0, a.lhs_scales_stride0, (uint32_t)rows, (uint32_t)a.M0, reciprocal_of((uint32_t)a.M0)};
+  p->rhs = {a.rhs, a.rhs_scales, a.rhs_stride0, a.rhs_scales_stride0, (uint32_t)cols, (uint32_t)a.N0, reciprocal_of((uint32_t)a.N0)};
+  p->out = a.out;
+  p->out_stride0 = a.out_stride0;
+  p->chunks = (uint32_t)(depth / 128);
+  p->n0 = (uint32_t)a.N0;
+  p->n0_reciprocal = reciprocal_of((uint32_t)a.N0);
+  p->out_tile = (uint32_t)a.M0 * (uint32_t)a.N0;
+  p->out_type = a.out_type;
+  p->accumulate = a.accumulate;
+  // (Tiles one row tall and one column wide are a row-major result.)
+  if (a.M0 == 1 && a.N0 == 1) {
+    p->n0 = p->rhs.rows;
+    p->n0_reciprocal = reciprocal_of(p->n0);
+    p->out_tile = 0;
+  }
+  p->fours = (p->n0 % 4 == 0 || (a.M0 == 1 && a.N0 == 1)) && aligned(a.out, a.out_stride0 * out_bytes, a.M, 4 * out_bytes);
+  return true;
+}
+
 }  // namespace
 
 hipError_t launch_mx_mmt4d(const MxMmt4dArgs& a, hipStream_t stream, const char** name) {
+  MxProduct p;
+  if (as_product(a, &p)) return launch_mx_few(p, a.lhs_bits, stream, name);
   return launch_generic(a, stream, name);
 }
 

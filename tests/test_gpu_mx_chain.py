@@ -61,9 +61,11 @@ class Layer:
         want = lhs @ rhs.T
         got = ref.from_raw(host(self.out).view(np.float32 if self.out_type == "f32" else np.uint16), self.out_type)
         got = got.reshape(self.m, self.np).astype(np.float64)
-        # The summation (at most K additions, each off by a unit in the last place of a partial sum) and half a step of the
+        # The summation (at most K additions, each off by a unit in the last place of a partial sum; 16-bit results of 8-bit
+        # codes: of eight products, seven lose what lies 13 bits below the largest one's exponent) and half a step of the
         # result's type.
-        bound = self.kp * 2.0 ** -23 * (np.abs(lhs) @ np.abs(rhs).T)
+        loss = 7 * 2.0 ** -13 if self.lhs_format == "e4m3" and self.out_type != "f32" else 0
+        bound = (self.kp * 2.0 ** -23 + loss) * (np.abs(lhs) @ np.abs(rhs).T)
         bound += {"f32": 0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[self.out_type] * (np.abs(want) + bound) + 2.0 ** -25
         assert (np.abs(got - want) <= bound).all()
 
