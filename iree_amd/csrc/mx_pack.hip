@@ -61,6 +61,8 @@ struct MxPackKernelArgs {
   uint8_t* codes;
   uint8_t* scales;
   int64_t in_stride0, in_stride1, in_size0, in_size1;
+  // mx_pack_transposed: rows and blocks of a row, padded; workgroups' rows.
+  uint32_t rows, blocks, down, down_reciprocal, row_blocks_reciprocal;
 };
 
 template <typename INDEX>
@@ -71,6 +73,21 @@ struct MxUnpackKernelArgs {
   uint8_t* out;
   int64_t out_stride0, out_stride1, out_size0, out_size1;
 };
+
+// A whole block: its scale byte, and its codes.
+template <int BITS, Float T>
+__device__ __forceinline__ uint32_t mx_block(const MxEight<T> (&v)[4], uint32_t codes[BITS]) {
+  uint32_t largest = 0;
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    const uint32_t m = mx_largest<T>(v[h]);
+    largest = m > largest ? m : largest;
+  }
+  const uint32_t b = mx_scale_byte<BITS>(largest);
+#pragma unroll
+  for (int h = 0; h < 4; ++h) mx_codes<BITS, T>(v[h], b, codes + h * (BITS / 4));
+  return b;
+}
 
 // Rows whose values are next to each other (in_stride1 == 1).
 template <Float T, int BITS, int AT_ONCE, typename INDEX>
@@ -98,74 +115,171 @@ __global__ __launch_bounds__(kThreads) void mx_pack_rows(const MxPackKernelArgs<
   }
 }
 
-// Any strides: a lane takes a whole block and neighbouring lanes neighbouring rows, whose values are next to each other in
-// a transposed matrix. Block number n: rows fastest.
+// Any strides: a lane takes a whole block and neighbouring lanes neighbouring rows, whose values are next to each other in a
+// transposed matrix. A wavefront takes 64 rows and the four of a workgroup four blocks of them that follow each other, so that
+// the codes of a row that share a cache line are written together.
 template <Float T, int BITS>
 __global__ __launch_bounds__(kThreads) void mx_pack_strided(const MxPackKernelArgs<uint64_t> a) {
   constexpr int SIZE = T == Float::kF32 ? 4 : 2;
   const MxShape<uint64_t>& s = a.shape;
-  const uint64_t rows = s.segments / (s.outer1 * s.row_segments), blocks = s.segments / 4;
-  for (uint64_t n = (uint64_t)blockIdx.x * kThreads + threadIdx.x; n < blocks; n += (uint64_t)gridDim.x * kThreads) {
-    const uint64_t row = n % rows, block = n / rows;
-    const uint64_t o0 = row / s.tile0, t0 = row % s.tile0, o1 = block / (s.row_segments / 4), in_row = block % (s.row_segments / 4);
-    MxEight<T> v[4];
-    uint32_t largest = 0;
+  const uint64_t row_blocks = s.row_segments / 4, blocks = s.outer1 * row_blocks, rows = s.segments / (4 * blocks);
+  const uint64_t down = (rows + 63) / 64, across = (blocks + 3) / 4;
+  for (uint64_t n = blockIdx.x; n < down * across; n += gridDim.x) {
+    const uint64_t row = n % down * 64 + threadIdx.x % 64, block = n / down * 4 + threadIdx.x / 64;
+    if (row >= rows || block >= blocks) continue;
+    const uint64_t o0 = row / s.tile0, t0 = row - o0 * s.tile0, o1 = block / row_blocks, in_row = block - o1 * row_blocks;
+    const int64_t left = (int64_t)row < a.in_size0 ? a.in_size1 - (int64_t)block * 32 : 0;
+    const uint8_t* const from = a.in + ((int64_t)row * a.in_stride0 + (int64_t)block * 32 * a.in_stride1) * SIZE;
+    const int64_t step = a.in_stride1 * SIZE;
+    uint32_t x[32];
+    if (left >= 32) {
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
+      for (int i = 0; i < 32; ++i) x[i] = SIZE == 4 ? *(const uint32_t*)(from + i * step) : *(const uint16_t*)(from + i * step);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t col = (int64_t)block * 32 + h * 8 + i;
-        const bool there = (int64_t)row < a.in_size0 && col < a.in_size1;
-        const uint8_t* at = a.in + ((int64_t)row * a.in_stride0 + col * a.in_stride1) * SIZE;
-        if constexpr (T == Float::kF32) {
-          v[h].w[i] = there ? *(const uint32_t*)at : 0;
-        } else {
-          const uint32_t x = there ? *(const uint16_t*)at : 0;
-          v[h].w[i / 2] = i & 1 ? v[h].w[i / 2] | x << 16 : x;
-        }
-      }
-      const uint32_t m = mx_largest<T>(v[h]);
-      largest = m > largest ? m : largest;
+      for (int i = 0; i < 32; ++i)
+        x[i] = i >= left ? 0u : SIZE == 4 ? *(const uint32_t*)(from + i * step) : *(const uint16_t*)(from + i * step);
     }
-    const uint32_t b = mx_scale_byte<BITS>(largest);
-    uint32_t codes[BITS];
+    MxEight<T> v[4];
 #pragma unroll
-    for (int h = 0; h < 4; ++h) mx_codes<BITS, T>(v[h], b, codes + h * (BITS / 4));
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int i = 0; i < MxEight<T>::kWords; ++i)
+        v[h].w[i] = SIZE == 4 ? x[8 * h + i] : x[8 * h + 2 * i] | x[8 * h + 2 * i + 1] << 16;
+    uint32_t codes[BITS];
+    const uint32_t b = mx_block<BITS, T>(v, codes);
     const int64_t in_panel = (int64_t)((o1 * s.tile0 + t0) * s.row_segments + in_row * 4);
     __builtin_memcpy(a.codes + (int64_t)o0 * s.codes_stride0 + in_panel * BITS, codes, 4 * BITS);
     a.scales[(int64_t)o0 * s.scales_stride0 + in_panel / 4] = (uint8_t)b;
   }
 }
 
+// A transposed matrix (in_stride0 == 1) whose columns and their distance are multiples of 16 bytes: 128 of K of 64 rows (128 of a
+// 16-bit type) go straight to LDS, 16 bytes a lane along the rows, and lanes take whole blocks out of it, a word (one value, or
+// two neighbouring rows' values) at a time, 64 of them next to each other. Codes go out through LDS too, 16 bytes a lane in the
+// order of the tile. 14336 x 4096 f32 to E2M1: a lane loading its own block 72.5 us.
+template <Float T, int BITS>
+__global__ __launch_bounds__(kThreads) void mx_pack_transposed(const MxPackKernelArgs<uint32_t> a) {
+  constexpr int SIZE = T == Float::kF32 ? 4 : 2, AT_ONCE = 4 / SIZE, ROWS = 64 * AT_ONCE;  // rows of a lane, of a workgroup
+  constexpr int LOADS = 128 * 256 / (kThreads * 16), PIECES = BITS / 4;                     // of a lane; 16 bytes of a block's codes
+  __shared__ uint4 values[128 * 16];                                                      // [k][ROWS]: 256 bytes each
+  __shared__ uint32_t scales[ROWS];
+  const MxShape<uint32_t>& s = a.shape;
+  const uint32_t row_blocks = s.row_segments / 4;
+  const uint32_t rows = a.rows, blocks = a.blocks, down = a.down;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t group = divide(blockIdx.x, down, a.down_reciprocal);
+  const uint32_t first_row = (blockIdx.x - group * down) * ROWS, first_block = group * 4;
+  const int64_t k0 = (int64_t)first_block * 32;
+
+  // Load n of a wavefront: K (n * 4 + wave) * 4 + lane / 16, 16 lanes for the 256 bytes of its rows.
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)values;
+  const int64_t load_row = first_row + (lane & 15) * (16 / SIZE);
+#pragma unroll
+  for (int n = 0; n < LOADS; ++n) {
+    const int k = (n * 4 + wave) * 4 + (lane >> 4);
+    if (load_row < a.in_size0 && k0 + k < a.in_size1) {
+      const uint8_t* const from = a.in + ((k0 + k) * a.in_stride1 + load_row) * SIZE;
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds + (n * 4 + wave) * 1024), "v"(from) : "memory");
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+
+  // A wavefront's block: words [k][lane].
+  const uint32_t* const words = (const uint32_t*)values + (wave * 32) * 64 + lane;
+  const int64_t left = a.in_size1 - k0 - wave * 32;
+  uint32_t x[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) x[i] = words[i * 64];
+  if (left < 32) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = i < left ? x[i] : 0;
+  }
+  if (first_row + lane * AT_ONCE >= a.in_size0) {  // (rows come in whole loads)
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = 0;
+  }
+  uint32_t codes[AT_ONCE][BITS], b[AT_ONCE];
+#pragma unroll
+  for (int t = 0; t < AT_ONCE; ++t) {
+    MxEight<T> v[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int i = 0; i < MxEight<T>::kWords; ++i)
+        v[h].w[i] = SIZE == 4 ? x[8 * h + i] : __builtin_amdgcn_perm(x[8 * h + 2 * i + 1], x[8 * h + 2 * i], t == 0 ? 0x05040100 : 0x07060302);
+    b[t] = mx_block<BITS, T>(v, codes[t]);
+  }
+  __syncthreads();
+  // [row][block][piece], the pieces of a row exchanged among themselves by its number so that lanes write to different banks.
+  constexpr int ROW_PIECES = 4 * PIECES;
+#pragma unroll
+  for (int t = 0; t < AT_ONCE; ++t) {
+    const int row = lane * AT_ONCE + t;
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c) {
+      const int at = (wave * PIECES + c) ^ (row / AT_ONCE % ROW_PIECES);
+      values[row * ROW_PIECES + at] = make_uint4(codes[t][4 * c], codes[t][4 * c + 1], codes[t][4 * c + 2], codes[t][4 * c + 3]);
+    }
+    ((uint8_t*)scales)[row * 4 + wave] = (uint8_t)b[t];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = threadIdx.x; n < ROWS * ROW_PIECES; n += kThreads) {
+    const int row = n / ROW_PIECES, piece = n % ROW_PIECES, block = piece / PIECES;
+    const uint32_t r = first_row + row, k = first_block + block;
+    if (r >= rows || k >= blocks) continue;
+    const uint32_t o0 = divide(r, s.tile0, s.tile0_reciprocal), o1 = divide(k, row_blocks, a.row_blocks_reciprocal);
+    const int64_t in_panel = (int64_t)(o1 * (uint64_t)s.tile0 + (r - o0 * s.tile0)) * row_blocks + (k - o1 * row_blocks);
+    *(uint4*)(a.codes + (int64_t)o0 * s.codes_stride0 + in_panel * (4 * BITS) + piece % PIECES * 16) =
+        values[row * ROW_PIECES + (piece ^ (row / AT_ONCE % ROW_PIECES))];
+    if (piece % PIECES == 0) a.scales[(int64_t)o0 * s.scales_stride0 + in_panel] = ((const uint8_t*)scales)[row * 4 + block];
+  }
+}
+
+// A lane's values make 16 bytes of the result, eight of a 16-bit type or four of f32 (with eight, whose stores leave every other
+// 16 bytes to the next instruction, 14336 x 4096 E2M1 to f32 took 59.1 us).
 template <Float T, int BITS, int AT_ONCE, typename INDEX>
 __global__ __launch_bounds__(kThreads) void mx_unpack_rows(const MxUnpackKernelArgs<INDEX> a) {
-  constexpr int SIZE = T == Float::kF32 ? 4 : 2;
-  // (One turn, but for operands of 2^34 values and more.)
-  for (INDEX first = (INDEX)blockIdx.x * (kThreads * AT_ONCE) + threadIdx.x; first < a.shape.segments;
+  constexpr int SIZE = T == Float::kF32 ? 4 : 2, VALUES = 16 / SIZE, SHARES = 8 / VALUES;
+  const INDEX items = a.shape.segments * SHARES;
+  // (One turn, but for operands of 2^33 values and more.)
+  for (INDEX first = (INDEX)blockIdx.x * (kThreads * AT_ONCE) + threadIdx.x; first < items;
        first += (INDEX)gridDim.x * (kThreads * AT_ONCE)) {
-    uint32_t codes[AT_ONCE][BITS / 4], b[AT_ONCE];
+    uint32_t codes[AT_ONCE][2], b[AT_ONCE];
     MxPlace p[AT_ONCE];
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
       const INDEX n = first + (INDEX)(u * kThreads);
-      if (n >= a.shape.segments) break;
-      p[u] = mx_place<BITS>(a.shape, n);
-      __builtin_memcpy(codes[u], a.codes + p[u].code, BITS);
+      if (n >= items) break;
+      p[u] = mx_place<BITS>(a.shape, n / SHARES);
+      const int share = SHARES == 1 ? 0 : (int)(n % SHARES);
+      p[u].col += share * VALUES;
+      codes[u][0] = codes[u][1] = 0;
+      __builtin_memcpy(codes[u], a.codes + p[u].code + share * (VALUES * BITS / 8), VALUES * BITS / 8);
       b[u] = a.scales[p[u].scale];
     }
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
-      if (first + (INDEX)(u * kThreads) >= a.shape.segments) break;
-      const int64_t left = p[u].row < a.out_size0 ? a.out_size1 - p[u].col : 0;
+      if (first + (INDEX)(u * kThreads) >= items) break;
+      int64_t left = p[u].row < a.out_size0 ? a.out_size1 - p[u].col : 0;
       if (left <= 0) continue;
       float f[8];
       mx_values<BITS>(codes[u], b[u], f);
-      if (a.out_stride1 == 1) {
-        mx_store_eight<T>(a.out + (p[u].row * a.out_stride0 + p[u].col) * SIZE, f, left);
+      uint8_t* const at = a.out + (p[u].row * a.out_stride0 + p[u].col * a.out_stride1) * SIZE;
+      if (a.out_stride1 == 1 && left >= VALUES) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (T == Float::kF32) w[i] = __builtin_bit_cast(uint32_t, f[i]);
+          else w[i] = mx_narrow_pair<T>(f[2 * i], f[2 * i + 1]);
+        }
+        __builtin_memcpy(at, w, 16);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < left) mx_store_eight<T>(a.out + (p[u].row * a.out_stride0 + (p[u].col + i) * a.out_stride1) * SIZE, f + i, 1);
+        for (int i = 0; i < VALUES; ++i)
+          if (i < left) mx_store_eight<T>(at + i * a.out_stride1 * SIZE, f + i, 1);
       }
     }
   }
@@ -213,11 +327,29 @@ hipError_t pack(const MxPackArgs& a, hipStream_t stream, const char** name) {
     return launch_kernel(mx_pack_rows<T, BITS, 1, uint32_t>, (unsigned)((segments + kThreads - 1) / kThreads), kThreads, 0,
                          stream, k);
   }
+  constexpr int SIZE = T == Float::kF32 ? 4 : 2;
+  auto sixteens = [](int64_t bytes) { return bytes % 16 == 0; };
+  const int64_t rows = a.outer0 * a.tile0, blocks = a.outer1 * (a.tile1 / 32), fours = (blocks + 3) / 4;
+  const int64_t down = (rows + 256 / SIZE - 1) / (256 / SIZE);
+  if (a.in_stride0 == 1 && segments < (1ll << 31) && rows < (1ll << 31) - 256 && down * fours < (1ll << 23) &&
+      sixteens((int64_t)(uintptr_t)a.in) && sixteens(a.in_stride1 * SIZE) && sixteens(a.in_size0 * SIZE) &&
+      sixteens((int64_t)(uintptr_t)a.codes) && sixteens(a.codes_stride0)) {
+    MxPackKernelArgs<uint32_t> k;
+    k.shape = mx_shape<uint32_t>(a.outer0, a.outer1, a.tile0, a.tile1, a.codes_stride0, a.scales_stride0);
+    fill(k);
+    k.rows = (uint32_t)rows;
+    k.blocks = (uint32_t)blocks;
+    k.down = (uint32_t)down;
+    k.down_reciprocal = reciprocal_of(k.down);
+    k.row_blocks_reciprocal = reciprocal_of((uint32_t)(a.tile1 / 32));
+    *name = "mx_pack_transposed";
+    return launch_kernel(mx_pack_transposed<T, BITS>, (unsigned)(down * fours), kThreads, 0, stream, k);
+  }
   MxPackKernelArgs<uint64_t> k;
   k.shape = mx_shape<uint64_t>(a.outer0, a.outer1, a.tile0, a.tile1, a.codes_stride0, a.scales_stride0);
   fill(k);
   *name = "mx_pack_strided";
-  const int64_t groups = (segments / 4 + kThreads - 1) / kThreads;
+  const int64_t groups = (rows + 63) / 64 * fours;
   return launch_kernel(mx_pack_strided<T, BITS>, (unsigned)(groups < (1 << 22) ? groups : 1 << 22), kThreads, 0, stream, k);
 }
 
@@ -235,15 +367,15 @@ hipError_t unpack(const MxUnpackArgs& given, hipStream_t stream, const char** na
   };
   *name = "mx_unpack_rows";
   constexpr int MANY = 4;
-  const unsigned groups = (unsigned)((segments + kThreads - 1) / kThreads);
-  if (segments < (1ll << 31)) {
+  const int64_t items = segments * (T == Float::kF32 ? 2 : 1);
+  if (items < (1ll << 31)) {
     MxUnpackKernelArgs<uint32_t> k;
     k.shape = mx_shape<uint32_t>(a.outer0, a.outer1, a.tile0, a.tile1, a.codes_stride0, a.scales_stride0);
     fill(k);
-    if (segments >= (int64_t)MANY * kThreads * 1024)
-      return launch_kernel(mx_unpack_rows<T, BITS, MANY, uint32_t>,
-                           (unsigned)((segments + MANY * kThreads - 1) / (MANY * kThreads)), kThreads, 0, stream, k);
-    return launch_kernel(mx_unpack_rows<T, BITS, 1, uint32_t>, groups, kThreads, 0, stream, k);
+    if (items >= (int64_t)MANY * kThreads * 1024)
+      return launch_kernel(mx_unpack_rows<T, BITS, MANY, uint32_t>, (unsigned)((items + MANY * kThreads - 1) / (MANY * kThreads)),
+                           kThreads, 0, stream, k);
+    return launch_kernel(mx_unpack_rows<T, BITS, 1, uint32_t>, (unsigned)((items + kThreads - 1) / kThreads), kThreads, 0, stream, k);
   }
   MxUnpackKernelArgs<uint64_t> k;
   k.shape = mx_shape<uint64_t>(a.outer0, a.outer1, a.tile0, a.tile1, a.codes_stride0, a.scales_stride0);

@@ -132,6 +132,30 @@ def test_pack_strides(gpu_lib, type, format, rows, cols, t0, t1, strides):
     np.testing.assert_array_equal(host(scales), expect)
 
 
+@pytest.mark.parametrize("format", ["e2m1", "e4m3"])
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols,t0,t1,pitch,row_offset", [
+    (8, 1, 16, 128, 8, 0), (64, 128, 16, 128, 64, 0), (200, 300, 16, 128, 200, 0), (136, 129, 1, 32, 144, 0),
+    (512, 257, 7, 96, 520, 8), (72, 1000, 16, 64, 80, 0), (1032, 40, 32, 128, 1032, 0)])
+def test_pack_transposed(gpu_lib, type, format, rows, cols, t0, t1, pitch, row_offset):
+    # Columns of whole 16 bytes, as many as a workgroup takes, fewer and more; specials among the values.
+    rng = np.random.default_rng(rows + cols)
+    flat = ref.to_type(rng.standard_normal(row_offset + (cols - 1) * pitch + rows) * 2.0 ** rng.integers(-9, 9), type)
+    flat[rng.integers(0, flat.size, 2)] = [np.nan, -np.inf]
+    x = flat[row_offset + np.arange(rows)[:, None] + np.arange(cols)[None] * pitch]
+    src = on_device(ref.raw(flat, type))
+    n = ref.up(rows, t0) * ref.up(cols, t1)
+    codes, scales = guarded(n * ref.BITS[format] // 8), guarded(n // 32)
+    p = ref.pack_params(src.data_ptr(), rows, cols, codes.data_ptr(), scales.data_ptr(), t0, t1, type, format, (1, pitch))
+    p.in_offset = row_offset
+    gpu_lib.iree_uk_mi355x_mx_pack_p(C.byref(p))
+    assert gpu_lib.iree_uk_mi355x_last_kernel() == b"mx_pack_transposed"
+    want = wanted(x, format, t0, t1)
+    np.testing.assert_array_equal(host(scales)[:-64], want[1])
+    np.testing.assert_array_equal(host(codes)[:-64], want[0])
+    assert (host(codes)[-64:] == GUARD).all() and (host(scales)[-64:] == GUARD).all()
+
+
 def test_pack_without_input_is_all_padding(gpu_lib):
     codes, scales = guarded(2 * 64 // 2), guarded(2 * 2)
     src = torch.zeros(1, device="cuda")
