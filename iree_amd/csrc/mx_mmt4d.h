@@ -33,23 +33,27 @@ struct MxProduct {
   uint32_t tile_rows, tile_cols, band_reciprocal;  // grid of a block kernel's tiles
 };
 
-// The kernels for few rows (mx_mmt4d_few.hip): fragments of 16 rows of the lhs and of the rhs that a workgroup multiplies.
+// The kernels for few rows (mx_mmt4d_few.hip): fragments of 16 rows of the lhs and of the rhs that a workgroup multiplies, and
+// whether the lhs goes through LDS.
 struct MxFewShape {
   int mt, nt;
+  bool staged;
   const char* name;
 };
-constexpr MxFewShape kMxFewShapes[] = {{1, 1, "mx_mmt4d_few_16x16"}, {1, 2, "mx_mmt4d_few_16x32"}, {1, 4, "mx_mmt4d_few_16x64"},
-                                       {2, 1, "mx_mmt4d_few_32x16"}, {2, 2, "mx_mmt4d_few_32x32"}, {2, 4, "mx_mmt4d_few_32x64"},
-                                       {4, 4, "mx_mmt4d_few_64x64"}};
+constexpr MxFewShape kMxFewShapes[] = {
+    {1, 1, false, "mx_mmt4d_few_16x16"}, {1, 2, false, "mx_mmt4d_few_16x32"}, {1, 4, false, "mx_mmt4d_few_16x64"},
+    {1, 1, true, "mx_mmt4d_few_16x16_staged"}, {1, 2, true, "mx_mmt4d_few_16x32_staged"},
+    {1, 4, true, "mx_mmt4d_few_16x64_staged"}, {2, 1, true, "mx_mmt4d_few_32x16_staged"},
+    {2, 2, true, "mx_mmt4d_few_32x32_staged"}, {2, 4, true, "mx_mmt4d_few_32x64_staged"}};
 // The block kernels (mx_mmt4d_block.h): fragments of 64 rows and columns of a workgroup's tile.
 struct MxBlockTile {
   int am, bn;
   const char* name;
 };
-constexpr MxBlockTile kMxBlockTiles[] = {{4, 4, "mx_mmt4d_block_256x256"}, {4, 2, "mx_mmt4d_block_256x128"},
-                                         {2, 2, "mx_mmt4d_block_128x128"}, {2, 3, "mx_mmt4d_block_128x192"},
-                                         {2, 4, "mx_mmt4d_block_128x256"}, {1, 1, "mx_mmt4d_block_64x64"},
-                                         {2, 1, "mx_mmt4d_block_128x64"},  {1, 2, "mx_mmt4d_block_64x128"}};
+constexpr MxBlockTile kMxBlockTiles[] = {{4, 4, "mx_mmt4d_block_256x256"}, {2, 2, "mx_mmt4d_block_128x128"},
+                                         {2, 3, "mx_mmt4d_block_128x192"}, {2, 4, "mx_mmt4d_block_128x256"},
+                                         {1, 1, "mx_mmt4d_block_64x64"},   {2, 1, "mx_mmt4d_block_128x64"},
+                                         {1, 2, "mx_mmt4d_block_64x128"}};
 hipError_t launch_mx_few(const MxProduct& p, int lhs_bits, int shape, hipStream_t stream);
 hipError_t launch_mx_block_e2m1(const MxProduct& p, int tile, hipStream_t stream);
 hipError_t launch_mx_block_e4m3(const MxProduct& p, int tile, hipStream_t stream);

@@ -107,17 +107,17 @@ bool as_product(const MxMmt4dArgs& a, MxProduct* p) {
   return true;
 }
 
+// Whether rows up to 256 apart lie within 32 bits of each other.
+bool near(const MxOperand& o) {
+  const int64_t panels = 256 / o.tile_rows + 2, most = 1ll << 31;
+  return o.stride0 < most / panels && o.scales_stride0 < most / panels;
+}
+
 // Whether the block kernels' 32-bit offsets inside a tile, and their stores of eight rows at a time, take the problem.
 bool block_covers(const MxProduct& p) {
-  const uint32_t m0 = p.lhs.tile_rows, n0 = p.rhs.tile_rows;
+  const uint32_t m0 = p.lhs.tile_rows;
   if (m0 != 1 && m0 % 8 != 0) return false;
-  auto spans = [](const MxOperand& o) {
-    const int64_t panels = 256 / o.tile_rows + 2, most = 1ll << 31;
-    return o.stride0 < most / panels && o.scales_stride0 < most / panels;
-  };
-  const int64_t tiles_across = 256 / p.n0 + 2;
-  return spans(p.lhs) && spans(p.rhs) && (m0 > 1 || p.out_stride0 < (1ll << 26)) && p.out_tile < (1ll << 28) / tiles_across &&
-         m0 < (1u << 15) && n0 < (1u << 15);
+  return near(p.lhs) && near(p.rhs) && (m0 > 1 || p.out_stride0 < (1ll << 26)) && p.out_tile < (1ll << 28) / (256 / p.n0 + 2);
 }
 
 // Which kernel: the least of the times that a model gives, in microseconds.
@@ -126,38 +126,42 @@ bool block_covers(const MxProduct& p) {
 // registers hold two, with two; more workgroups than that follow each other. From the times of every tile with 128 to 1024 of
 // them, row-major lhs, K = 1024 and 5120.
 //
-// Few rows: a workgroup's loads are what takes time, 16 rows in a cache line each 31 ns a KiB, 4-bit rows of a tile, or one row,
-// 13.5, and what mx_split takes; or the rhs from memory at 5.8 TB/s; whichever is more, and a
-// part of the other. More workgroups than compute units: what a workgroup begins and ends with, again.
+// Few rows: a workgroup's loads and its matrix instructions, or the rhs from memory at 6.5 TB/s, whichever is more, and a part of
+// the other. A chunk's sixteen rows straight into registers take 8 to 14 ns a KiB where lanes lie next to each other or have one
+// row, 25 with a cache line each; through LDS 18 (4 bits) and 12 (8 bits). Fitted to the times of every shape in 440 problems.
+//
+// Over these, drawn from 1 to 4096 rows, 64 to 28672 columns, K of 64 to 14336, with tiles and row-major, the kernel taken is
+// slower than the best one by 2 % in the mean.
 struct Choice {
   bool block;
   int number;
 };
 Choice choose(const MxProduct& p, int lhs_bits) {
   struct Times { float start, one, two, start_again; };
-  static const Times kE2m1[] = {{12.1f, .898f, 1.731f, 11}, {7.4f, .569f, 1.153f, 5}, {4.9f, .344f, .639f, 2.2f}, {5.8f, .444f, .817f, 2.7f},
+  static const Times kE2m1[] = {{12.1f, .898f, 1.731f, 11}, {4.9f, .344f, .639f, 2.2f}, {5.8f, .444f, .817f, 2.7f},
                                 {7.6f, .531f, 1.093f, 5}, {3.4f, .219f, .333f, 1}, {3.8f, .271f, .499f, 1.3f}, {3.9f, .265f, .457f, 1.4f}};
-  static const Times kE4m3[] = {{12, 1.247f, 2.494f, 9.5f}, {7.6f, .797f, 1.533f, 5.3f}, {4.6f, .441f, .813f, 2.5f}, {6.2f, .565f, 1.155f, 4},
+  static const Times kE4m3[] = {{12, 1.247f, 2.494f, 9.5f}, {4.6f, .441f, .813f, 2.5f}, {6.2f, .565f, 1.155f, 4},
                                 {8, .710f, 1.456f, 5.7f}, {3.5f, .247f, .396f, 1}, {3.9f, .315f, .572f, 1.1f}, {3.9f, .288f, .501f, 1.3f}};
-  static const Times kE4m3F32[] = {{14.4f, 2.67f, 5.42f, 11}, {9.8f, 1.714f, 3.403f, 6}, {6.6f, .929f, 1.544f, 2}, {7.5f, 1.169f, 2.339f, 4},
+  static const Times kE4m3F32[] = {{14.4f, 2.67f, 5.42f, 11}, {6.6f, .929f, 1.544f, 2}, {7.5f, 1.169f, 2.339f, 4},
                                    {10.1f, 1.396f, 2.846f, 5}, {3.6f, .488f, .65f, 1}, {4.5f, .732f, 1.071f, 1.9f}, {4.5f, .537f, .871f, 1.4f}};
   const Times* times = lhs_bits == 4 ? kE2m1 : p.out_type == Float::kF32 ? kE4m3F32 : kE4m3;
   const int64_t rows = p.lhs.rows, cols = p.rhs.rows;
   Choice best = {false, 0};
   float least = 0;
   const float lines = p.lhs.tile_rows >= 16 && lhs_bits == 4 ? 0 : (float)(rows < 16 ? rows - 1 : 15) / 15;
-  const float lhs_chunk = (lhs_bits == 8 ? 2 : 1) * (.0135f + .0175f * lines) + (times == kE4m3F32 ? .03f : 0);
-  const float rhs_chunk = p.rhs.tile_rows >= 16 ? .0135f : .031f;
-  const float memory = (float)cols * p.chunks * 68e-6f / 5.8f;
+  const bool eight = lhs_bits == 8, split = times == kE4m3F32, lhs_near = near(p.lhs);
+  const float lhs_direct = (eight ? 2 : 1) * (.008f + .0165f * lines) + (split ? .008f : 0), lhs_staged = eight ? .024f : .018f;
+  const float rhs_chunk = p.rhs.tile_rows >= 16 ? .014f : .026f, product = split ? .008f : .0016f;
+  const float memory = (float)cols * p.chunks * 68e-6f;
   for (int i = 0; i < (int)(sizeof kMxFewShapes / sizeof kMxFewShapes[0]); ++i) {
     const MxFewShape& s = kMxFewShapes[i];
     const int64_t down = (rows + 16 * s.mt - 1) / (16 * s.mt), across = (cols + 16 * s.nt - 1) / (16 * s.nt);
-    if (down > 65535 || (lhs_bits == 8 && s.mt == 4)) continue;
-    const float rounds = (float)((down * across + 255) / 256);
-    const float loads = rounds * p.chunks * (s.mt * lhs_chunk + s.nt * rhs_chunk);
-    const float streamed = down * across < 448 ? 1.12f * memory : memory;
-    const float cost = 2.3f + (rounds - 1) * (.3f + .2f * s.mt * s.nt) + (loads > streamed ? loads + .25f * streamed : streamed + .25f * loads);
-    if (i == 0 || cost < least) {
+    if (down > 65535 || (s.staged && !lhs_near)) continue;
+    const float rounds = (float)((down * across + 255) / 256), start = 1.95f + .27f * s.mt * s.nt;
+    const float loads = rounds * p.chunks * (s.mt * (s.staged ? lhs_staged : lhs_direct) + s.nt * rhs_chunk + s.mt * s.nt * product);
+    const float streamed = memory / (down * across < 448 ? 5.8f : 6.5f);
+    const float cost = start + (rounds - 1) * .37f * start + (loads > streamed ? loads + .13f * streamed : streamed + .13f * loads);
+    if (least == 0 || cost < least) {
       least = cost;
       best.number = i;
     }
@@ -168,7 +172,8 @@ Choice choose(const MxProduct& p, int lhs_bits) {
     const int64_t tiles = ((rows + 64 * t.am - 1) / (64 * t.am)) * ((cols + 64 * t.bn - 1) / (64 * t.bn)), rounds = (tiles + 255) / 256;
     if (tiles > (1 << 23)) continue;
     const float steps = p.chunks * ((rounds >> 1) * times[i].two + (rounds & 1) * times[i].one);
-    const float cost = times[i].start + (rounds - 1) * times[i].start_again + (steps > memory ? steps : memory) + .15f * memory;
+    const float streamed = memory / 5.8f;
+    const float cost = times[i].start + (rounds - 1) * times[i].start_again + (steps > streamed ? steps : streamed) + .15f * streamed;
     if (cost < least) {
       least = cost;
       best = {true, i};

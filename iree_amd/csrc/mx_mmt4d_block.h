@@ -399,13 +399,12 @@ hipError_t launch_block(const MxProduct& p, int tile, hipStream_t stream) {
   constexpr bool FOUR = LBITS == 4;
   switch (tile) {  // kMxBlockTiles
     case 0: return launch<LBITS, SPLIT, 4, 4, FOUR ? 4 : 3>(p, stream);
-    case 1: return launch<LBITS, SPLIT, 4, 2, 3>(p, stream);
-    case 2: return launch<LBITS, SPLIT, 2, 2, FOUR ? 4 : 3>(p, stream);
-    case 3: return launch<LBITS, SPLIT, 2, 3, 3>(p, stream);
-    case 4: return launch<LBITS, SPLIT, 2, 4, FOUR ? 3 : 4>(p, stream);
-    case 5: return launch<LBITS, SPLIT, 1, 1, FOUR ? 6 : 5>(p, stream);
-    case 6: return launch<LBITS, SPLIT, 2, 1, FOUR ? 5 : 3>(p, stream);
-    case 7: return launch<LBITS, SPLIT, 1, 2, FOUR ? 5 : 4>(p, stream);
+    case 1: return launch<LBITS, SPLIT, 2, 2, FOUR ? 4 : 3>(p, stream);
+    case 2: return launch<LBITS, SPLIT, 2, 3, 3>(p, stream);
+    case 3: return launch<LBITS, SPLIT, 2, 4, FOUR ? 3 : 4>(p, stream);
+    case 4: return launch<LBITS, SPLIT, 1, 1, FOUR ? 6 : 5>(p, stream);
+    case 5: return launch<LBITS, SPLIT, 2, 1, FOUR ? 5 : 3>(p, stream);
+    case 6: return launch<LBITS, SPLIT, 1, 2, FOUR ? 5 : 4>(p, stream);
   }
   return hipErrorInvalidValue;
 }

@@ -18,15 +18,34 @@ __device__ __forceinline__ uint32_t scales_of_blocks(uint32_t loaded, int g) {
   return __builtin_amdgcn_perm(low[1], low[0], pick) | __builtin_amdgcn_perm(high[1], high[0], pick) << 16;
 }
 
+constexpr int kWaves = 8;
+
+extern __shared__ uint4 few_lds[];
+
+__device__ __forceinline__ void load_pieces(uint32_t lds, uint32_t offset, const uint8_t* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+// At most the last N loads of the wavefront are still under way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 // A workgroup multiplies 16 * MT rows of the lhs with 16 * NT of the rhs; its wavefronts take four chunks of 128 of K in turn, and
-// add their sums through LDS in the order of their numbers. A chunk's registers are loaded again as soon as it is multiplied.
-// Rows beyond the last are read as the last one and not stored.
-template <int LBITS, int MT, int NT, int WAVES, bool STREAM, bool SPLIT>
-__global__ __launch_bounds__(64 * WAVES) void mx_mmt4d_few_kernel(const MxProduct p) {
-  __shared__ mx_v4f32 partial[WAVES][MT * NT][64];
+// add their sums through LDS in the order of their numbers. A chunk is loaded again as soon as it is multiplied. Rows beyond
+// the last are read as the last one and not stored.
+//
+// STAGED: the lhs goes through LDS, a wavefront's own part of it, where a row's pieces are exchanged among themselves for the
+// banks' sake. Straight into registers a load's neighbouring lanes have 16 rows, 16 cache lines, and take 31 ns a KiB; to LDS
+// eight (sixteen) neighbouring lanes have one row: 8.5 ns. Against the same shapes without: 32 rows x 4096 columns x 14336 in
+// 8.8 us (4-bit lhs; 12.4 at best), 128 x 4096 x 4096 in 7.2 (8.5; 8-bit 8.4, 11.3), 128 x 4096 x 14336 in 15.1 (22.8).
+template <int LBITS, int MT, int NT, bool STREAM, bool SPLIT, bool STAGED>
+__global__ __launch_bounds__(64 * kWaves) void mx_mmt4d_few_kernel(const MxProduct p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   const uint32_t first_col = blockIdx.x * (16 * NT), first_row = blockIdx.y * (16 * MT);
+  constexpr int ROW = 16 * LBITS, PIECES = ROW / 16, ROWS_OF_LOAD = 64 / PIECES;  // bytes of a row's chunk
+  constexpr int CHUNK = MT * 16 * ROW, LOADS = CHUNK / 1024;                      // the lhs's, of a wavefront
 
   const uint8_t *rhs[NT], *rhs_scales[NT], *lhs[MT], *lhs_scales[MT];
 #pragma unroll
@@ -41,12 +60,29 @@ __global__ __launch_bounds__(64 * WAVES) void mx_mmt4d_few_kernel(const MxProduc
     lhs[i] = p.lhs.codes + mx_row_codes<LBITS>(p.lhs, row) + 16 * g;
     lhs_scales[i] = p.lhs.scales + mx_row_scales(p.lhs, row);
   }
-  const int64_t rhs_step = 64 * (int64_t)p.rhs.tile_rows, lhs_step = 16 * LBITS * (int64_t)p.lhs.tile_rows;
+  const int64_t rhs_step = 64 * (int64_t)p.rhs.tile_rows, lhs_step = ROW * (int64_t)p.lhs.tile_rows;
   const int64_t rhs_scales_step = 4 * (int64_t)p.rhs.tile_rows, lhs_scales_step = 4 * (int64_t)p.lhs.tile_rows;
+  // Staged: load n of a chunk has rows n * ROWS_OF_LOAD + lane / PIECES; a row's piece c lies at c ^ exchanged(row).
+  const uint32_t first_panel = divide(first_row, p.lhs.tile_rows, p.lhs.tile_reciprocal);
+  const uint8_t* const lhs_base = p.lhs.codes + (int64_t)first_panel * p.lhs.stride0;
+  uint32_t lhs_from[STAGED ? LOADS : 1];
+  auto exchanged = [](uint32_t row) { return LBITS == 4 ? ((row >> 2) & 3) ^ (row & 2) : ((row >> 1) & 7) ^ ((row & 1) << 2); };
+  if constexpr (STAGED) {
+#pragma unroll
+    for (int n = 0; n < LOADS; ++n) {
+      const uint32_t at = n * ROWS_OF_LOAD + lane / PIECES;
+      const uint32_t row = first_row + at < p.lhs.rows ? first_row + at : p.lhs.rows - 1;
+      const uint32_t panel = divide(row, p.lhs.tile_rows, p.lhs.tile_reciprocal);
+      lhs_from[n] = (uint32_t)((panel - first_panel) * p.lhs.stride0) + (row - panel * p.lhs.tile_rows) * ROW +
+                    16 * ((lane % PIECES) ^ exchanged(at));
+    }
+  }
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)few_lds + wave * (4 * CHUNK);
+  const uint8_t* const staged = (const uint8_t*)few_lds + wave * (4 * CHUNK) + r * ROW;
 
   mx_v4f32 acc[MT][NT] = {};
   MxFragment<4> b[4][NT];
-  MxFragment<LBITS> a[4][MT];
+  MxFragment<LBITS> a[STAGED ? 1 : 4][MT];
   uint32_t bs[NT], as[MT], b_loaded[NT], a_loaded[MT];
   auto load_scales = [&](uint32_t first) {
     const uint32_t chunk = first + g < p.chunks ? first + g : p.chunks - 1;
@@ -64,6 +100,10 @@ __global__ __launch_bounds__(64 * WAVES) void mx_mmt4d_few_kernel(const MxProduc
   auto load = [&](auto number, uint32_t first) {
     constexpr int U = decltype(number)::value;
     const uint32_t chunk = first + U < p.chunks ? first + U : p.chunks - 1;
+    if constexpr (STAGED) {
+#pragma unroll
+      for (int n = 0; n < LOADS; ++n) load_pieces(lds0 + U * CHUNK + n * 1024, lhs_from[n], lhs_base + chunk * lhs_step);
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const uint8_t* from = rhs[j] + chunk * rhs_step;
@@ -74,20 +114,30 @@ __global__ __launch_bounds__(64 * WAVES) void mx_mmt4d_few_kernel(const MxProduc
         __builtin_memcpy(b[U][j].w, __builtin_assume_aligned(from, 16), 16);
       }
     }
+    if constexpr (!STAGED) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const uint8_t* from = lhs[i] + chunk * lhs_step;
-      __builtin_memcpy(a[U][i].w, __builtin_assume_aligned(from, 16), 16);
-      if constexpr (LBITS == 8) __builtin_memcpy(a[U][i].w + 4, __builtin_assume_aligned(from + 64, 16), 16);
+      for (int i = 0; i < MT; ++i) {
+        const uint8_t* from = lhs[i] + chunk * lhs_step;
+        __builtin_memcpy(a[U][i].w, __builtin_assume_aligned(from, 16), 16);
+        if constexpr (LBITS == 8) __builtin_memcpy(a[U][i].w + 4, __builtin_assume_aligned(from + 64, 16), 16);
+      }
     }
   };
   auto multiply = [&](auto number) {
-    constexpr int U = decltype(number)::value;
+    constexpr int U = decltype(number)::value, HELD = STAGED ? 0 : U;
+    if constexpr (STAGED) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const uint8_t* const row = staged + U * CHUNK + i * 16 * ROW;
+        *(uint4*)a[0][i].w = *(const uint4*)(row + 16 * (g ^ exchanged(r)));
+        if constexpr (LBITS == 8) *(uint4*)(a[0][i].w + 4) = *(const uint4*)(row + 16 * ((4 + g) ^ exchanged(r)));
+      }
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       if constexpr (SPLIT) {
         MxFragment<8> high, low;
-        mx_split(a[U][i], high, low);
+        mx_split(a[HELD][i], high, low);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           acc[i][j] = mx_mfma_16<4, 8, U>(b[U][j], bs[j], high, as[i], acc[i][j]);
@@ -95,9 +145,11 @@ __global__ __launch_bounds__(64 * WAVES) void mx_mmt4d_few_kernel(const MxProduc
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = mx_mfma_16<4, LBITS, U>(b[U][j], bs[j], a[U][i], as[i], acc[i][j]);
+        for (int j = 0; j < NT; ++j) acc[i][j] = mx_mfma_16<4, LBITS, U>(b[U][j], bs[j], a[HELD][i], as[i], acc[i][j]);
       }
     }
+    // (What has been read from LDS has been read before its place is loaded again.)
+    if constexpr (STAGED) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
   auto of_four = [](auto f) {
     f(std::integral_constant<int, 0>{});
@@ -116,60 +168,75 @@ __global__ __launch_bounds__(64 * WAVES) void mx_mmt4d_few_kernel(const MxProduc
     uint32_t four = wave, first = begin(four);
     load_scales(first);
     of_four([&](auto u) { load(u, first); });
-    for (; four + WAVES < fours; four += WAVES) {  // (all of four chunks)
+    for (; four + kWaves < fours; four += kWaves) {  // (all of four chunks)
       take_scales();
-      first = begin(four + WAVES);
+      first = begin(four + kWaves);
       load_scales(first);
       of_four([&](auto u) {
+        // (Behind a chunk's loads come three chunks', and of each only those to LDS are counted on: the compiler may leave out
+        // or join its own.)
+        if constexpr (STAGED) wait_loads<3 * LOADS>();
         multiply(u);
         load(u, first);
       });
     }
     take_scales();
     const uint32_t skip = 4 * four - first, end = p.chunks - first;
+    if constexpr (STAGED) wait_loads<0>();
     of_four([&](auto u) {
       constexpr uint32_t U = decltype(u)::value;
       if (U >= skip && U < end) multiply(u);
     });
   }
 
+  mx_v4f32* const partial = (mx_v4f32*)few_lds;  // [kWaves][MT * NT][64]
+  if constexpr (STAGED) __syncthreads();
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) partial[wave][i * NT + j][lane] = acc[i][j];
+    for (int j = 0; j < NT; ++j) partial[(wave * (MT * NT) + i * NT + j) * 64 + lane] = acc[i][j];
   __syncthreads();
-  for (int f = wave; f < MT * NT; f += WAVES) {
-    mx_v4f32 v = partial[0][f][lane];
+  for (int f = wave; f < MT * NT; f += kWaves) {
+    mx_v4f32 v = partial[f * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) v += partial[w][f][lane];
+    for (int w = 1; w < kWaves; ++w) v += partial[(w * (MT * NT) + f) * 64 + lane];
     const uint32_t row = first_row + 16 * (f / NT) + r, col = first_col + 16 * (f % NT) + 4 * g;
     if (row < p.lhs.rows) mx_store_four(p, mx_out_row(p, row), col, v);
   }
 }
 
-template <int LBITS, int MT, int NT, int WAVES>
+template <int LBITS, int MT, int NT, bool STAGED>
 hipError_t launch(const MxProduct& p, hipStream_t stream) {
   const dim3 grid((p.rhs.rows + 16 * NT - 1) / (16 * NT), (p.lhs.rows + 16 * MT - 1) / (16 * MT));
   void* args[] = {const_cast<MxProduct*>(&p)};
   const bool stream_rhs = comes_from_hbm((int64_t)p.rhs.rows * p.chunks * 64);
   const bool split = LBITS == 8 && p.out_type == Float::kF32;
-  const void* kernel = split ? (stream_rhs ? (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, WAVES, true, LBITS == 8>
-                                           : (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, WAVES, false, LBITS == 8>)
-                             : (stream_rhs ? (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, WAVES, true, false>
-                                           : (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, WAVES, false, false>);
-  return hipLaunchKernel(kernel, grid, dim3(64 * WAVES), args, 0, stream);
+  constexpr bool EIGHT = LBITS == 8;
+  const void* kernel = split ? (stream_rhs ? (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, true, EIGHT, STAGED>
+                                           : (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, false, EIGHT, STAGED>)
+                             : (stream_rhs ? (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, true, false, STAGED>
+                                           : (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, false, false, STAGED>);
+  constexpr int SUMS = kWaves * MT * NT * 1024, LHS = STAGED ? kWaves * 4 * MT * 256 * LBITS : 0, LDS = SUMS > LHS ? SUMS : LHS;
+  static_assert(LDS <= 160 * 1024, "LDS");
+  if (LDS > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e != hipSuccess) return e;
+  }
+  return hipLaunchKernel(kernel, grid, dim3(64 * kWaves), args, LDS, stream);
 }
 
 template <int LBITS>
 hipError_t launch_of(const MxProduct& p, int shape, hipStream_t stream) {
   switch (shape) {  // kMxFewShapes
-    case 0: return launch<LBITS, 1, 1, 8>(p, stream);
-    case 1: return launch<LBITS, 1, 2, 8>(p, stream);
-    case 2: return launch<LBITS, 1, 4, 8>(p, stream);
-    case 3: return launch<LBITS, 2, 1, 8>(p, stream);
-    case 4: return launch<LBITS, 2, 2, 8>(p, stream);
-    case 5: return launch<LBITS, 2, 4, 8>(p, stream);
-    case 6: if constexpr (LBITS == 4) return launch<4, 4, 4, 8>(p, stream);  // (8-bit codes do not fit the registers)
+    case 0: return launch<LBITS, 1, 1, false>(p, stream);
+    case 1: return launch<LBITS, 1, 2, false>(p, stream);
+    case 2: return launch<LBITS, 1, 4, false>(p, stream);
+    case 3: return launch<LBITS, 1, 1, true>(p, stream);
+    case 4: return launch<LBITS, 1, 2, true>(p, stream);
+    case 5: return launch<LBITS, 1, 4, true>(p, stream);
+    case 6: return launch<LBITS, 2, 1, true>(p, stream);
+    case 7: return launch<LBITS, 2, 2, true>(p, stream);
+    case 8: return launch<LBITS, 2, 4, true>(p, stream);
   }
   return hipErrorInvalidValue;
 }
