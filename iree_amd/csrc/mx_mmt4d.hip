@@ -133,7 +133,7 @@ bool block_covers(const MxProduct& p) {
 // Over these, drawn from 1 to 4096 rows, 64 to 28672 columns, K of 64 to 14336, with tiles and row-major, the kernel taken is
 // slower than the best one by 2 % in the mean.
 struct Choice {
-  bool block;
+  enum { kGeneric, kFew, kBlock } kernel;
   int number;
 };
 Choice choose(const MxProduct& p, int lhs_bits) {
@@ -146,7 +146,7 @@ Choice choose(const MxProduct& p, int lhs_bits) {
                                    {10.1f, 1.396f, 2.846f, 5}, {3.6f, .488f, .65f, 1}, {4.5f, .732f, 1.071f, 1.9f}, {4.5f, .537f, .871f, 1.4f}};
   const Times* times = lhs_bits == 4 ? kE2m1 : p.out_type == Float::kF32 ? kE4m3F32 : kE4m3;
   const int64_t rows = p.lhs.rows, cols = p.rhs.rows;
-  Choice best = {false, 0};
+  Choice best = {Choice::kGeneric, 0};
   float least = 0;
   const float lines = p.lhs.tile_rows >= 16 && lhs_bits == 4 ? 0 : (float)(rows < 16 ? rows - 1 : 15) / 15;
   const bool eight = lhs_bits == 8, split = times == kE4m3F32, lhs_near = near(p.lhs);
@@ -156,14 +156,15 @@ Choice choose(const MxProduct& p, int lhs_bits) {
   for (int i = 0; i < (int)(sizeof kMxFewShapes / sizeof kMxFewShapes[0]); ++i) {
     const MxFewShape& s = kMxFewShapes[i];
     const int64_t down = (rows + 16 * s.mt - 1) / (16 * s.mt), across = (cols + 16 * s.nt - 1) / (16 * s.nt);
-    if (down > 65535 || (s.staged && !lhs_near)) continue;
+    // (A grid has fewer than 2^32 threads, and 2^16 rows.)
+    if (down > 65535 || down * across > (1 << 22) || (s.staged && !lhs_near)) continue;
     const float rounds = (float)((down * across + 255) / 256), start = 1.95f + .27f * s.mt * s.nt;
     const float loads = rounds * p.chunks * (s.mt * (s.staged ? lhs_staged : lhs_direct) + s.nt * rhs_chunk + s.mt * s.nt * product);
     const float streamed = memory / (down * across < 448 ? 5.8f : 6.5f);
     const float cost = start + (rounds - 1) * .37f * start + (loads > streamed ? loads + .13f * streamed : streamed + .13f * loads);
-    if (least == 0 || cost < least) {
+    if (best.kernel == Choice::kGeneric || cost < least) {
       least = cost;
-      best.number = i;
+      best = {Choice::kFew, i};
     }
   }
   if (!block_covers(p)) return best;
@@ -174,9 +175,9 @@ Choice choose(const MxProduct& p, int lhs_bits) {
     const float steps = p.chunks * ((rounds >> 1) * times[i].two + (rounds & 1) * times[i].one);
     const float streamed = memory / 5.8f;
     const float cost = times[i].start + (rounds - 1) * times[i].start_again + (steps > streamed ? steps : streamed) + .15f * streamed;
-    if (cost < least) {
+    if (best.kernel == Choice::kGeneric || cost < least) {
       least = cost;
-      best = {true, i};
+      best = {Choice::kBlock, i};
     }
   }
   return best;
@@ -188,7 +189,8 @@ hipError_t launch_mx_mmt4d(const MxMmt4dArgs& a, hipStream_t stream, const char*
   MxProduct p;
   if (!as_product(a, &p)) return launch_generic(a, stream, name);
   const Choice c = choose(p, a.lhs_bits);
-  if (!c.block) {
+  if (c.kernel == Choice::kGeneric) return launch_generic(a, stream, name);
+  if (c.kernel == Choice::kFew) {
     *name = kMxFewShapes[c.number].name;
     return launch_mx_few(p, a.lhs_bits, c.number, stream);
   }

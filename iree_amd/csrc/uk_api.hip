@@ -1002,8 +1002,8 @@ bool overlap(const Operand& a, const Operand& b) {
   return between < a.region.width || between + b.region.width > pitch;
 }
 
-// Whether an operand that a call touches has an address.
-bool given(const Operand& o) { return o.region.span == 0 || o.ptr != nullptr; }
+// Whether an operand that a call touches has a buffer.
+bool given(const Operand& o, const void* buffer) { return o.region.span == 0 || buffer != nullptr; }
 
 bool same_place(const Operand& a, const Operand& b) {
   return a.ptr == b.ptr && (a.region.rows == 1 || a.region.pitch == b.region.pitch);
@@ -1074,7 +1074,9 @@ UK_API void iree_uk_mi355x_mx_pack_p(const iree_uk_mi355x_mx_pack_params_t* p) {
   UK_REQUIRE(!overlap(o_codes, o_in));
   UK_REQUIRE(!overlap(o_scales, o_in));
   Operand* const operands[] = {&o_in, &o_codes, &o_scales};
-  for (const Operand* o : operands) UK_REQUIRE(given(*o));
+  UK_REQUIRE(given(o_in, p->in_buffer));
+  UK_REQUIRE(given(o_codes, p->out_buffer));
+  UK_REQUIRE(given(o_scales, p->scales_buffer));
   if (!stage_operands(stager, operands, 3, stream)) {
     abandon(stager, stream);
     return;
@@ -1141,7 +1143,9 @@ UK_API void iree_uk_mi355x_mx_unpack_p(const iree_uk_mi355x_mx_unpack_params_t* 
   UK_REQUIRE(!overlap(o_out, o_codes));
   UK_REQUIRE(!overlap(o_out, o_scales));
   Operand* const operands[] = {&o_codes, &o_scales, &o_out};
-  for (const Operand* o : operands) UK_REQUIRE(given(*o));
+  UK_REQUIRE(given(o_codes, p->in_buffer));
+  UK_REQUIRE(given(o_scales, p->scales_buffer));
+  UK_REQUIRE(given(o_out, p->out_buffer));
   if (!stage_operands(stager, operands, 3, stream)) {
     abandon(stager, stream);
     return;
@@ -1211,7 +1215,11 @@ UK_API void iree_uk_mi355x_mx_mmt4d_p(const iree_uk_mi355x_mx_mmt4d_params_t* p)
   Operand o_rhs_scales{offset_pointer(p->rhs_scales_buffer, p->rhs_scales_offset), as_copied(rhs_scales_region), true};
   Operand o_out{offset_pointer(p->out_buffer, out_offset_bytes), out_region, accumulate};
   Operand* const operands[] = {&o_lhs, &o_lhs_scales, &o_rhs, &o_rhs_scales, &o_out};
-  for (const Operand* o : operands) UK_REQUIRE(given(*o));
+  UK_REQUIRE(given(o_lhs, p->lhs_buffer));
+  UK_REQUIRE(given(o_lhs_scales, p->lhs_scales_buffer));
+  UK_REQUIRE(given(o_rhs, p->rhs_buffer));
+  UK_REQUIRE(given(o_rhs_scales, p->rhs_scales_buffer));
+  UK_REQUIRE(given(o_out, p->out_buffer));
   for (int i = 0; i < 4; ++i) UK_REQUIRE(!overlap(o_out, *operands[i]));
   if (!stage_operands(stager, operands, 5, stream)) {
     abandon(stager, stream);
@@ -1304,7 +1312,9 @@ UK_API void iree_uk_mi355x_rms_norm_p(const iree_uk_mi355x_rms_norm_params_t* p)
   }
   UK_REQUIRE(!overlap(o_out, o_scales));
   Operand* const operands[] = {&o_in, &o_residual, &o_sum, &o_weight, &o_out, &o_scales};
-  for (const Operand* o : operands) UK_REQUIRE(given(*o));
+  UK_REQUIRE(given(o_in, p->in_buffer));
+  UK_REQUIRE(given(o_out, p->out_buffer));
+  UK_REQUIRE(given(o_scales, p->scales_buffer));
   if (!stage_operands(stager, operands, 6, stream)) {
     abandon(stager, stream);
     return;

@@ -58,7 +58,7 @@ def test_null_parameters(entry):
     dict(scales_stride0=-1), dict(out_offset=1), dict(out_stride0=2049), dict(in_size0=17), dict(in_size1=129),
     dict(out_size0=2, in_size0=32, out_stride0=2046), dict(out_size0=2, in_size0=32, out_stride0=2048, scales_stride0=63),
     dict(scales_buffer=AT + 16384 + 1000), dict(scales_buffer=AT), dict(out_buffer=AT + 8000),
-    dict(in_buffer=None), dict(out_buffer=None), dict(scales_buffer=None),
+    dict(in_buffer=None), dict(out_buffer=None), dict(scales_buffer=None), dict(in_buffer=None, in_offset=4),
     dict(out_size1=1 << 62), dict(out_size0=1 << 40, out_size1=1 << 40)])
 def test_pack(kw):
     refused("mx_pack", pack(**kw))
@@ -69,7 +69,7 @@ def test_pack(kw):
     dict(in_stride0=-2), dict(in_offset=3), dict(in_stride0=1001), dict(scales_stride0=-1), dict(out_stride0=-1),
     dict(out_stride1=-1), dict(out_stride0=127), dict(out_stride1=0), dict(out_size0=17), dict(out_size1=129),
     dict(out_buffer=AT + 512), dict(out_buffer=AT + 16384 + 8), dict(out_buffer=None), dict(in_buffer=None),
-    dict(scales_buffer=None)])
+    dict(scales_buffer=None), dict(scales_buffer=None, scales_offset=16)])
 def test_unpack(kw):
     refused("mx_unpack", unpack(**kw))
 
@@ -80,7 +80,7 @@ def test_unpack(kw):
     dict(rhs_stride0=2047), dict(lhs_stride0=-2048), dict(rhs_scales_stride0=-64), dict(out_stride0=511),
     dict(out_buffer=AT), dict(out_buffer=AT + 8192), dict(out_buffer=AT + 16384), dict(out_buffer=AT + 24576 - 4),
     dict(lhs_buffer=None), dict(lhs_scales_buffer=None), dict(rhs_buffer=None), dict(rhs_scales_buffer=None),
-    dict(out_buffer=None)])
+    dict(out_buffer=None), dict(out_buffer=None, out_offset=4)])
 def test_mmt4d(kw):
     refused("mx_mmt4d", mmt4d(**kw))
 
@@ -92,7 +92,7 @@ def test_mmt4d(kw):
     dict(sum_stride0=63), dict(out_stride0=63), dict(scales_stride0=1), dict(flags=abi.RMS_NORM_TYPE_F32E2M1, out_offset=1),
     dict(sum_buffer=AT + 4), dict(sum_buffer=AT + 8192, sum_stride0=65), dict(sum_buffer=AT + 24576),
     dict(out_buffer=AT + 24576), dict(out_buffer=AT), dict(scales_buffer=AT + 16384), dict(scales_buffer=AT + 32768 + 8),
-    dict(in_buffer=None), dict(out_buffer=None), dict(scales_buffer=None)])
+    dict(in_buffer=None), dict(out_buffer=None), dict(scales_buffer=None), dict(out_buffer=None, out_offset=32)])
 def test_norm(kw):
     refused("rms_norm", norm(**kw))
 

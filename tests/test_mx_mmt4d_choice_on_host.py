@@ -187,3 +187,14 @@ def test_what_the_fast_kernels_do_not_take(recorder, change, kernel):  # noqa: F
     assert name.startswith("mx_mmt4d_" + kernel), name
     if p.lhs_stride0 == 1 << 24:
         assert not name.endswith("staged")
+
+
+@pytest.mark.parametrize("tiles,tile,kernel", [
+    # More rows of 16 or 32 than a grid has, in tiles that no block kernel takes; more columns than it has threads for.
+    ((1 << 20, 1, 1), (4, 16, 128), "generic"), ((1 << 16, 1, 1), (4, 16, 128), "few"),
+    ((1, 1 << 30, 1), (2, 1, 128), "generic"), ((1, 1 << 24, 1), (2, 1, 128), "few"),
+    ((1, 1 << 30, 1), (1, 1, 128), "generic"), ((1 << 22, 1, 1), (1, 16, 128), "block")])
+def test_grids_of_any_size(recorder, tiles, tile, kernel):  # noqa: F811
+    p = ref.mmt4d_params(1 << 36, 2 << 39, 3 << 39, 4 << 39, 5 << 39, tiles, tile, "e4m3", "f32")
+    _, name = recorder.call("iree_uk_mi355x_mx_mmt4d_p", p)
+    assert name.startswith("mx_mmt4d_" + kernel), name
