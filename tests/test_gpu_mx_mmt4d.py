@@ -216,3 +216,62 @@ def test_the_same_call_gives_the_same_bits(gpu_lib, m, n, k):
     first, _ = product(gpu_lib, lhs, rhs, (1, 16, 128), "e4m3", "f32")
     for _ in range(3):
         np.testing.assert_array_equal(product(gpu_lib, lhs, rhs, (1, 16, 128), "e4m3", "f32")[0], first)
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_a_rhs_beyond_32_bits(gpu_lib, m):
+    # 4.5 GiB of weights in tiles of 16 x 128: ones, but for the last 64 columns. All values are multiples of 1/2 below 16: sums of
+    # 131072 products with random signs are multiples of 1/4 below 2^22.
+    cols, k = 73728, 131072
+    rng = np.random.default_rng(m)
+    lhs, last = exact_codes(rng, m, k, "e2m1"), exact_codes(rng, 64, k, "e2m1")
+    codes = torch.full((cols * k // 2,), 0x22, dtype=torch.uint8, device="cuda")
+    scales = torch.full((cols * k // 32,), 127, dtype=torch.uint8, device="cuda")
+    codes[-32 * k:] = on_device(ref.to_bytes(ref.tiled(last[0], 16, 128), "e2m1"))
+    scales[-2 * k:] = on_device(ref.tiled(last[1], 16, 4))
+    out = torch.zeros(m, cols, device="cuda")
+    a, s = on_device(ref.to_bytes(lhs[0], "e2m1")), on_device(lhs[1])
+    p = ref.mmt4d_params(a.data_ptr(), s.data_ptr(), codes.data_ptr(), scales.data_ptr(), out.data_ptr(),
+                         (m, cols // 16, k // 128), (1, 16, 128), "e2m1", "f32")
+    gpu_lib.iree_uk_mi355x_mx_mmt4d_p(C.byref(p))
+    want = torch.from_numpy(ref.widen(*lhs, "e2m1").sum(1)).float().cuda()
+    assert float(want.abs().max()) < 2.0 ** 22
+    assert bool((out[:, :-64] == want[:, None]).all())
+    np.testing.assert_array_equal(host(out[:, -64:].contiguous()).reshape(m, 64), in_64_bits(lhs, last, "e2m1"))
+
+
+@pytest.mark.parametrize("m0", [1, 16])
+def test_a_result_beyond_32_bits(gpu_lib, m0):
+    # 4.5 GiB of bf16: ones times the weights, but for the last 48 rows.
+    rows, cols = 73728, 32768
+    rng = np.random.default_rng(m0)
+    last, rhs = exact_codes(rng, 48, 128, "e4m3"), exact_codes(rng, cols, 128, "e2m1")
+    lhs = torch.full((rows * 128,), 0x38, dtype=torch.uint8, device="cuda")
+    scales = torch.full((rows * 4,), 127, dtype=torch.uint8, device="cuda")
+    lhs[-48 * 128:], scales[-48 * 4:] = on_device(ref.tiled(last[0], m0, 128)), on_device(ref.tiled(last[1], m0, 4))
+    b, t = on_device(ref.to_bytes(ref.tiled(rhs[0], 16, 128), "e2m1")), on_device(ref.tiled(rhs[1], 16, 4))
+    out = torch.zeros(rows // m0, cols // 16, m0, 16, dtype=torch.int16, device="cuda")
+    p = ref.mmt4d_params(lhs.data_ptr(), scales.data_ptr(), b.data_ptr(), t.data_ptr(), out.data_ptr(),
+                         (rows // m0, cols // 16, 1), (m0, 16, 128), "e4m3", "bf16")
+    gpu_lib.iree_uk_mi355x_mx_mmt4d_p(C.byref(p))
+    ones = ref.raw(ref.to_type(ref.widen(*rhs, "e2m1").sum(1).astype(np.float32), "bf16"), "bf16").view(np.int16)
+    ones = torch.from_numpy(ones.reshape(cols // 16, 1, 16)).cuda()
+    for first in range(0, rows - 48, 8192):
+        end = min(first + 8192, rows - 48)
+        assert bool((out[first // m0:end // m0] == ones).all())
+    got = ref.untiled(host(out[-48 // m0:].contiguous()).view(np.uint16).reshape(48 // m0, cols // 16, m0, 16))
+    want = in_64_bits(last, rhs, "e4m3").astype(np.float32)
+    np.testing.assert_array_equal(got, ref.raw(ref.to_type(want, "bf16"), "bf16"))
+
+
+def test_accumulation_into_a_host_result_with_gaps(gpu_lib):
+    rng = np.random.default_rng(4)
+    lhs, rhs = exact_codes(rng, 20, 256, "e4m3"), exact_codes(rng, 48, 256, "e2m1")
+    a, s, b, t = lhs[0], lhs[1], ref.to_bytes(ref.tiled(rhs[0], 16, 128), "e2m1"), ref.tiled(rhs[1], 16, 4)
+    out = np.full((20, 50), 9, np.float32)
+    p = ref.mmt4d_params(a.ctypes.data, s.ctypes.data, b.ctypes.data, t.ctypes.data, out.ctypes.data, (20, 3, 2),
+                         (1, 16, 128), "e4m3", "f32", True)
+    p.out_stride0 = 50
+    gpu_lib.iree_uk_mi355x_mx_mmt4d_p(C.byref(p))
+    np.testing.assert_array_equal(out[:, :48], in_64_bits(lhs, rhs, "e4m3") + 9)
+    assert (out[:, 48:] == 9).all()

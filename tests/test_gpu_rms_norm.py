@@ -193,3 +193,31 @@ def test_a_row_does_not_depend_on_its_company(gpu_lib):
         one = run(gpu_lib, x[i:i + 1], r[i:i + 1], w, "bf16", "e2m1", 8000)
         for a, b in zip(many, one):
             np.testing.assert_array_equal(a[i:i + 1], b)
+
+
+@pytest.mark.parametrize("format", ["s8", "e4m3"])
+def test_rows_beyond_32_bits(gpu_lib, format):
+    # 4.5 GiB of bf16, sums in place of the residual: the last rows as a call of their own has them.
+    rows, cols, few = 73728, 32768, 16
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.ones(rows, cols, dtype=torch.bfloat16, device="cuda")
+    total = torch.ones(rows, cols, dtype=torch.bfloat16, device="cuda")
+    for t in (x, total):
+        t[-few:] = torch.randn(few, cols, generator=gen, device="cuda").bfloat16()
+    weight = torch.randn(cols, generator=gen, device="cuda").bfloat16()
+
+    def call(x, total):
+        n = x.shape[0]
+        codes = torch.zeros(n, cols, dtype=torch.uint8, device="cuda")
+        scales = torch.zeros(n, 4 if format == "s8" else cols // 32, dtype=torch.uint8, device="cuda")
+        p = ref.norm_params(x.data_ptr(), total.data_ptr(), total.data_ptr(), weight.data_ptr(), codes.data_ptr(),
+                            scales.data_ptr(), n, cols, cols, "bf16", format)
+        gpu_lib.iree_uk_mi355x_rms_norm_p(C.byref(p))
+        return total, codes, scales
+
+    alone = call(x[-few:].clone(), total[-few:].clone())
+    first = call(x[:1].clone(), total[:1].clone())
+    everything = call(x, total)
+    for all_rows, last, one in zip(everything, alone, first):
+        assert torch.equal(all_rows[-few:], last)
+        assert bool((all_rows[:-few] == one).all())
