@@ -12,19 +12,19 @@ KERNELS = [
     ("e2m1", "f32", 1302, 1551, 128, 1, 1, "block_128x128"),
     ("e2m1", "bf16", 1957, 2127, 128, 1, 1, "block_128x192"),
     ("e2m1", "bf16", 2667, 2351, 640, 1, 1, "block_128x256"),
-    ("e2m1", "f32", 1041, 975, 128, 1, 1, "block_128x64"),
+    ("e2m1", "bf16", 1232, 785, 128, 16, 1, "block_128x64"),
     ("e2m1", "f32", 3856, 3292, 384, 16, 1, "block_256x256"),
     ("e2m1", "f32", 1424, 1369, 128, 16, 1, "block_64x128"),
-    ("e2m1", "bf16", 552, 496, 128, 1, 16, "block_64x64"),
+    ("e2m1", "f32", 592, 434, 128, 1, 1, "block_64x64"),
     ("e2m1", "f32", 1, 16, 128, 1, 16, "few_16x16"),
-    ("e2m1", "f32", 13, 16, 128, 1, 16, "few_16x16_staged"),
-    ("e2m1", "f32", 240, 288, 128, 16, 16, "few_16x32"),
-    ("e2m1", "f32", 326, 208, 128, 1, 16, "few_16x32_staged"),
-    ("e2m1", "bf16", 432, 320, 128, 16, 16, "few_16x64"),
+    ("e2m1", "f32", 15, 16, 128, 1, 1, "few_16x16_staged"),
+    ("e2m1", "f32", 1, 4106, 128, 1, 1, "few_16x32"),
+    ("e2m1", "f32", 304, 401, 128, 1, 1, "few_16x32_staged"),
+    ("e2m1", "bf16", 1, 8224, 128, 1, 16, "few_16x64"),
     ("e2m1", "bf16", 357, 688, 128, 1, 16, "few_16x64_staged"),
     ("e2m1", "f32", 202, 310, 128, 1, 1, "few_32x16_staged"),
-    ("e2m1", "bf16", 320, 410, 128, 16, 1, "few_32x32_staged"),
-    ("e2m1", "bf16", 430, 736, 896, 1, 16, "few_32x64_staged"),
+    ("e2m1", "f32", 394, 331, 128, 1, 1, "few_32x32_staged"),
+    ("e2m1", "bf16", 832, 320, 1024, 16, 16, "few_32x64_staged"),
     ("e4m3", "bf16", 1584, 1312, 128, 16, 16, "block_128x128"),
     ("e4m3", "bf16", 1824, 2221, 128, 16, 1, "block_128x192"),
     ("e4m3", "bf16", 2206, 2880, 1152, 1, 16, "block_128x256"),
@@ -40,7 +40,7 @@ KERNELS = [
     ("e4m3", "bf16", 226, 1078, 128, 1, 1, "few_16x64_staged"),
     ("e4m3", "bf16", 214, 302, 128, 1, 1, "few_32x16_staged"),
     ("e4m3", "bf16", 336, 389, 128, 16, 1, "few_32x32_staged"),
-    ("e4m3", "bf16", 512, 592, 640, 16, 16, "few_32x64_staged"),
+    ("e4m3", "bf16", 903, 352, 768, 1, 16, "few_32x64_staged"),
     ("e4m3", "f32", 2732, 2182, 128, 1, 1, "block_128x128"),
     ("e4m3", "f32", 2582, 1584, 128, 1, 16, "block_128x192"),
     ("e4m3", "f32", 3081, 1968, 1664, 1, 16, "block_128x256"),
@@ -48,15 +48,15 @@ KERNELS = [
     ("e4m3", "f32", 3102, 4498, 640, 1, 1, "block_256x256"),
     ("e4m3", "f32", 658, 1551, 128, 1, 1, "block_64x128"),
     ("e4m3", "f32", 558, 464, 128, 1, 1, "block_64x64"),
-    ("e4m3", "f32", 1, 18, 128, 1, 1, "few_16x16"),
-    ("e4m3", "f32", 2, 16, 128, 1, 1, "few_16x16_staged"),
+    ("e4m3", "f32", 2, 16, 128, 1, 1, "few_16x16"),
+    ("e4m3", "f32", 9, 16, 128, 1, 16, "few_16x16_staged"),
     ("e4m3", "f32", 1, 4144, 128, 1, 16, "few_16x32"),
-    ("e4m3", "f32", 246, 288, 128, 1, 16, "few_16x32_staged"),
+    ("e4m3", "f32", 288, 240, 128, 16, 16, "few_16x32_staged"),
     ("e4m3", "f32", 1, 8232, 128, 1, 1, "few_16x64"),
-    ("e4m3", "f32", 807, 320, 128, 1, 16, "few_16x64_staged"),
+    ("e4m3", "f32", 304, 816, 128, 16, 16, "few_16x64_staged"),
     ("e4m3", "f32", 288, 253, 128, 16, 1, "few_32x16_staged"),
     ("e4m3", "f32", 414, 309, 128, 1, 1, "few_32x32_staged"),
-    ("e4m3", "f32", 526, 496, 256, 1, 16, "few_32x64_staged"),
+    ("e4m3", "f32", 472, 592, 384, 1, 16, "few_32x64_staged"),
     ("e2m1", "bf16", 1699, 1254, 896, 1, 1, "block_128x128"),
     ("e2m1", "f32", 2576, 1551, 896, 16, 1, "block_128x192"),
     ("e2m1", "f32", 2744, 2504, 896, 8, 8, "block_128x256"),
@@ -65,10 +65,9 @@ KERNELS = [
     ("e2m1", "bf16", 795, 2360, 896, 1, 8, "block_64x128"),
     ("e2m1", "bf16", 584, 442, 896, 8, 1, "block_64x64"),
     ("e2m1", "bf16", 1, 16, 4736, 1, 16, "few_16x16"),
-    ("e2m1", "bf16", 12, 17, 5504, 1, 1, "few_16x16_staged"),
-    ("e2m1", "bf16", 256, 288, 4864, 16, 8, "few_16x32"),
-    ("e2m1", "f32", 173, 400, 4864, 1, 16, "few_16x32_staged"),
-    ("e2m1", "f32", 384, 368, 5504, 16, 16, "few_16x64"),
+    ("e2m1", "f32", 16, 16, 4608, 16, 8, "few_16x16_staged"),
+    ("e2m1", "bf16", 8, 4160, 4608, 8, 16, "few_16x32"),
+    ("e2m1", "f32", 232, 544, 4608, 1, 16, "few_16x32_staged"),
     ("e2m1", "bf16", 272, 912, 4736, 8, 16, "few_16x64_staged"),
     ("e2m1", "bf16", 248, 276, 4480, 1, 1, "few_32x16_staged"),
     ("e2m1", "f32", 366, 372, 4480, 1, 1, "few_32x32_staged"),
@@ -96,7 +95,7 @@ KERNELS = [
     ("e4m3", "f32", 1232, 800, 896, 8, 1, "block_64x128"),
     ("e4m3", "f32", 715, 761, 896, 1, 1, "block_64x64"),
     ("e4m3", "f32", 1, 19, 4608, 1, 1, "few_16x16"),
-    ("e4m3", "f32", 2, 18, 5248, 1, 1, "few_16x16_staged"),
+    ("e4m3", "f32", 8, 16, 4608, 8, 1, "few_16x16_staged"),
     ("e4m3", "f32", 1, 4128, 4608, 1, 8, "few_16x32"),
     ("e4m3", "f32", 177, 384, 4480, 1, 16, "few_16x32_staged"),
     ("e4m3", "f32", 805, 312, 5120, 1, 8, "few_16x64_staged"),
