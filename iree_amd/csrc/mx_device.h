@@ -44,12 +44,27 @@ struct MxEight {
   uint32_t w[kWords];
 };
 
+// STREAM: past the caches.
+template <Float T, bool STREAM>
+__device__ __forceinline__ void mx_load_eight(MxEight<T>& v, const uint8_t* p) {
+  if constexpr (STREAM) {
+    typedef uint32_t unaligned_v4u32 __attribute__((ext_vector_type(4), aligned(2)));
+#pragma unroll
+    for (int i = 0; i < MxEight<T>::kBytes / 16; ++i) {
+      const unaligned_v4u32 q = __builtin_nontemporal_load((const unaligned_v4u32*)p + i);
+      __builtin_memcpy(v.w + 4 * i, &q, 16);
+    }
+  } else {
+    __builtin_memcpy(v.w, p, MxEight<T>::kBytes);
+  }
+}
+
 // `count` of them exist (any number, also none or more); the others are zero. The address is a multiple of the element's
 // size and of nothing more: a row of an odd length starts anywhere, and loads of 16 bytes need no alignment here.
-template <Float T>
+template <Float T, bool STREAM = false>
 __device__ __forceinline__ void mx_load(MxEight<T>& v, const uint8_t* p, int64_t count) {
   if (count >= 8) {
-    __builtin_memcpy(v.w, p, MxEight<T>::kBytes);
+    mx_load_eight<T, STREAM>(v, p);
     return;
   }
 #pragma unroll
@@ -70,6 +85,14 @@ __device__ __forceinline__ void mx_widen_eight(const MxEight<T>& v, float f[8]) 
     if constexpr (T == Float::kF32) f[i] = __builtin_bit_cast(float, v.w[i]);
     else f[i] = mx_widen<T>((uint16_t)(v.w[i / 2] >> (16 * (i & 1))));
   }
+}
+
+// 16 bytes to an address of any alignment; STREAM: past the caches.
+template <bool STREAM>
+__device__ __forceinline__ void mx_store_sixteen(uint8_t* p, const uint32_t w[4]) {
+  typedef uint32_t unaligned_v4u32 __attribute__((ext_vector_type(4), aligned(1)));
+  if constexpr (STREAM) __builtin_nontemporal_store(unaligned_v4u32{w[0], w[1], w[2], w[3]}, (unaligned_v4u32*)p);
+  else __builtin_memcpy(p, w, 16);
 }
 
 // Eight f32 values to memory as T, the first `count` of them.

@@ -89,8 +89,8 @@ __device__ __forceinline__ uint32_t mx_block(const MxEight<T> (&v)[4], uint32_t 
   return b;
 }
 
-// Rows whose values are next to each other (in_stride1 == 1).
-template <Float T, int BITS, int AT_ONCE, typename INDEX>
+// Rows whose values are next to each other (in_stride1 == 1). STREAM: past the caches. 14336 x 4096 f32 to E2M1 45.2 us, 5.9 TB/s.
+template <Float T, int BITS, int AT_ONCE, bool STREAM, typename INDEX>
 __global__ __launch_bounds__(kThreads) void mx_pack_rows(const MxPackKernelArgs<INDEX> a) {
   constexpr int SIZE = T == Float::kF32 ? 4 : 2;
   const INDEX first = (INDEX)blockIdx.x * (kThreads * AT_ONCE) + threadIdx.x;
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kThreads) void mx_pack_rows(const MxPackKernelArgs<
     if (n >= a.shape.segments) break;
     p[u] = mx_place<BITS>(a.shape, n);
     const int64_t left = p[u].row < a.in_size0 ? a.in_size1 - p[u].col : 0;
-    mx_load<T>(v[u], a.in + (p[u].row * a.in_stride0 + p[u].col) * SIZE, left);
+    mx_load<T, STREAM>(v[u], a.in + (p[u].row * a.in_stride0 + p[u].col) * SIZE, left);
   }
 #pragma unroll
   for (int u = 0; u < AT_ONCE; ++u) {
@@ -157,8 +157,9 @@ __global__ __launch_bounds__(kThreads) void mx_pack_strided(const MxPackKernelAr
 // A transposed matrix (in_stride0 == 1) whose columns and their distance are multiples of 16 bytes: 128 of K of 64 rows (128 of a
 // 16-bit type) go straight to LDS, 16 bytes a lane along the rows, and lanes take whole blocks out of it, a word (one value, or
 // two neighbouring rows' values) at a time, 64 of them next to each other. Codes go out through LDS too, 16 bytes a lane in the
-// order of the tile. 14336 x 4096 f32 to E2M1: a lane loading its own block 72.5 us.
-template <Float T, int BITS>
+// order of the tile. 14336 x 4096 f32 to E2M1 from memory: 46.3 us, 5.8 TB/s; a lane loading its own block 72.5 us. STREAM: past the
+// caches.
+template <Float T, int BITS, bool STREAM>
 __global__ __launch_bounds__(kThreads) void mx_pack_transposed(const MxPackKernelArgs<uint32_t> a) {
   constexpr int SIZE = T == Float::kF32 ? 4 : 2, AT_ONCE = 4 / SIZE, ROWS = 64 * AT_ONCE;  // rows of a lane, of a workgroup
   constexpr int LOADS = 128 * 256 / (kThreads * 16), PIECES = BITS / 4;                     // of a lane; 16 bytes of a block's codes
@@ -180,7 +181,9 @@ __global__ __launch_bounds__(kThreads) void mx_pack_transposed(const MxPackKerne
     const int k = (n * 4 + wave) * 4 + (lane >> 4);
     if (load_row < a.in_size0 && k0 + k < a.in_size1) {
       const uint8_t* const from = a.in + ((k0 + k) * a.in_stride1 + load_row) * SIZE;
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds + (n * 4 + wave) * 1024), "v"(from) : "memory");
+      const uint32_t to = lds + (n * 4 + wave) * 1024;
+      if constexpr (STREAM) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(to), "v"(from) : "memory");
+      else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -239,8 +242,9 @@ __global__ __launch_bounds__(kThreads) void mx_pack_transposed(const MxPackKerne
 }
 
 // A lane's values make 16 bytes of the result, eight of a 16-bit type or four of f32 (with eight, whose stores leave every other
-// 16 bytes to the next instruction, 14336 x 4096 E2M1 to f32 took 59.1 us).
-template <Float T, int BITS, int AT_ONCE, typename INDEX>
+// 16 bytes to the next instruction, 14336 x 4096 E2M1 to f32 took 59.1 us, through the caches; now 48.2, and 38.9, 6.8 TB/s, with
+// STREAM, past the caches).
+template <Float T, int BITS, int AT_ONCE, bool STREAM, typename INDEX>
 __global__ __launch_bounds__(kThreads) void mx_unpack_rows(const MxUnpackKernelArgs<INDEX> a) {
   constexpr int SIZE = T == Float::kF32 ? 4 : 2, VALUES = 16 / SIZE, SHARES = 8 / VALUES;
   const INDEX items = a.shape.segments * SHARES;
@@ -275,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void mx_unpack_rows(const MxUnpackKernelA
           if constexpr (T == Float::kF32) w[i] = __builtin_bit_cast(uint32_t, f[i]);
           else w[i] = mx_narrow_pair<T>(f[2 * i], f[2 * i + 1]);
         }
-        __builtin_memcpy(at, w, 16);
+        mx_store_sixteen<STREAM>(at, w);
       } else {
 #pragma unroll
         for (int i = 0; i < VALUES; ++i)
@@ -307,8 +311,19 @@ MxShape<INDEX> mx_shape(int64_t outer0, int64_t outer1, int64_t tile0, int64_t t
 // (Fits: the tiles of a result lie apart in memory.)
 int64_t segments_of(int64_t outer0, int64_t outer1, int64_t tile0, int64_t tile1) { return outer0 * outer1 * tile0 * (tile1 / 8); }
 
+// Loads of a matrix past the caches: with a weight matrix from memory, up to 14336 x 4096 f32, in 46.3 us where loads through the
+// caches take 51.2 (transposed; row by row 45.2 and 47.4), 14336 x 4096 bf16 27.4 and 30.7 (24.8 and 27.8). One that the
+// last-level cache holds takes up to a quarter more (38.6 us of the first through the caches), and smaller ones it may hold.
+bool streams_input(int64_t bytes) { return bytes > (96ll << 20); }
+
+// Stores past the caches: 14336 x 4096 f32 in 38.9 us, through the caches 48.2, and with a kernel that reads the result 134.6 and 146.3.
+// Smaller results are faster alone too (4096 x 4096 bf16 7.2 us, 9.1), but not with their reader (21.1, 19.6; 117 MB 72.3, 65.4), and
+// rows that are not aligned are not (14336 x 4095 f32 73.0, 72.0; 4096 x 4095 20.3, 14.2).
+bool streams_output(int64_t bytes, bool aligned) { return aligned && bytes > (192ll << 20); }
+
 template <Float T, int BITS>
 hipError_t pack(const MxPackArgs& a, hipStream_t stream, const char** name) {
+  constexpr int SIZE = T == Float::kF32 ? 4 : 2;
   const int64_t segments = segments_of(a.outer0, a.outer1, a.tile0, a.tile1);
   auto fill = [&](auto& k) {
     k.in = a.in; k.codes = a.codes; k.scales = a.scales;
@@ -322,12 +337,12 @@ hipError_t pack(const MxPackArgs& a, hipStream_t stream, const char** name) {
     *name = "mx_pack_rows";
     constexpr int MANY = 4;
     if (segments >= (int64_t)MANY * kThreads * 1024)
-      return launch_kernel(mx_pack_rows<T, BITS, MANY, uint32_t>,
+      return launch_kernel(streams_input(a.in_size0 * a.in_size1 * SIZE) ? mx_pack_rows<T, BITS, MANY, true, uint32_t>
+                                                                         : mx_pack_rows<T, BITS, MANY, false, uint32_t>,
                            (unsigned)((segments + MANY * kThreads - 1) / (MANY * kThreads)), kThreads, 0, stream, k);
-    return launch_kernel(mx_pack_rows<T, BITS, 1, uint32_t>, (unsigned)((segments + kThreads - 1) / kThreads), kThreads, 0,
+    return launch_kernel(mx_pack_rows<T, BITS, 1, false, uint32_t>, (unsigned)((segments + kThreads - 1) / kThreads), kThreads, 0,
                          stream, k);
   }
-  constexpr int SIZE = T == Float::kF32 ? 4 : 2;
   auto sixteens = [](int64_t bytes) { return bytes % 16 == 0; };
   const int64_t rows = a.outer0 * a.tile0, blocks = a.outer1 * (a.tile1 / 32), fours = (blocks + 3) / 4;
   const int64_t down = (rows + 256 / SIZE - 1) / (256 / SIZE);
@@ -343,7 +358,8 @@ hipError_t pack(const MxPackArgs& a, hipStream_t stream, const char** name) {
     k.down_reciprocal = reciprocal_of(k.down);
     k.row_blocks_reciprocal = reciprocal_of((uint32_t)(a.tile1 / 32));
     *name = "mx_pack_transposed";
-    return launch_kernel(mx_pack_transposed<T, BITS>, (unsigned)(down * fours), kThreads, 0, stream, k);
+    return launch_kernel(streams_input(a.in_size0 * a.in_size1 * SIZE) ? mx_pack_transposed<T, BITS, true> : mx_pack_transposed<T, BITS, false>,
+                         (unsigned)(down * fours), kThreads, 0, stream, k);
   }
   MxPackKernelArgs<uint64_t> k;
   k.shape = mx_shape<uint64_t>(a.outer0, a.outer1, a.tile0, a.tile1, a.codes_stride0, a.scales_stride0);
@@ -372,15 +388,20 @@ hipError_t unpack(const MxUnpackArgs& given, hipStream_t stream, const char** na
     MxUnpackKernelArgs<uint32_t> k;
     k.shape = mx_shape<uint32_t>(a.outer0, a.outer1, a.tile0, a.tile1, a.codes_stride0, a.scales_stride0);
     fill(k);
-    if (items >= (int64_t)MANY * kThreads * 1024)
-      return launch_kernel(mx_unpack_rows<T, BITS, MANY, uint32_t>, (unsigned)((items + MANY * kThreads - 1) / (MANY * kThreads)),
-                           kThreads, 0, stream, k);
-    return launch_kernel(mx_unpack_rows<T, BITS, 1, uint32_t>, (unsigned)((items + kThreads - 1) / kThreads), kThreads, 0, stream, k);
+    if (items >= (int64_t)MANY * kThreads * 1024) {
+      constexpr int SIZE = T == Float::kF32 ? 4 : 2;
+      const bool aligned = (uintptr_t)a.out % 16 == 0 && a.out_stride0 * SIZE % 16 == 0 && a.out_stride1 == 1;
+      return launch_kernel(streams_output(a.out_size0 * a.out_size1 * SIZE, aligned) ? mx_unpack_rows<T, BITS, MANY, true, uint32_t>
+                                                                                     : mx_unpack_rows<T, BITS, MANY, false, uint32_t>,
+                           (unsigned)((items + MANY * kThreads - 1) / (MANY * kThreads)), kThreads, 0, stream, k);
+    }
+    return launch_kernel(mx_unpack_rows<T, BITS, 1, false, uint32_t>, (unsigned)((items + kThreads - 1) / kThreads), kThreads, 0,
+                         stream, k);
   }
   MxUnpackKernelArgs<uint64_t> k;
   k.shape = mx_shape<uint64_t>(a.outer0, a.outer1, a.tile0, a.tile1, a.codes_stride0, a.scales_stride0);
   fill(k);
-  return launch_kernel(mx_unpack_rows<T, BITS, MANY, uint64_t>, 1u << 21, kThreads, 0, stream, k);
+  return launch_kernel(mx_unpack_rows<T, BITS, MANY, false, uint64_t>, 1u << 21, kThreads, 0, stream, k);
 }
 
 }  // namespace

@@ -262,3 +262,30 @@ def test_offsets_beyond_32_bits(gpu_lib):
     assert bool((back[64:-64] == 1.0).all())
     c, s = ref.quantise(x[-64:].float().cpu().numpy(), "e2m1")
     np.testing.assert_array_equal(back[-64:].float().cpu().numpy(), ref.widen(c, s, "e2m1").astype(np.float32))
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("type,format,rows", [("f32", "e2m1", 8192), ("bf16", "e4m3", 16384)])
+def test_matrices_that_no_cache_holds(gpu_lib, type, format, rows, transposed):
+    # 210 MB, which are read and written past the caches: one block of 512 x 640 over and over.
+    cols = 6400
+    rng = np.random.default_rng(rows)
+    block = ref.to_type(rng.standard_normal((512, 640)) * np.exp2(rng.integers(-4, 5, (512, 1))), type)
+    dtype = torch.float32 if type == "f32" else torch.bfloat16
+    x = torch.from_numpy(block.astype(np.float32)).to(dtype).cuda().repeat(rows // 512, cols // 640)
+    given = x.t().contiguous() if transposed else x
+    codes = torch.zeros(rows * cols * ref.BITS[format] // 8, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(rows * cols // 32, dtype=torch.uint8, device="cuda")
+    p = ref.pack_params(given.data_ptr(), rows, cols, codes.data_ptr(), scales.data_ptr(), 16, 128, type, format)
+    p.in_stride0, p.in_stride1 = (1, rows) if transposed else (cols, 1)
+    gpu_lib.iree_uk_mi355x_mx_pack_p(C.byref(p))
+    assert gpu_lib.iree_uk_mi355x_last_kernel() == (b"mx_pack_transposed" if transposed else b"mx_pack_rows")
+    want_codes, want_scales = wanted(block, format, 16, 128)
+    for got, want in ((codes, want_codes), (scales, want_scales)):
+        want = on_device(want).view(1, 32, 1, 5, -1)   # [.][panels of 16 rows][.][tiles of 128 columns][a tile]
+        assert bool((got.view(rows // 512, 32, cols // 640, 5, -1) == want).all())
+    back = torch.zeros_like(x)
+    p = ref.unpack_params(codes.data_ptr(), scales.data_ptr(), back.data_ptr(), rows, cols, 16, 128, format, type)
+    gpu_lib.iree_uk_mi355x_mx_unpack_p(C.byref(p))
+    values = torch.from_numpy(ref.widen(*ref.quantise(block, format), format).astype(np.float32)).cuda().to(dtype)
+    assert bool((back.view(rows // 512, 512, cols // 640, 640) == values.view(1, 512, 1, 640)).all())
