@@ -55,6 +55,9 @@ constexpr MxBlockTile kMxBlockTiles[] = {{4, 4, "mx_mmt4d_block_256x256"}, {2, 2
                                          {1, 1, "mx_mmt4d_block_64x64"},   {2, 1, "mx_mmt4d_block_128x64"},
                                          {1, 2, "mx_mmt4d_block_64x128"}};
 hipError_t launch_mx_few(const MxProduct& p, int lhs_bits, int shape, hipStream_t stream);
+// The one that keeps up to 16 rows of up to kMxResidentChunks chunks in registers, with this many workgroups.
+constexpr uint32_t kMxResidentChunks = 64, kMxResidentGroups = 256;
+hipError_t launch_mx_resident(const MxProduct& p, int lhs_bits, hipStream_t stream);
 hipError_t launch_mx_block_e2m1(const MxProduct& p, int tile, hipStream_t stream);
 hipError_t launch_mx_block_e4m3(const MxProduct& p, int tile, hipStream_t stream);
 hipError_t launch_mx_block_e4m3_f32(const MxProduct& p, int tile, hipStream_t stream);

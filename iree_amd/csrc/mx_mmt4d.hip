@@ -107,9 +107,9 @@ bool as_product(const MxMmt4dArgs& a, MxProduct* p) {
   return true;
 }
 
-// Whether rows up to 256 apart lie within 32 bits of each other.
-bool near(const MxOperand& o) {
-  const int64_t panels = 256 / o.tile_rows + 2, most = 1ll << 31;
+// Whether rows up to 256 (or `apart`) apart lie within 32 bits of each other.
+bool near(const MxOperand& o, int64_t apart = 256) {
+  const int64_t panels = apart / o.tile_rows + 2, most = 1ll << 31;
   return o.stride0 < most / panels && o.scales_stride0 < most / panels;
 }
 
@@ -131,10 +131,12 @@ bool block_covers(const MxProduct& p) {
 // Sixteen rows of a chunk straight into registers take 19 to 21 ns a KiB where they lie in a tile, 5 to 20 where they are one row to
 // sixteen rows of a matrix (29 of a rhs); through LDS 19 (4 bits) and 12 (8 bits). Fitted to the times of every shape in 660 problems.
 //
+// The lhs in registers: the rhs at 6.1 TB/s, less where wavefronts or workgroups have no part of it.
+//
 // Over these, drawn from 1 to 4096 rows, 64 to 32768 columns, K of 64 to 16384, with tiles and row-major, the kernel taken is
 // slower than the best one by 2 % in the mean.
 struct Choice {
-  enum { kGeneric, kFew, kBlock } kernel;
+  enum { kGeneric, kFew, kResident, kBlock } kernel;
   int number;
 };
 Choice choose(const MxProduct& p, int lhs_bits) {
@@ -169,6 +171,22 @@ Choice choose(const MxProduct& p, int lhs_bits) {
       best = {Choice::kFew, i};
     }
   }
+  // (Up to three rows are read as quickly by every workgroup anew: one of E4M3 x 57000 x 4096 20.1 us, here 21.3; but not beside the
+  // rows of a matrix: x 28672 x 8192 35.4 and 27.3.)
+  if (rows <= 16 && (rows >= 4 || p.rhs.tile_rows < 16) && p.chunks <= kMxResidentChunks && comes_from_hbm(cols * p.chunks * 64)) {
+    const int64_t panels = (cols + 15) / 16, most = (panels + kMxResidentGroups - 1) / kMxResidentGroups;
+    if (lhs_near && near(p.rhs, 16 * most)) {
+      // (Wavefronts without a part of K load nothing, and some workgroups have a panel less than the others.)
+      const float fours = (float)((p.chunks + 3) / 4), held = p.chunks <= 32 ? 8 : 16;
+      const float each = .5f * ((float)most + (float)panels / kMxResidentGroups);
+      const float read = memory / (float)panels * kMxResidentGroups * each / 6.1f * held / fours;
+      const float cost = 2 + 1.5f / most + (eight ? .5f : 0) + read + (split ? .004f * most * p.chunks : 0);
+      if (best.kernel == Choice::kGeneric || cost < least) {
+        least = cost;
+        best = {Choice::kResident, 0};
+      }
+    }
+  }
   if (!block_covers(p)) return best;
   for (int i = 0; i < (int)(sizeof kMxBlockTiles / sizeof kMxBlockTiles[0]); ++i) {
     const MxBlockTile& t = kMxBlockTiles[i];
@@ -195,6 +213,10 @@ hipError_t launch_mx_mmt4d(const MxMmt4dArgs& a, hipStream_t stream, const char*
   if (c.kernel == Choice::kFew) {
     *name = kMxFewShapes[c.number].name;
     return launch_mx_few(p, a.lhs_bits, c.number, stream);
+  }
+  if (c.kernel == Choice::kResident) {
+    *name = "mx_mmt4d_resident";
+    return launch_mx_resident(p, a.lhs_bits, stream);
   }
   *name = kMxBlockTiles[c.number].name;
   if (a.lhs_bits == 4) return launch_mx_block_e2m1(p, c.number, stream);

@@ -205,6 +205,168 @@ __global__ __launch_bounds__(64 * kWaves) void mx_mmt4d_few_kernel(const MxProdu
   }
 }
 
+// Up to 16 rows against a rhs from memory, K up to 8192: a workgroup, one on a compute unit, keeps the lhs in registers, a wavefront
+// its part of K (FOURS times four chunks), and goes through panels of 16 rows of the rhs, AHEAD of which are under way. Sums of
+// PANELS panels at a time meet in LDS, in the order of the wavefronts' numbers.
+//
+// Above, every workgroup loads the lhs anew, next to as many bytes of the rhs with 8-bit codes, and these loads delay the stream: 16
+// rows x 28672 x 8192 take 23.2 us (4 bits) and 25.3 (8 bits), one row 20.4; here 21.0 (6.0 TB/s) and 21.8. Of two workgroups on a
+// unit, with 128 registers a lane, the second's start cost what it gained (21.9; 8 bits 28.5, with spills). A rhs of less than 48 MiB,
+// which the caches may hold, goes faster above: 14336 x 4096 7.5 us, here 8.6. A row-major rhs gains more: 16 x 28672 x 8192 of 8 bits
+// in 27.9 us (42.5).
+template <int LBITS, int FOURS, bool SPLIT>
+__global__ __launch_bounds__(64 * kWaves) void mx_mmt4d_resident_kernel(const MxProduct p) {
+  static_assert(4 * kWaves * 2 == kMxResidentChunks, "two fours at most");
+  constexpr int PANELS = 4, AHEAD = 4 / FOURS;
+  constexpr int ROW = 16 * LBITS, PIECES = ROW / 16, ROWS_OF_LOAD = 64 / PIECES, CHUNK = 16 * ROW, LOADS = CHUNK / 1024;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const uint32_t panels = (p.rhs.rows + 15) / 16;
+  const uint32_t first = (uint32_t)((uint64_t)blockIdx.x * panels / gridDim.x),
+                 end = (uint32_t)((uint64_t)(blockIdx.x + 1) * panels / gridDim.x);
+
+  MxFragment<4> b[AHEAD][FOURS][4];
+  MxFragment<LBITS> a[FOURS][4];
+  uint32_t as[FOURS], b_loaded[AHEAD][FOURS];
+  auto chunk_of = [&](int f, int u) { return (uint32_t)(4 * (wave + f * kWaves) + u); };
+  auto inside = [&](uint32_t chunk) { return chunk < p.chunks ? chunk : p.chunks - 1; };
+  // Offsets of a lane from the panel of tiles that the workgroup begins in.
+  const uint32_t first_panel = divide(16 * first, p.rhs.tile_rows, p.rhs.tile_reciprocal);
+  const uint8_t* const codes = p.rhs.codes + first_panel * p.rhs.stride0;
+  const uint8_t* const scales = p.rhs.scales + first_panel * p.rhs.scales_stride0;
+  uint32_t codes_at, scales_at;
+  auto to_panel = [&](uint32_t panel) {
+    const uint32_t at = 16 * panel + r, row = at < p.rhs.rows ? at : p.rhs.rows - 1;
+    const uint32_t of = divide(row, p.rhs.tile_rows, p.rhs.tile_reciprocal), in = row - of * p.rhs.tile_rows;
+    codes_at = (uint32_t)((of - first_panel) * p.rhs.stride0) + in * 64 + 16 * g;
+    scales_at = (uint32_t)((of - first_panel) * p.rhs.scales_stride0) + in * 4;
+  };
+  auto load = [&](int d, int f, int u) {
+    const uint8_t* const from = codes + inside(chunk_of(f, u)) * (64 * (int64_t)p.rhs.tile_rows);
+    const mx_v4f32 v = __builtin_nontemporal_load((const mx_v4f32*)(from + codes_at));
+    __builtin_memcpy(b[d][f][u].w, &v, 16);
+  };
+  auto load_scales = [&](int d, int f) {
+    b_loaded[d][f] = *(const uint32_t*)(scales + scales_at + inside(chunk_of(f, 0) + g) * (4 * (int64_t)p.rhs.tile_rows));
+  };
+
+  // The lhs, by way of LDS (as above). Chunks behind the last are zeros with a scale of one.
+  auto exchanged = [](uint32_t row) { return LBITS == 4 ? ((row >> 2) & 3) ^ (row & 2) : ((row >> 1) & 7) ^ ((row & 1) << 2); };
+  const int64_t lhs_step = ROW * (int64_t)p.lhs.tile_rows;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)few_lds + wave * (FOURS * 4 * CHUNK);
+  const uint8_t* const staged = (const uint8_t*)few_lds + wave * (FOURS * 4 * CHUNK) + r * ROW;
+  uint32_t a_loaded[FOURS];
+#pragma unroll
+  for (int n = 0; n < LOADS; ++n) {
+    const uint32_t at = n * ROWS_OF_LOAD + lane / PIECES;
+    const uint32_t from = (uint32_t)mx_row_codes<LBITS>(p.lhs, at < p.lhs.rows ? at : p.lhs.rows - 1) + 16 * ((lane % PIECES) ^ exchanged(at));
+#pragma unroll
+    for (int f = 0; f < FOURS; ++f)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        load_pieces(lds0 + (f * 4 + u) * CHUNK + n * 1024, from, p.lhs.codes + inside(chunk_of(f, u)) * lhs_step);
+  }
+  {
+    const uint8_t* const lhs_scales = p.lhs.scales + mx_row_scales(p.lhs, (uint32_t)r < p.lhs.rows ? r : p.lhs.rows - 1);
+#pragma unroll
+    for (int f = 0; f < FOURS; ++f) {
+      const uint32_t chunk = chunk_of(f, 0) + g;
+      a_loaded[f] = *(const uint32_t*)(lhs_scales + inside(chunk) * (4 * (int64_t)p.lhs.tile_rows));
+      if (chunk >= p.chunks) a_loaded[f] = 0x7F7F7F7Fu;
+    }
+  }
+  // (Loads behind those to LDS, none of which is counted on.)
+#pragma unroll
+  for (int d = 0; d < AHEAD; ++d) {
+    if (first + d >= end) break;
+    to_panel(first + d);
+#pragma unroll
+    for (int f = 0; f < FOURS; ++f) {
+      load_scales(d, f);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) load(d, f, u);
+    }
+  }
+  wait_loads<0>();
+#pragma unroll
+  for (int f = 0; f < FOURS; ++f) {
+    as[f] = scales_of_blocks(a_loaded[f], g);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint8_t* const row = staged + (f * 4 + u) * CHUNK;
+      *(uint4*)a[f][u].w = *(const uint4*)(row + 16 * (g ^ exchanged(r)));
+      if constexpr (LBITS == 8) *(uint4*)(a[f][u].w + 4) = *(const uint4*)(row + 16 * ((4 + g) ^ exchanged(r)));
+      if (chunk_of(f, u) >= p.chunks) a[f][u] = {};
+    }
+  }
+  // Everyone's LDS writes and reads have ended. (No wait for loads: they go on.)
+  auto meet = [] {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  meet();
+
+  mx_v4f32* const partial = (mx_v4f32*)few_lds;  // [2][PANELS][kWaves][64], the halves in turn
+  uint32_t half = 0, held = 0;
+  for (uint32_t group = first; group < end; group += AHEAD) {
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) {
+      const uint32_t panel = group + d;
+      if (panel >= end) break;
+      mx_v4f32 acc = {};
+      const bool more = panel + AHEAD < end;
+      auto multiply = [&](int f, auto number, uint32_t bs) {
+        constexpr int U = decltype(number)::value;
+        if constexpr (SPLIT) {
+          MxFragment<8> whole = a[f][U], high, low;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(whole.w[i]));  // (or both parts are kept in registers)
+          mx_split(whole, high, low);
+          acc = mx_mfma_16<4, 8, U>(b[d][f][U], bs, high, as[f], acc);
+          acc = mx_mfma_16<4, 8, U>(b[d][f][U], bs, low, as[f], acc);
+        } else {
+          acc = mx_mfma_16<4, LBITS, U>(b[d][f][U], bs, a[f][U], as[f], acc);
+        }
+      };
+      auto of_panel = [&](auto loads) {
+#pragma unroll
+        for (int f = 0; f < FOURS; ++f) {
+          const uint32_t bs = scales_of_blocks(b_loaded[d][f], g);
+          if constexpr (decltype(loads)::value) load_scales(d, f);
+          auto one = [&](auto u) {
+            multiply(f, u, bs);
+            if constexpr (decltype(loads)::value) load(d, f, decltype(u)::value);
+          };
+          one(std::integral_constant<int, 0>{});
+          one(std::integral_constant<int, 1>{});
+          one(std::integral_constant<int, 2>{});
+          one(std::integral_constant<int, 3>{});
+        }
+      };
+      if (more) {
+        to_panel(panel + AHEAD);
+        of_panel(std::true_type{});
+      } else {
+        of_panel(std::false_type{});
+      }
+      partial[((half * PANELS + held) * kWaves + wave) * 64 + lane] = acc;
+      if (++held == PANELS || panel + 1 == end) {
+        meet();
+        for (uint32_t n = wave; n < held; n += kWaves) {
+          const mx_v4f32* const of = partial + (half * PANELS + n) * kWaves * 64 + lane;
+          mx_v4f32 v = of[0];
+#pragma unroll
+          for (int w = 1; w < kWaves; ++w) v += of[w * 64];
+          if ((uint32_t)r < p.lhs.rows) mx_store_four(p, mx_out_row(p, r), 16 * (panel + 1 - held + n) + 4 * g, v);
+        }
+        half ^= 1;
+        held = 0;
+      }
+    }
+  }
+}
+
 template <int LBITS, int MT, int NT, bool STAGED>
 hipError_t launch(const MxProduct& p, hipStream_t stream) {
   const dim3 grid((p.rhs.rows + 16 * NT - 1) / (16 * NT), (p.lhs.rows + 16 * MT - 1) / (16 * MT));
@@ -223,6 +385,21 @@ hipError_t launch(const MxProduct& p, hipStream_t stream) {
     if (e != hipSuccess) return e;
   }
   return hipLaunchKernel(kernel, grid, dim3(64 * kWaves), args, LDS, stream);
+}
+
+template <int LBITS, int FOURS>
+hipError_t launch_resident(const MxProduct& p, hipStream_t stream) {
+  const bool split = LBITS == 8 && p.out_type == Float::kF32;
+  const void* kernel = split ? (const void*)mx_mmt4d_resident_kernel<LBITS, FOURS, LBITS == 8>
+                             : (const void*)mx_mmt4d_resident_kernel<LBITS, FOURS, false>;
+  constexpr int SUMS = 2 * 4 * kWaves * 1024, LHS = kWaves * FOURS * 4 * 256 * LBITS, LDS = SUMS > LHS ? SUMS : LHS;
+  if (LDS > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e != hipSuccess) return e;
+  }
+  const uint32_t panels = (p.rhs.rows + 15) / 16;
+  void* args[] = {const_cast<MxProduct*>(&p)};
+  return hipLaunchKernel(kernel, dim3(panels < kMxResidentGroups ? panels : kMxResidentGroups), dim3(64 * kWaves), args, LDS, stream);
 }
 
 template <int LBITS>
@@ -245,6 +422,11 @@ hipError_t launch_of(const MxProduct& p, int shape, hipStream_t stream) {
 
 hipError_t launch_mx_few(const MxProduct& p, int lhs_bits, int shape, hipStream_t stream) {
   return lhs_bits == 4 ? launch_of<4>(p, shape, stream) : launch_of<8>(p, shape, stream);
+}
+
+hipError_t launch_mx_resident(const MxProduct& p, int lhs_bits, hipStream_t stream) {
+  if (p.chunks <= 32) return lhs_bits == 4 ? launch_resident<4, 1>(p, stream) : launch_resident<8, 1>(p, stream);
+  return lhs_bits == 4 ? launch_resident<4, 2>(p, stream) : launch_resident<8, 2>(p, stream);
 }
 
 }  // namespace uk

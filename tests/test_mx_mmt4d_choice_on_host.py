@@ -106,7 +106,16 @@ KERNELS = [
     ("e4m3", "f32", 1, 8232, 4608, 1, 1, "few_16x64"),
 ]
 
-# The same, and microseconds of the four best kernels.
+# The same for the kernel that keeps the lhs in registers: whole and partial shares of K, rows and columns, matrices and tiles.
+RESIDENT = [
+    ("e2m1", "f32", 16, 28672, 8192, 1, 16), ("e2m1", "f16", 9, 33008, 4096, 1, 16), ("e2m1", "bf16", 13, 28672, 8064, 1, 16),
+    ("e2m1", "f32", 16, 57000, 4096, 16, 1), ("e2m1", "bf16", 5, 40001, 3200, 1, 1), ("e2m1", "f16", 4, 33001, 4096, 1, 1),
+    ("e4m3", "bf16", 16, 28672, 8192, 1, 16), ("e4m3", "f16", 16, 57008, 4096, 16, 16), ("e4m3", "bf16", 1, 28672, 8064, 1, 1),
+    ("e4m3", "f32", 16, 28672, 8192, 16, 16), ("e4m3", "f32", 9, 40000, 3200, 1, 16), ("e4m3", "f32", 3, 28675, 8192, 1, 1),
+    ("e4m3", "f32", 8, 33008, 4096, 1, 8),
+]
+
+# The same as above, and microseconds of the four best kernels.
 TIMES = [
     ("e2m1", "f16", 352, 8653, 3584, 16, 1, {"block_128x128": 20.17, "block_128x64": 21.10, "block_64x128": 25.58, "block_128x192": 26.14}),
     ("e2m1", "f16", 723, 6288, 6912, 1, 16, {"block_128x192": 27.07, "block_128x256": 29.82, "block_128x128": 34.54, "block_64x128": 39.86}),
@@ -155,6 +164,11 @@ def test_every_kernel_is_picked(recorder, lhs, out, rows, cols, k, m0, n0, kerne
     assert picked(recorder, lhs, out, rows, cols, k, m0, n0) == kernel
 
 
+@pytest.mark.parametrize("lhs,out,rows,cols,k,m0,n0", RESIDENT)
+def test_the_lhs_stays_in_registers(recorder, lhs, out, rows, cols, k, m0, n0):  # noqa: F811
+    assert picked(recorder, lhs, out, rows, cols, k, m0, n0) == "resident"
+
+
 @pytest.mark.parametrize("lhs,out,rows,cols,k,m0,n0,times", TIMES, ids=lambda v: "times" if isinstance(v, dict) else str(v))
 def test_the_kernel_picked_is_among_the_best(recorder, lhs, out, rows, cols, k, m0, n0, times):  # noqa: F811
     name = picked(recorder, lhs, out, rows, cols, k, m0, n0)
@@ -191,8 +205,8 @@ def test_what_the_fast_kernels_do_not_take(recorder, change, kernel):  # noqa: F
 @pytest.mark.parametrize("tiles,tile,kernel", [
     # More rows of 16 or 32 than a grid has, in tiles that no block kernel takes; more columns than it has threads for.
     ((1 << 20, 1, 1), (4, 16, 128), "generic"), ((1 << 16, 1, 1), (4, 16, 128), "few"),
-    ((1, 1 << 30, 1), (2, 1, 128), "generic"), ((1, 1 << 24, 1), (2, 1, 128), "few"),
-    ((1, 1 << 30, 1), (1, 1, 128), "generic"), ((1 << 22, 1, 1), (1, 16, 128), "block")])
+    ((10, 1 << 30, 1), (2, 1, 128), "generic"), ((10, 1 << 24, 1), (2, 1, 128), "few"),
+    ((10, 1 << 30, 1), (1, 1, 128), "resident"), ((1 << 22, 1, 1), (1, 16, 128), "block")])
 def test_grids_of_any_size(recorder, tiles, tile, kernel):  # noqa: F811
     p = ref.mmt4d_params(1 << 36, 2 << 39, 3 << 39, 4 << 39, 5 << 39, tiles, tile, "e4m3", "f32")
     _, name = recorder.call("iree_uk_mi355x_mx_mmt4d_p", p)
