@@ -179,8 +179,13 @@ __device__ __forceinline__ void load_end(MxEight<T>& v, const uint8_t* row, int 
 
 // LANES lanes (64, or the workgroup) to a row of up to 8 * LANES * PIECES values; WEIGHT: the weight's type.
 //
-// 4096 rows of 8192 bf16 values, with a residual, to E4M3 (236 MB): 52.4 us, 4.5 TB/s; with 256 lanes of four pieces 55.0 (140
-// registers, three wavefronts on a SIMD), with 1024 of one 54.7; with a branch in front of every load 59.7.
+// 4096 rows of 8192 bf16 values, with a residual, to E4M3 (236 MB): 47.0 us, 5.0 TB/s. With the sum stored through the caches 52.4; of
+// that form, 256 lanes of four pieces took 55.0 (140 registers, three wavefronts on a SIMD), 1024 of one 54.7, and a branch in
+// front of every load 59.7.
+//
+// Sums of 16-bit types of more than 24 MiB go past the caches: also where 100 MB of other traffic and then a kernel that reads the
+// sum follow, 96 us instead of 104 (2048 rows 55 and 59; 512 rows, the other way, 25.3 and 24.9). Of f32 a lane's eight values
+// are two stores with gaps between the lanes, which lose more past the caches than there is to gain.
 template <Float T, Float WEIGHT, NormOut OUT, int LANES, int PIECES>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void rms_norm_row(const RmsNormArgs a) {
   constexpr int WAVES = LANES / 64, ROWS = LANES < 256 ? 256 / LANES : 1, SIZE = T == Float::kF32 ? 4 : 2;
@@ -221,14 +226,21 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void rms_norm_row(const 
         mx_widen_eight<T>(old[p], o);
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[p][i] += o[i];
+        MxEight<T> rounded;
         if constexpr (T != Float::kF32) {
-          MxEight<T> rounded;
 #pragma unroll
           for (int i = 0; i < 4; ++i) rounded.w[i] = mx_narrow_pair<T>(s[p][2 * i], s[p][2 * i + 1]);
           mx_widen_eight<T>(rounded, s[p]);
         }
-        if (a.sum && col < size)
-          mx_store_eight<T>(a.sum + (row * a.sum_stride0 + col) * SIZE, s[p], size - col);
+        if (a.sum && col < size) {
+          uint8_t* const to = a.sum + (row * a.sum_stride0 + col) * SIZE;
+          if constexpr (T != Float::kF32) {
+            if (a.stream_sum && size - col >= 8) mx_store_sixteen<true>(to, rounded.w);
+            else mx_store_eight<T>(to, s[p], size - col);
+          } else {
+            mx_store_eight<T>(to, s[p], size - col);
+          }
+        }
       }
       part[p] = 0;
 #pragma unroll
@@ -387,7 +399,10 @@ hipError_t launch_of(const RmsNormArgs& a, hipStream_t stream, const char** name
 
 }  // namespace
 
-hipError_t launch_rms_norm(const RmsNormArgs& a, hipStream_t stream, const char** name) {
+hipError_t launch_rms_norm(const RmsNormArgs& given, hipStream_t stream, const char** name) {
+  RmsNormArgs a = given;
+  const int e = float_bytes(a.type);
+  a.stream_sum = a.size0 * a.size1 * e > (24ll << 20) && (uintptr_t)a.sum % 16 == 0 && a.sum_stride0 * e % 16 == 0;
   const bool f32 = a.weight_type == Float::kF32;
   switch (a.type) {
     case Float::kF32: return launch_of<Float::kF32, Float::kF32>(a, stream, name);

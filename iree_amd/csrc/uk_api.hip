@@ -1330,7 +1330,7 @@ UK_API void iree_uk_mi355x_rms_norm_p(const iree_uk_mi355x_rms_norm_params_t* p)
   a.out_stride0 = out_region.pitch; a.scales_stride0 = scales_region.pitch;
   a.size0 = p->size0; a.size1 = p->size1; a.out_size1 = p->out_size1;
   a.epsilon = p->epsilon;
-  a.type = type; a.weight_type = weight_type; a.out_type = out_type;
+  a.type = type; a.weight_type = weight_type; a.out_type = out_type; a.stream_sum = false;
   if (!launch_ok(uk::launch_rms_norm(a, stream, &tl_last_kernel), "rms_norm")) {
     abandon(stager, stream);
     return;

@@ -107,6 +107,7 @@ struct RmsNormArgs {
   float epsilon;
   Float type, weight_type;
   NormOut out_type;
+  bool stream_sum;  // past the caches; the launcher's
 };
 
 // Enqueues a kernel that takes one argument struct. (Half a hundred nanoseconds each of the triple-bracket form's

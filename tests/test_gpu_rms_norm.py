@@ -221,3 +221,31 @@ def test_rows_beyond_32_bits(gpu_lib, format):
     for all_rows, last, one in zip(everything, alone, first):
         assert torch.equal(all_rows[-few:], last)
         assert bool((all_rows[:-few] == one).all())
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("cols,pitch", [(4092, 4096), (4096, 4096), (4096, 4100)])
+def test_sums_that_go_past_the_caches(gpu_lib, type, cols, pitch):
+    # 28 MB in rows of whole or broken eights, aligned or not: the sum is torch's, codes are those of a few rows by themselves.
+    rows, few, out_cols = 3400, 20, 4096
+    dtype = torch.float16 if type == "f16" else torch.bfloat16
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x, residual = (torch.randn(rows, pitch, generator=gen, device="cuda").to(dtype) for _ in range(2))
+
+    def call(first, n):
+        total = torch.full((n, pitch), 7.0, dtype=dtype, device="cuda")
+        codes = torch.zeros(n, out_cols, dtype=torch.uint8, device="cuda")
+        scales = torch.zeros(n, out_cols // 32, dtype=torch.uint8, device="cuda")
+        p = ref.norm_params(x[first].data_ptr(), residual[first].data_ptr(), total.data_ptr(), None, codes.data_ptr(),
+                            scales.data_ptr(), n, cols, out_cols, type, "e4m3")
+        p.in_stride0 = p.residual_stride0 = p.sum_stride0 = pitch
+        gpu_lib.iree_uk_mi355x_rms_norm_p(C.byref(p))
+        return total, codes, scales
+
+    total, codes, scales = call(0, rows)
+    want = (x.float() + residual.float()).to(dtype)
+    want[:, cols:] = 7.0
+    assert torch.equal(total, want)
+    for first in (0, rows - few):
+        alone = call(first, few)
+        assert torch.equal(codes[first:first + few], alone[1]) and torch.equal(scales[first:first + few], alone[2])
