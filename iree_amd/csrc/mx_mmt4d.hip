@@ -124,12 +124,12 @@ bool block_covers(const MxProduct& p) {
 //
 // Block tiles: a start, and chunks of K times what one of them takes with one workgroup on a compute unit and, where LDS and
 // registers hold two, with two; more workgroups than that follow each other. From the times of every tile with 128 to 1024 of
-// them, row-major lhs, K = 1024 and 5120.
+// them, row-major lhs, K = 1024 and 5120. The rhs comes from memory beside that.
 //
 // Few rows: a workgroup's loads and its matrix instructions (and, with more workgroups than compute units, what a start costs again),
 // or the rhs from memory at 6.4 TB/s with a share of what the loads of the lhs take, whichever is more, and a part of the other.
-// Sixteen rows of a chunk straight into registers take 19 to 21 ns a KiB where they lie in a tile, 5 to 20 where they are one row to
-// sixteen rows of a matrix (29 of a rhs); through LDS 19 (4 bits) and 12 (8 bits). Fitted to the times of every shape in 660 problems.
+// Sixteen rows of a chunk straight into registers take 19 to 23 ns a KiB where they lie in a tile, 5 to 20 where they are one row to
+// sixteen rows of a matrix (30 of a rhs); through LDS 19 (4 bits) and 11 (8 bits). Fitted to the times of every shape in 880 problems.
 //
 // The lhs in registers: the rhs at 6.1 TB/s, less where wavefronts or workgroups have no part of it.
 //
@@ -152,20 +152,20 @@ Choice choose(const MxProduct& p, int lhs_bits) {
   Choice best = {Choice::kGeneric, 0};
   float least = 0;
   const bool eight = lhs_bits == 8, split = times == kE4m3F32, lhs_near = near(p.lhs);
-  const float row_major = (eight ? 2 : 1) * (.0049f + .0147f * (float)(rows < 16 ? rows - 1 : 15) / 15);
-  const float lhs_direct = p.lhs.tile_rows >= 16 && !eight ? .0186f : row_major, lhs_staged = eight ? .0232f : .0185f;
-  const float rhs_chunk = p.rhs.tile_rows >= 16 ? .0209f : .0292f, product = split ? .0127f : .0008f;
+  const float row_major = (eight ? 2 : 1) * (.0049f + .0151f * (float)(rows < 16 ? rows - 1 : 15) / 15);
+  const float lhs_direct = p.lhs.tile_rows >= 16 && !eight ? .019f : row_major, lhs_staged = eight ? .0237f : .0188f;
+  const float rhs_chunk = p.rhs.tile_rows >= 16 ? .0232f : .0295f, product = split ? .0105f : .0003f;
   const float memory = (float)cols * p.chunks * 68e-6f;
   for (int i = 0; i < (int)(sizeof kMxFewShapes / sizeof kMxFewShapes[0]); ++i) {
     const MxFewShape& s = kMxFewShapes[i];
     const int64_t down = (rows + 16 * s.mt - 1) / (16 * s.mt), across = (cols + 16 * s.nt - 1) / (16 * s.nt);
     // (A grid has fewer than 2^32 threads, and 2^16 rows.)
     if (down > 65535 || down * across > (1 << 22) || (s.staged && !lhs_near)) continue;
-    const float rounds = (float)((down * across + 255) / 256), start = 1.96f + .27f * s.mt * s.nt;
+    const float rounds = (float)((down * across + 255) / 256), start = 1.94f + .286f * s.mt * s.nt;
     const float lhs = s.mt * (s.staged ? lhs_staged : lhs_direct) * p.chunks;
-    const float loads = rounds * (lhs + (s.nt * rhs_chunk + s.mt * s.nt * product) * p.chunks) + (rounds - 1) * .364f * start;
-    const float streamed = memory / 6.38f + .148f / 256 * (float)(down * across) * lhs;
-    const float cost = start + (loads > streamed ? loads + .093f * streamed : streamed + .093f * loads);
+    const float loads = rounds * (lhs + (s.nt * rhs_chunk + s.mt * s.nt * product) * p.chunks) + (rounds - 1) * .321f * start;
+    const float streamed = memory / 6.41f + .137f / 256 * (float)(down * across) * lhs;
+    const float cost = start + (loads > streamed ? loads + .115f * streamed : streamed + .115f * loads);
     if (best.kernel == Choice::kGeneric || cost < least) {
       least = cost;
       best = {Choice::kFew, i};
@@ -193,8 +193,8 @@ Choice choose(const MxProduct& p, int lhs_bits) {
     const int64_t tiles = ((rows + 64 * t.am - 1) / (64 * t.am)) * ((cols + 64 * t.bn - 1) / (64 * t.bn)), rounds = (tiles + 255) / 256;
     if (tiles > (1 << 23)) continue;
     const float steps = p.chunks * ((rounds >> 1) * times[i].two + (rounds & 1) * times[i].one);
-    const float read = memory / 5.8f;
-    const float cost = times[i].start + (rounds - 1) * times[i].start_again + (steps > read ? steps : read) + .15f * read;
+    const float read = memory / 7.2f;
+    const float cost = times[i].start + (rounds - 1) * times[i].start_again + (steps > read ? steps + .116f * read : read + .182f * steps);
     if (best.kernel == Choice::kGeneric || cost < least) {
       least = cost;
       best = {Choice::kBlock, i};

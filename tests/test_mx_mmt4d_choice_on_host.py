@@ -24,7 +24,7 @@ KERNELS = [
     ("e2m1", "bf16", 357, 688, 128, 1, 16, "few_16x64_staged"),
     ("e2m1", "f32", 202, 310, 128, 1, 1, "few_32x16_staged"),
     ("e2m1", "f32", 394, 331, 128, 1, 1, "few_32x32_staged"),
-    ("e2m1", "bf16", 832, 320, 1024, 16, 16, "few_32x64_staged"),
+    ("e2m1", "bf16", 459, 640, 1280, 1, 16, "few_32x64_staged"),
     ("e4m3", "bf16", 1584, 1312, 128, 16, 16, "block_128x128"),
     ("e4m3", "bf16", 1824, 2221, 128, 16, 1, "block_128x192"),
     ("e4m3", "bf16", 2206, 2880, 1152, 1, 16, "block_128x256"),
@@ -40,7 +40,7 @@ KERNELS = [
     ("e4m3", "bf16", 226, 1078, 128, 1, 1, "few_16x64_staged"),
     ("e4m3", "bf16", 214, 302, 128, 1, 1, "few_32x16_staged"),
     ("e4m3", "bf16", 336, 389, 128, 16, 1, "few_32x32_staged"),
-    ("e4m3", "bf16", 903, 352, 768, 1, 16, "few_32x64_staged"),
+    ("e4m3", "bf16", 470, 560, 1024, 1, 16, "few_32x64_staged"),
     ("e4m3", "f32", 2732, 2182, 128, 1, 1, "block_128x128"),
     ("e4m3", "f32", 2582, 1584, 128, 1, 16, "block_128x192"),
     ("e4m3", "f32", 3081, 1968, 1664, 1, 16, "block_128x256"),
@@ -56,7 +56,7 @@ KERNELS = [
     ("e4m3", "f32", 304, 816, 128, 16, 16, "few_16x64_staged"),
     ("e4m3", "f32", 288, 253, 128, 16, 1, "few_32x16_staged"),
     ("e4m3", "f32", 414, 309, 128, 1, 1, "few_32x32_staged"),
-    ("e4m3", "f32", 472, 592, 384, 1, 16, "few_32x64_staged"),
+    ("e4m3", "f32", 565, 523, 512, 1, 1, "few_32x64_staged"),
     ("e2m1", "bf16", 1699, 1254, 896, 1, 1, "block_128x128"),
     ("e2m1", "f32", 2576, 1551, 896, 16, 1, "block_128x192"),
     ("e2m1", "f32", 2744, 2504, 896, 8, 8, "block_128x256"),
@@ -103,7 +103,7 @@ KERNELS = [
     ("e4m3", "f32", 344, 389, 4480, 8, 1, "few_32x32_staged"),
     ("e4m3", "f32", 464, 616, 4480, 16, 8, "few_32x64_staged"),
     ("e4m3", "bf16", 1, 8232, 4608, 1, 1, "few_16x64"),
-    ("e4m3", "f32", 1, 8232, 4608, 1, 1, "few_16x64"),
+    ("e4m3", "f32", 3, 8240, 4608, 1, 1, "few_16x64"),
 ]
 
 # The same for the kernel that keeps the lhs in registers: whole and partial shares of K, rows and columns, matrices and tiles.
