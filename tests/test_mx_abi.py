@@ -1,5 +1,8 @@
 """What the microscaled operators and the norm refuse, and what they return from early: no GPU needed."""
 import ctypes as C
+import os
+import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -132,3 +135,27 @@ def test_reference_quantiser_rounds_to_nearest_even():
     x[0, :3] = [448, 464, -500]
     codes, scales = ref.quantise(x, "e4m3")
     assert scales[0, 0] == 127 and codes[0, :3].tolist() == [126, 126, 254]
+
+
+def test_structs_and_flags_match_the_header(tmp_path):
+    structs = {"mx_pack": abi.MxPackParams, "mx_unpack": abi.MxUnpackParams, "mx_mmt4d": abi.MxMmt4dParams,
+               "rms_norm": abi.RmsNormParams}
+    flags = [n for n in vars(abi) if re.match(r"(MX_PACK|MX_UNPACK|MX_MMT4D|RMS_NORM)_", n)]
+    lines, want = [], []
+    for name, struct in structs.items():
+        c = "iree_uk_mi355x_%s_params_t" % name
+        lines.append('printf("%%zu\\n", sizeof(%s));' % c)
+        want.append(C.sizeof(struct))
+        for field, _ in struct._fields_:
+            lines.append('printf("%%zu\\n", offsetof(%s, %s));' % (c, field))
+            want.append(getattr(struct, field).offset)
+    for flag in flags:
+        lines.append('printf("%%d\\n", (int)IREE_UK_MI355X_FLAG_%s);' % flag)
+        want.append(getattr(abi, flag))
+    source, program = tmp_path / "layout.c", tmp_path / "layout"
+    source.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "iree_uk_mi355x.h"\nint main(void) {\n%s\nreturn 0;\n}\n' %
+                      "\n".join(lines))
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-I" + include, str(source), "-o", str(program)], check=True)
+    got = subprocess.run([str(program)], check=True, stdout=subprocess.PIPE, text=True).stdout.split()
+    assert [int(x) for x in got] == want and len(flags) == 29
