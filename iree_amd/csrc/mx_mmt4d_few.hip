@@ -37,7 +37,7 @@ __device__ __forceinline__ void wait_loads() {
 //
 // STAGED: the lhs goes through LDS, a wavefront's own part of it, where a row's pieces are exchanged among themselves for the
 // banks' sake. Straight into registers a load's neighbouring lanes have 16 rows, 16 cache lines, and take 31 ns a KiB; to LDS
-// eight (sixteen) neighbouring lanes have one row: 8.5 ns. Against the same shapes without: 32 rows x 4096 columns x 14336 in
+// four (eight) neighbouring lanes have one row: 8.5 ns. Against the same shapes without: 32 rows x 4096 columns x 14336 in
 // 8.8 us (4-bit lhs; 12.4 at best), 128 x 4096 x 4096 in 7.2 (8.5; 8-bit 8.4, 11.3), 128 x 4096 x 14336 in 15.1 (22.8).
 template <int LBITS, int MT, int NT, bool STREAM, bool SPLIT, bool STAGED>
 __global__ __launch_bounds__(64 * kWaves) void mx_mmt4d_few_kernel(const MxProduct p) {
