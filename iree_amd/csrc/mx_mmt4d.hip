@@ -134,7 +134,8 @@ bool block_covers(const MxProduct& p) {
 // The lhs in registers: the rhs at 6.1 TB/s, less where wavefronts or workgroups have no part of it.
 //
 // Over these, drawn from 1 to 4096 rows, 64 to 32768 columns, K of 64 to 16384, with tiles and row-major, the kernel taken is
-// slower than the best one by 2 % in the mean.
+// slower than the best one by 2 % in the mean. For 16-bit results of an E4M3 lhs the constants are those of products with one matrix
+// instruction each, not two: 3.5 % in the mean of 101 problems, from 1 to 4096 rows (1.4 % with those of f32 results).
 struct Choice {
   enum { kGeneric, kFew, kResident, kBlock } kernel;
   int number;
@@ -171,8 +172,8 @@ Choice choose(const MxProduct& p, int lhs_bits) {
       best = {Choice::kFew, i};
     }
   }
-  // (Up to three rows are read as quickly by every workgroup anew: one of E4M3 x 57000 x 4096 20.1 us, here 21.3; but not beside the
-  // rows of a matrix: x 28672 x 8192 35.4 and 27.3.)
+  // (Up to three rows are read as quickly by every workgroup anew: one of E4M3 x 57008 x 4096 22.0 us, here 24.0; but not beside the
+  // rows of a matrix: x 28672 x 8192 30.7 and 29.0.)
   if (rows <= 16 && (rows >= 4 || p.rhs.tile_rows < 16) && p.chunks <= kMxResidentChunks && comes_from_hbm(cols * p.chunks * 64)) {
     const int64_t panels = (cols + 15) / 16, most = (panels + kMxResidentGroups - 1) / kMxResidentGroups;
     if (lhs_near && near(p.rhs, 16 * most)) {
@@ -219,8 +220,7 @@ hipError_t launch_mx_mmt4d(const MxMmt4dArgs& a, hipStream_t stream, const char*
     return launch_mx_resident(p, a.lhs_bits, stream);
   }
   *name = kMxBlockTiles[c.number].name;
-  if (a.lhs_bits == 4) return launch_mx_block_e2m1(p, c.number, stream);
-  return p.out_type == Float::kF32 ? launch_mx_block_e4m3_f32(p, c.number, stream) : launch_mx_block_e4m3(p, c.number, stream);
+  return a.lhs_bits == 4 ? launch_mx_block_e2m1(p, c.number, stream) : launch_mx_block_e4m3(p, c.number, stream);
 }
 
 }  // namespace uk

@@ -155,7 +155,7 @@ constexpr int lds_bytes(int lbits, int am, int bn, int stages, bool grouped) {
 // GROUPED: the lhs is row-major. A chunk's scales are then four bytes of each row, a cache line each, and a load takes a cycle for
 // every line that it touches: 64 rows, 64 cycles, where 16 bytes a lane take 16. So they come four chunks at a time, 16 bytes
 // of a row, sixteen rows with each chunk's loads and a whole group of four chunks ahead of its use.
-template <int LBITS, int AM, int BN, int STAGES, bool SPLIT, bool GROUPED>
+template <int LBITS, int AM, int BN, int STAGES, bool GROUPED>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AM * BN <= 8 && lds_bytes(LBITS, AM, BN, STAGES, GROUPED) <= 80 * 1024 ? 2 : 1, 2)))
 void mx_mmt4d_block_kernel(const MxProduct p) {
   constexpr int ROWS = 64 * AM, COLS = 64 * BN;
@@ -308,6 +308,7 @@ void mx_mmt4d_block_kernel(const MxProduct p) {
   mx_v16f32 acc[AM][BN] = {};
   // A step's MFMAs, and R reads and L loads (numbered) dealt out among them: a wavefront issues in order, what stands in front
   // of an MFMA keeps the matrix pipe waiting, and a load stands there for 16 cycles of every wavefront's.
+  constexpr bool SPLIT = LBITS == 8;  // (mx_split)
   constexpr int MFMAS = AM * BN * (SPLIT ? 2 : 1);
   auto multiply = [&](auto step, auto read_count, auto read_one, auto load_count, auto load_one) {
     constexpr int S = decltype(step)::value, R = decltype(read_count)::value, L = decltype(load_count)::value;
@@ -371,14 +372,13 @@ void mx_mmt4d_block_kernel(const MxProduct p) {
     for (int j = 0; j < BN; ++j) asm volatile("" : "+a"(acc[i][j]));
   const uint32_t row0 = first_row + wave_m * 32 * AM, col0 = first_col + wave_n * 32 * BN;
   if (p.out_type == Float::kF32) store_tile<Float::kF32, AM, BN>(p, acc, row0, col0, lane);
-  else if (SPLIT) {}  // (f32 results only)
   else if (p.out_type == Float::kF16) store_tile<Float::kF16, AM, BN>(p, acc, row0, col0, lane);
   else store_tile<Float::kBf16, AM, BN>(p, acc, row0, col0, lane);
   // (The last loads have reached LDS before it is given to another workgroup.)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <int LBITS, bool SPLIT, int AM, int BN, int STAGES>
+template <int LBITS, int AM, int BN, int STAGES>
 hipError_t launch(MxProduct p, hipStream_t stream) {
   p.tile_rows = (p.lhs.rows + 64 * AM - 1) / (64 * AM);
   p.tile_cols = (p.rhs.rows + 64 * BN - 1) / (64 * BN);
@@ -387,24 +387,24 @@ hipError_t launch(MxProduct p, hipStream_t stream) {
   const bool grouped = p.lhs.tile_rows == 1 && p.chunks >= 4;
   const int lds = lds_bytes(LBITS, AM, BN, STAGES, grouped);
   static_assert(lds_bytes(LBITS, AM, BN, STAGES, true) <= 160 * 1024 && lds_bytes(LBITS, AM, BN, STAGES, false) <= 160 * 1024, "LDS");
-  auto* kernel = grouped ? mx_mmt4d_block_kernel<LBITS, AM, BN, STAGES, SPLIT, true>
-                         : mx_mmt4d_block_kernel<LBITS, AM, BN, STAGES, SPLIT, false>;
+  auto* kernel = grouped ? mx_mmt4d_block_kernel<LBITS, AM, BN, STAGES, true>
+                         : mx_mmt4d_block_kernel<LBITS, AM, BN, STAGES, false>;
   const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
   return launch_kernel(kernel, (tiles + 7) / 8 * 8, 256, lds, stream, p);
 }
 
-template <int LBITS, bool SPLIT>
+template <int LBITS>
 hipError_t launch_block(const MxProduct& p, int tile, hipStream_t stream) {
   constexpr bool FOUR = LBITS == 4;
   switch (tile) {  // kMxBlockTiles
-    case 0: return launch<LBITS, SPLIT, 4, 4, FOUR ? 4 : 3>(p, stream);
-    case 1: return launch<LBITS, SPLIT, 2, 2, FOUR ? 4 : 3>(p, stream);
-    case 2: return launch<LBITS, SPLIT, 2, 3, 3>(p, stream);
-    case 3: return launch<LBITS, SPLIT, 2, 4, FOUR ? 3 : 4>(p, stream);
-    case 4: return launch<LBITS, SPLIT, 1, 1, FOUR ? 6 : 5>(p, stream);
-    case 5: return launch<LBITS, SPLIT, 2, 1, FOUR ? 5 : 3>(p, stream);
-    case 6: return launch<LBITS, SPLIT, 1, 2, FOUR ? 5 : 4>(p, stream);
+    case 0: return launch<LBITS, 4, 4, FOUR ? 4 : 3>(p, stream);
+    case 1: return launch<LBITS, 2, 2, FOUR ? 4 : 3>(p, stream);
+    case 2: return launch<LBITS, 2, 3, 3>(p, stream);
+    case 3: return launch<LBITS, 2, 4, FOUR ? 3 : 4>(p, stream);
+    case 4: return launch<LBITS, 1, 1, FOUR ? 6 : 5>(p, stream);
+    case 5: return launch<LBITS, 2, 1, FOUR ? 5 : 3>(p, stream);
+    case 6: return launch<LBITS, 1, 2, FOUR ? 5 : 4>(p, stream);
   }
   return hipErrorInvalidValue;
 }

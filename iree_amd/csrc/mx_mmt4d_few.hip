@@ -36,10 +36,10 @@ __device__ __forceinline__ void wait_loads() {
 // the last are read as the last one and not stored.
 //
 // STAGED: the lhs goes through LDS, a wavefront's own part of it, where a row's pieces are exchanged among themselves for the
-// banks' sake. Straight into registers a load's neighbouring lanes have 16 rows, 16 cache lines, and take 31 ns a KiB; to LDS
-// four (eight) neighbouring lanes have one row: 8.5 ns. Against the same shapes without: 32 rows x 4096 columns x 14336 in
-// 8.8 us (4-bit lhs; 12.4 at best), 128 x 4096 x 4096 in 7.2 (8.5; 8-bit 8.4, 11.3), 128 x 4096 x 14336 in 15.1 (22.8).
-template <int LBITS, int MT, int NT, bool STREAM, bool SPLIT, bool STAGED>
+// banks' sake. Straight into registers a load's neighbouring lanes have 16 rows, 16 cache lines; to LDS four (eight) neighbouring
+// lanes have one row. The best staged shape against the best without: 32 rows x 4096 columns x 14336 in 8.1 us (9.3; 8-bit lhs 9.5,
+// 13.0), 128 x 4096 x 4096 in 7.4 (9.5; 8.9, 12.2), 128 x 4096 x 14336 in 14.3 (23.7; 17.9, 31.6).
+template <int LBITS, int MT, int NT, bool STREAM, bool STAGED>
 __global__ __launch_bounds__(64 * kWaves) void mx_mmt4d_few_kernel(const MxProduct p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_mmt4d_few_kernel(const MxProdu
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      if constexpr (SPLIT) {
+      if constexpr (LBITS == 8) {
         MxFragment<8> high, low;
         mx_split(a[HELD][i], high, low);
 #pragma unroll
@@ -210,11 +210,11 @@ __global__ __launch_bounds__(64 * kWaves) void mx_mmt4d_few_kernel(const MxProdu
 // PANELS panels at a time meet in LDS, in the order of the wavefronts' numbers.
 //
 // Above, every workgroup loads the lhs anew, next to as many bytes of the rhs with 8-bit codes, and these loads delay the stream: 16
-// rows x 28672 x 8192 take 23.2 us (4 bits) and 25.3 (8 bits), one row 20.4; here 21.0 (6.0 TB/s) and 21.8. Of two workgroups on a
-// unit, with 128 registers a lane, the second's start cost what it gained (21.9; 8 bits 28.5, with spills). A rhs of less than 48 MiB,
-// which the caches may hold, goes faster above: 14336 x 4096 7.5 us, here 8.6. A row-major rhs gains more: 16 x 28672 x 8192 of 8 bits
-// in 27.9 us (42.5).
-template <int LBITS, int FOURS, bool SPLIT>
+// rows x 28672 x 8192 take 22.7 us (4 bits) and 25.9 (8 bits), one row of 4 bits 20.4; here 21.5 (5.8 TB/s) and 25.1, of which what
+// the 8-bit codes' two parts take (21.8 without). Of two workgroups on a unit, with 128 registers a lane, the second's start cost
+// what it gained (4 bits). A rhs of less than 48 MiB, which the caches may hold, goes faster above: 16 x 14336 x 4096 7.1 us, here 7.7
+// (8 bits 7.9, 11.0). A row-major rhs gains more: 16 x 28672 x 8192 in 26.9 us (37.8; 8 bits 30.0, 38.5).
+template <int LBITS, int FOURS>
 __global__ __launch_bounds__(64 * kWaves) void mx_mmt4d_resident_kernel(const MxProduct p) {
   static_assert(4 * kWaves * 2 == kMxResidentChunks, "two fours at most");
   constexpr int PANELS = 4, AHEAD = 4 / FOURS;
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_mmt4d_resident_kernel(const Mx
       const bool more = panel + AHEAD < end;
       auto multiply = [&](int f, auto number, uint32_t bs) {
         constexpr int U = decltype(number)::value;
-        if constexpr (SPLIT) {
+        if constexpr (LBITS == 8) {
           MxFragment<8> whole = a[f][U], high, low;
 #pragma unroll
           for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(whole.w[i]));  // (or both parts are kept in registers)
@@ -372,12 +372,8 @@ hipError_t launch(const MxProduct& p, hipStream_t stream) {
   const dim3 grid((p.rhs.rows + 16 * NT - 1) / (16 * NT), (p.lhs.rows + 16 * MT - 1) / (16 * MT));
   void* args[] = {const_cast<MxProduct*>(&p)};
   const bool stream_rhs = comes_from_hbm((int64_t)p.rhs.rows * p.chunks * 64);
-  const bool split = LBITS == 8 && p.out_type == Float::kF32;
-  constexpr bool EIGHT = LBITS == 8;
-  const void* kernel = split ? (stream_rhs ? (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, true, EIGHT, STAGED>
-                                           : (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, false, EIGHT, STAGED>)
-                             : (stream_rhs ? (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, true, false, STAGED>
-                                           : (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, false, false, STAGED>);
+  const void* kernel = stream_rhs ? (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, true, STAGED>
+                                  : (const void*)mx_mmt4d_few_kernel<LBITS, MT, NT, false, STAGED>;
   constexpr int SUMS = kWaves * MT * NT * 1024, LHS = STAGED ? kWaves * 4 * MT * 256 * LBITS : 0, LDS = SUMS > LHS ? SUMS : LHS;
   static_assert(LDS <= 160 * 1024, "LDS");
   if (LDS > 64 * 1024) {
@@ -389,9 +385,7 @@ hipError_t launch(const MxProduct& p, hipStream_t stream) {
 
 template <int LBITS, int FOURS>
 hipError_t launch_resident(const MxProduct& p, hipStream_t stream) {
-  const bool split = LBITS == 8 && p.out_type == Float::kF32;
-  const void* kernel = split ? (const void*)mx_mmt4d_resident_kernel<LBITS, FOURS, LBITS == 8>
-                             : (const void*)mx_mmt4d_resident_kernel<LBITS, FOURS, false>;
+  const void* kernel = (const void*)mx_mmt4d_resident_kernel<LBITS, FOURS>;
   constexpr int SUMS = 2 * 4 * kWaves * 1024, LHS = kWaves * FOURS * 4 * 256 * LBITS, LDS = SUMS > LHS ? SUMS : LHS;
   if (LDS > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
