@@ -177,7 +177,8 @@ Choice choose(const MxProduct& p, int lhs_bits) {
   if (rows <= 16 && (rows >= 4 || p.rhs.tile_rows < 16) && p.chunks <= kMxResidentChunks && comes_from_hbm(cols * p.chunks * 64)) {
     const int64_t panels = (cols + 15) / 16, most = (panels + kMxResidentGroups - 1) / kMxResidentGroups;
     if (lhs_near && near(p.rhs, 16 * most)) {
-      // (Wavefronts without a part of K load nothing, and some workgroups have a panel less than the others.)
+      // (32 or 64 chunks of every panel are loaded, the last one over and over where K has fewer, and some workgroups have a panel
+      // less than the others.)
       const float fours = (float)((p.chunks + 3) / 4), held = p.chunks <= 32 ? 8 : 16;
       const float each = .5f * ((float)most + (float)panels / kMxResidentGroups);
       const float read = memory / (float)panels * kMxResidentGroups * each / 6.1f * held / fours;

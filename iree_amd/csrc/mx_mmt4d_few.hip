@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_mmt4d_few_kernel(const MxProdu
 }
 
 // Up to 16 rows against a rhs from memory, K up to 8192: a workgroup, one on a compute unit, keeps the lhs in registers, a wavefront
-// its part of K (FOURS times four chunks), and goes through panels of 16 rows of the rhs, AHEAD of which are under way. Sums of
+// its part of K (FOURS times four chunks, the last one over and over where K ends before them), and goes through panels of 16 rows of the rhs, AHEAD of which are under way. Sums of
 // PANELS panels at a time meet in LDS, in the order of the wavefronts' numbers.
 //
 // Above, every workgroup loads the lhs anew, next to as many bytes of the rhs with 8-bit codes, and these loads delay the stream: 16
