@@ -124,6 +124,29 @@ typedef long long iree_uk_index_t;
 #define IREE_UK_MI355X_FLAG_RMS_NORM_TYPE_BF16E2M1 0x09
 #define IREE_UK_MI355X_FLAG_RMS_NORM_WEIGHT_F32 0x100
 
+/* Flag values of the feed-forward operators (no counterpart in the reference).
+ * Type flags name the operands' type twice, then the result's. */
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_TYPE_MASK 0xFF
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_TYPE_F16F16F32 0x01
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_TYPE_F16F16F16 0x02
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_TYPE_BF16BF16F32 0x03
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_TYPE_BF16BF16BF16 0x04
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_ACTIVATION_MASK 0xF00
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_SILU 0x100
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_GELU 0x200
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_SIGMOID 0x300
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_PRE_LOAD 0x1000
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_PRE_STORE 0x2000
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_PRE_F32 0x4000
+#define IREE_UK_MI355X_FLAG_GATED_MMT4D_ACCUMULATE 0x8000
+
+#define IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_TYPE_MASK 0xFF
+#define IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_TYPE_F16F16F32 0x01
+#define IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_TYPE_F16F16F16 0x02
+#define IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_TYPE_BF16BF16F32 0x03
+#define IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_TYPE_BF16BF16BF16 0x04
+#define IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_ACCUMULATE 0x100
+
 /*===--------------------------------------------------------------------===*/
 /* Parameter structs (field order and types are ABI).                         */
 /*===--------------------------------------------------------------------===*/
@@ -299,6 +322,105 @@ typedef struct iree_uk_mi355x_rms_norm_params_t {
   uint32_t flags;
 } iree_uk_mi355x_rms_norm_params_t;
 
+typedef struct iree_uk_mi355x_gated_mmt4d_params_t {
+  const void* lhs_buffer;
+  iree_uk_index_t lhs_offset;
+  iree_uk_index_t lhs_stride0;
+  const void* gate_buffer;
+  iree_uk_index_t gate_offset;
+  iree_uk_index_t gate_stride0;
+  const void* up_buffer;
+  iree_uk_index_t up_offset;
+  iree_uk_index_t up_stride0;
+  void* gate_pre_buffer; /* with PRE_LOAD or PRE_STORE */
+  iree_uk_index_t gate_pre_offset;
+  iree_uk_index_t gate_pre_stride0;
+  void* up_pre_buffer;
+  iree_uk_index_t up_pre_offset;
+  iree_uk_index_t up_pre_stride0;
+  void* out_buffer;
+  iree_uk_index_t out_offset;
+  iree_uk_index_t out_stride0;
+  iree_uk_index_t M;
+  iree_uk_index_t N;
+  iree_uk_index_t K;
+  int32_t M0;
+  int32_t N0;
+  int32_t K0;
+  uint32_t flags;
+} iree_uk_mi355x_gated_mmt4d_params_t;
+
+typedef struct iree_uk_mi355x_gated_mmt4d_backward_params_t {
+  const void* lhs_buffer;
+  iree_uk_index_t lhs_offset;
+  iree_uk_index_t lhs_stride0;
+  const void* gate_buffer;
+  iree_uk_index_t gate_offset;
+  iree_uk_index_t gate_stride0;
+  const void* up_buffer;
+  iree_uk_index_t up_offset;
+  iree_uk_index_t up_stride0;
+  const void* gate_pre_buffer;
+  iree_uk_index_t gate_pre_offset;
+  iree_uk_index_t gate_pre_stride0;
+  const void* up_pre_buffer;
+  iree_uk_index_t up_pre_offset;
+  iree_uk_index_t up_pre_stride0;
+  const void* out_grad_buffer;
+  iree_uk_index_t out_grad_offset;
+  iree_uk_index_t out_grad_stride0;
+  void* lhs_grad_buffer; /* NULL: not computed */
+  iree_uk_index_t lhs_grad_offset;
+  iree_uk_index_t lhs_grad_stride0;
+  void* gate_grad_buffer; /* NULL: not computed */
+  iree_uk_index_t gate_grad_offset;
+  iree_uk_index_t gate_grad_stride0;
+  void* up_grad_buffer; /* NULL: not computed */
+  iree_uk_index_t up_grad_offset;
+  iree_uk_index_t up_grad_stride0;
+  void* workspace_buffer;
+  iree_uk_index_t workspace_size; /* bytes */
+  iree_uk_index_t M;
+  iree_uk_index_t N;
+  iree_uk_index_t K;
+  int32_t M0;
+  int32_t N0;
+  int32_t K0;
+  uint32_t flags;
+} iree_uk_mi355x_gated_mmt4d_backward_params_t;
+
+typedef struct iree_uk_mi355x_adapter_mmt4d_params_t {
+  const void* lhs_buffer;
+  iree_uk_index_t lhs_offset;
+  iree_uk_index_t lhs_stride0;
+  const void* down_buffer;
+  iree_uk_index_t down_offset;
+  iree_uk_index_t down_stride0;
+  iree_uk_index_t down_stride1;
+  const void* up_buffer;
+  iree_uk_index_t up_offset;
+  iree_uk_index_t up_stride0;
+  iree_uk_index_t up_stride1;
+  const int32_t* index_buffer;
+  iree_uk_index_t index_offset;
+  const float* scales_buffer; /* NULL: ones */
+  iree_uk_index_t scales_offset;
+  void* out_buffer;
+  iree_uk_index_t out_offset;
+  iree_uk_index_t out_stride0;
+  void* workspace_buffer;
+  iree_uk_index_t workspace_size; /* bytes */
+  iree_uk_index_t M;
+  iree_uk_index_t N;
+  iree_uk_index_t K;
+  iree_uk_index_t rank;
+  iree_uk_index_t count;
+  int32_t M0;
+  int32_t N0;
+  int32_t K0;
+  uint32_t flags;
+} iree_uk_mi355x_adapter_mmt4d_params_t;
+
 /*===--------------------------------------------------------------------===*/
 /* Entry points shared with the reference.                                    */
 /*===--------------------------------------------------------------------===*/
@@ -459,6 +581,68 @@ void iree_uk_mi355x_mx_mmt4d_p(const iree_uk_mi355x_mx_mmt4d_params_t* params);
  * `sum` needs a residual. The outputs may not overlap each other or an input,
  * but for a `sum` at exactly the place of `in` or `residual`. */
 void iree_uk_mi355x_rms_norm_p(const iree_uk_mi355x_rms_norm_params_t* params);
+
+/* The gated part of a feed-forward block, both products in one kernel:
+ *   g = lhs * gate^T,  u = lhs * up^T,  out[M,N,M0,N0] = act(g) * u
+ * with lhs[M,K,M0,K0], gate[N,K,N0,K0] and up[N,K,N0,K0] as iree_uk_mmt4d has
+ * its operands, of f16 or bf16. Sums, act and its product are in f32; the result
+ * is rounded once, to f16 or bf16, where that is its type.
+ *   SILU:    act(x) = x * s(x), s(x) = 1 / (1 + e^-x)
+ *   GELU:    act(x) = x * s(2 * sqrt(2 / pi) * (x + 0.044715 * x^3)), the tanh form
+ *   SIGMOID: act(x) = s(x)
+ * x * s(x) is NaN where x is minus infinity.
+ *   gate_pre, up_pre: [M,N,M0,N0], of the operands' type or, with PRE_F32, of f32.
+ *   With PRE_LOAD what they hold is added to g and u first (adapters, or with a
+ *   stride of 0 and tiles one row tall a bias); with PRE_STORE g and u are stored
+ *   there, for the backward pass. With both they are updated in place. The
+ *   result is computed from g and u as they are ahead of that rounding.
+ * The order of summation is fixed for a call's parameters: the same call gives
+ * the same bits.
+ * The fast kernels take operands with tiles one row tall or a K0 of 8, 16 or 32,
+ * and buffers and strides that are multiples of 16 bytes; others run on a kernel
+ * with one thread for each result. What is written may not overlap an operand,
+ * another result or, row for row, itself. */
+void iree_uk_mi355x_gated_mmt4d_p(const iree_uk_mi355x_gated_mmt4d_params_t* params);
+
+/* Its backward pass. From lhs, gate, up, the stored gate_pre (g) and up_pre (u),
+ * and out_grad[M,N,M0,N0], the gradient of out:
+ *   dg = out_grad * u * act'(g),  du = out_grad * act(g)
+ *   lhs_grad[M,K,M0,K0]  = dg * gate + du * up
+ *   gate_grad[N,K,N0,K0] (+)= dg^T * lhs,  up_grad[N,K,N0,K0] (+)= du^T * lhs
+ * The result's type of the type flag is that of out_grad and of all gradients;
+ * with ACCUMULATE the gradients of the weights are added to what they hold. dg
+ * and du are rounded to the operands' type in between, which the matrix
+ * instructions take; the sums over them are in f32 and rounded once. A gradient
+ * whose buffer is NULL is not computed, and gate and up are not read without
+ * lhs_grad, nor lhs without the gradients of the weights.
+ *   workspace: device memory of iree_uk_mi355x_gated_mmt4d_backward_workspace()
+ *   bytes, 256-byte aligned, which is written before it is read and holds
+ *   nothing afterwards. Calls that may run at the same time, graphs that hold
+ *   them included, need workspaces of their own. (In synchronous mode it may be
+ *   host memory like any other buffer; it is not touched then.) */
+void iree_uk_mi355x_gated_mmt4d_backward_p(const iree_uk_mi355x_gated_mmt4d_backward_params_t* params);
+/* Bytes of workspace for a call with these sizes, flags and gradients (0 where
+ * the call would be refused, which is reported as by the call). */
+iree_uk_index_t iree_uk_mi355x_gated_mmt4d_backward_workspace(
+    const iree_uk_mi355x_gated_mmt4d_backward_params_t* params);
+
+/* Low-rank adapters of many requests at once, beside a product that they share:
+ * for each row i of the M * M0 rows of lhs[M,K,M0,K0],
+ *   out[i] (+)= scales[a] * (lhs[i] * down[a]^T) * up[a]^T,  a = index[i]
+ * with down[count][rank][K * K0] (adapters down_stride0 apart, rows
+ * down_stride1), up[count][N * N0][rank] (up_stride0, up_stride1), both of the
+ * operands' type and row-major, and scales of f32. A row whose index is
+ * negative, or count and more, has no adapter: nothing is added, and without
+ * ACCUMULATE its results are zero. With ACCUMULATE out holds the result of
+ * iree_uk_mmt4d with the same lhs, M, N, M0, N0; or out is what
+ * iree_uk_mi355x_gated_mmt4d_p loads (PRE_LOAD). Products and sums are in f32,
+ * rank sums included; the result is rounded once where it is f16 or bf16 (with
+ * ACCUMULATE the destination's value is added before that). Rows may come in
+ * any order; those of one adapter next to each other share the reads of it.
+ * The same call gives the same bits.
+ *   workspace: as above, of iree_uk_mi355x_adapter_mmt4d_workspace() bytes. */
+void iree_uk_mi355x_adapter_mmt4d_p(const iree_uk_mi355x_adapter_mmt4d_params_t* params);
+iree_uk_index_t iree_uk_mi355x_adapter_mmt4d_workspace(const iree_uk_mi355x_adapter_mmt4d_params_t* params);
 
 /* iree_uk_mmt4d_p for callers that cannot allocate. It has no counterpart in
  * the reference (whose microkernels never allocate, being CPU code); it is for

@@ -85,6 +85,24 @@ RMS_NORM_TYPE_F16E2M1 = 0x08
 RMS_NORM_TYPE_BF16E2M1 = 0x09
 RMS_NORM_WEIGHT_F32 = 0x100
 
+# --- feed-forward operators (no counterpart in the reference) ---------------
+GATED_MMT4D_TYPE_F16F16F32 = 0x01
+GATED_MMT4D_TYPE_F16F16F16 = 0x02
+GATED_MMT4D_TYPE_BF16BF16F32 = 0x03
+GATED_MMT4D_TYPE_BF16BF16BF16 = 0x04
+GATED_MMT4D_SILU = 0x100
+GATED_MMT4D_GELU = 0x200
+GATED_MMT4D_SIGMOID = 0x300
+GATED_MMT4D_PRE_LOAD = 0x1000
+GATED_MMT4D_PRE_STORE = 0x2000
+GATED_MMT4D_PRE_F32 = 0x4000
+GATED_MMT4D_ACCUMULATE = 0x8000
+ADAPTER_MMT4D_TYPE_F16F16F32 = 0x01
+ADAPTER_MMT4D_TYPE_F16F16F16 = 0x02
+ADAPTER_MMT4D_TYPE_BF16BF16F32 = 0x03
+ADAPTER_MMT4D_TYPE_BF16BF16BF16 = 0x04
+ADAPTER_MMT4D_ACCUMULATE = 0x100
+
 # (lhs bits, rhs bits, out bits) per mmt4d type flag.
 MMT4D_BITS = {
     MMT4D_TYPE_F32F32F32: (32, 32, 32),
@@ -207,6 +225,56 @@ class RmsNormParams(C.Structure):
         ("scales_buffer", C.c_void_p), ("scales_offset", index_t), ("scales_stride0", index_t),
         ("size0", index_t), ("size1", index_t), ("out_size1", index_t),
         ("epsilon", C.c_float), ("flags", C.c_uint32),
+    ]
+
+
+class GatedMmt4dParams(C.Structure):
+    _fields_ = [
+        ("lhs_buffer", C.c_void_p), ("lhs_offset", index_t), ("lhs_stride0", index_t),
+        ("gate_buffer", C.c_void_p), ("gate_offset", index_t), ("gate_stride0", index_t),
+        ("up_buffer", C.c_void_p), ("up_offset", index_t), ("up_stride0", index_t),
+        ("gate_pre_buffer", C.c_void_p), ("gate_pre_offset", index_t), ("gate_pre_stride0", index_t),
+        ("up_pre_buffer", C.c_void_p), ("up_pre_offset", index_t), ("up_pre_stride0", index_t),
+        ("out_buffer", C.c_void_p), ("out_offset", index_t), ("out_stride0", index_t),
+        ("M", index_t), ("N", index_t), ("K", index_t),
+        ("M0", C.c_int32), ("N0", C.c_int32), ("K0", C.c_int32),
+        ("flags", C.c_uint32),
+    ]
+
+
+class GatedMmt4dBackwardParams(C.Structure):
+    _fields_ = [
+        ("lhs_buffer", C.c_void_p), ("lhs_offset", index_t), ("lhs_stride0", index_t),
+        ("gate_buffer", C.c_void_p), ("gate_offset", index_t), ("gate_stride0", index_t),
+        ("up_buffer", C.c_void_p), ("up_offset", index_t), ("up_stride0", index_t),
+        ("gate_pre_buffer", C.c_void_p), ("gate_pre_offset", index_t), ("gate_pre_stride0", index_t),
+        ("up_pre_buffer", C.c_void_p), ("up_pre_offset", index_t), ("up_pre_stride0", index_t),
+        ("out_grad_buffer", C.c_void_p), ("out_grad_offset", index_t), ("out_grad_stride0", index_t),
+        ("lhs_grad_buffer", C.c_void_p), ("lhs_grad_offset", index_t), ("lhs_grad_stride0", index_t),
+        ("gate_grad_buffer", C.c_void_p), ("gate_grad_offset", index_t), ("gate_grad_stride0", index_t),
+        ("up_grad_buffer", C.c_void_p), ("up_grad_offset", index_t), ("up_grad_stride0", index_t),
+        ("workspace_buffer", C.c_void_p), ("workspace_size", index_t),
+        ("M", index_t), ("N", index_t), ("K", index_t),
+        ("M0", C.c_int32), ("N0", C.c_int32), ("K0", C.c_int32),
+        ("flags", C.c_uint32),
+    ]
+
+
+class AdapterMmt4dParams(C.Structure):
+    _fields_ = [
+        ("lhs_buffer", C.c_void_p), ("lhs_offset", index_t), ("lhs_stride0", index_t),
+        ("down_buffer", C.c_void_p), ("down_offset", index_t), ("down_stride0", index_t),
+        ("down_stride1", index_t),
+        ("up_buffer", C.c_void_p), ("up_offset", index_t), ("up_stride0", index_t),
+        ("up_stride1", index_t),
+        ("index_buffer", C.c_void_p), ("index_offset", index_t),
+        ("scales_buffer", C.c_void_p), ("scales_offset", index_t),
+        ("out_buffer", C.c_void_p), ("out_offset", index_t), ("out_stride0", index_t),
+        ("workspace_buffer", C.c_void_p), ("workspace_size", index_t),
+        ("M", index_t), ("N", index_t), ("K", index_t),
+        ("rank", index_t), ("count", index_t),
+        ("M0", C.c_int32), ("N0", C.c_int32), ("K0", C.c_int32),
+        ("flags", C.c_uint32),
     ]
 
 

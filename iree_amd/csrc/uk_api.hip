@@ -58,6 +58,15 @@ void report_failure(const char* file, int line, const char* function, const char
     }                                                         \
   } while (0)
 
+// The same in a function that returns whether its checks hold.
+#define UK_REQUIRE_TRUE(cond)                                 \
+  do {                                                        \
+    if (!(cond)) {                                            \
+      report_failure(__FILE__, __LINE__, __func__, #cond);    \
+      return false;                                           \
+    }                                                         \
+  } while (0)
+
 // Checks a HIP call inside a function returning bool (true = ok).
 #define UK_HIP_OK(expr)                                                       \
   do {                                                                        \
@@ -476,7 +485,7 @@ bool pipe_down(const Stager& stager, void* host, const void* dev, size_t bytes, 
 }
 
 // Makes the operands of a call reachable from the device.
-constexpr int kMostOperands = 6;
+constexpr int kMostOperands = 10;
 bool stage_operands(Stager& stager, Operand* const* ops, int count, hipStream_t stream) {
   Operand* mirrored[kMostOperands];
   int mirrors = 0, piped = 0;
@@ -1337,6 +1346,334 @@ UK_API void iree_uk_mi355x_rms_norm_p(const iree_uk_mi355x_rms_norm_params_t* p)
   }
   const Operand* const outs[] = {&o_sum, &o_out, &o_scales};
   finish(stager, stream, outs, 3);
+}
+
+//===----------------------------------------------------------------------===//
+// Feed-forward operators (no counterpart in the reference)
+//===----------------------------------------------------------------------===//
+
+namespace {
+
+// Type flags number the operands' types 1 and 3, with an f32 result, and 2 and 4, with a result of the operands' type.
+uk::Float operand_type_of(uint32_t type) { return type <= 2 ? uk::Float::kF16 : uk::Float::kBf16; }
+uk::Float result_type_of(uint32_t type) { return type % 2 ? uk::Float::kF32 : operand_type_of(type); }
+
+bool tile_counts_in_range(int64_t M, int64_t N, int64_t K, int32_t M0, int32_t N0, int32_t K0) {
+  return in_unsigned_range(M, 31) && in_unsigned_range(N, 31) && in_unsigned_range(K, 31) && in_unsigned_range(M0, 15) &&
+         in_unsigned_range(N0, 15) && in_unsigned_range(K0, 15);
+}
+
+constexpr uint32_t kGatedKnown = IREE_UK_MI355X_FLAG_GATED_MMT4D_TYPE_MASK |
+                                 IREE_UK_MI355X_FLAG_GATED_MMT4D_ACTIVATION_MASK | IREE_UK_MI355X_FLAG_GATED_MMT4D_PRE_F32;
+bool gated_flags_known(uint32_t flags, uint32_t more) {
+  const uint32_t type = flags & IREE_UK_MI355X_FLAG_GATED_MMT4D_TYPE_MASK;
+  const uint32_t activation = flags & IREE_UK_MI355X_FLAG_GATED_MMT4D_ACTIVATION_MASK;
+  return !(flags & ~(kGatedKnown | more)) && type >= IREE_UK_MI355X_FLAG_GATED_MMT4D_TYPE_F16F16F32 &&
+         type <= IREE_UK_MI355X_FLAG_GATED_MMT4D_TYPE_BF16BF16BF16 && activation >= IREE_UK_MI355X_FLAG_GATED_MMT4D_SILU &&
+         activation <= IREE_UK_MI355X_FLAG_GATED_MMT4D_SIGMOID;
+}
+uk::Activation activation_of(uint32_t flags) {
+  return (uk::Activation)(((flags & IREE_UK_MI355X_FLAG_GATED_MMT4D_ACTIVATION_MASK) >> 8) - 1);
+}
+
+// A tiled operand [outer0][outer1][tile0][tile1] of `bytes` an element (outer0 = 0: none).
+RowRegion tiled_region(Checked& c, int64_t outer0, int64_t outer1, int64_t tile0, int64_t tile1, int64_t stride0, int bytes) {
+  return make_region(c, outer0, c.mul(c.mul(outer1, tile0 * tile1), bytes), outer0 > 0 ? c.mul(stride0, bytes) : 0);
+}
+
+uint8_t* written(const Operand& o) { return (uint8_t*)const_cast<void*>(o.dev); }
+
+}  // namespace
+
+UK_API void iree_uk_mi355x_gated_mmt4d_p(const iree_uk_mi355x_gated_mmt4d_params_t* p) {
+  tl_last_kernel = "";
+  UK_REQUIRE(p != nullptr);
+  const bool load = p->flags & IREE_UK_MI355X_FLAG_GATED_MMT4D_PRE_LOAD, store = p->flags & IREE_UK_MI355X_FLAG_GATED_MMT4D_PRE_STORE;
+  const bool pre = load || store;
+  UK_REQUIRE(gated_flags_known(p->flags, IREE_UK_MI355X_FLAG_GATED_MMT4D_PRE_LOAD | IREE_UK_MI355X_FLAG_GATED_MMT4D_PRE_STORE));
+  UK_REQUIRE(pre || !(p->flags & IREE_UK_MI355X_FLAG_GATED_MMT4D_PRE_F32));
+  UK_REQUIRE(tile_counts_in_range(p->M, p->N, p->K, p->M0, p->N0, p->K0));
+  const uint32_t flag = p->flags & IREE_UK_MI355X_FLAG_GATED_MMT4D_TYPE_MASK;
+  const uk::Float type = operand_type_of(flag), out_type = result_type_of(flag),
+                  pre_type = p->flags & IREE_UK_MI355X_FLAG_GATED_MMT4D_PRE_F32 ? uk::Float::kF32 : type;
+  if (p->M == 0 || p->N == 0 || p->M0 == 0 || p->N0 == 0) return;
+
+  Checked c;
+  const int e = uk::float_bytes(out_type), pe = uk::float_bytes(pre_type);
+  const RowRegion lhs_region = tiled_region(c, p->M, p->K, p->M0, p->K0, p->lhs_stride0, 2);
+  const RowRegion gate_region = tiled_region(c, p->N, p->K, p->N0, p->K0, p->gate_stride0, 2);
+  const RowRegion up_region = tiled_region(c, p->N, p->K, p->N0, p->K0, p->up_stride0, 2);
+  const RowRegion gate_pre_region = tiled_region(c, pre ? p->M : 0, p->N, p->M0, p->N0, p->gate_pre_stride0, pe);
+  const RowRegion up_pre_region = tiled_region(c, pre ? p->M : 0, p->N, p->M0, p->N0, p->up_pre_stride0, pe);
+  const RowRegion out_region = tiled_region(c, p->M, p->N, p->M0, p->N0, p->out_stride0, e);
+  const int64_t lhs_offset = c.mul(p->lhs_offset, 2), gate_offset = c.mul(p->gate_offset, 2), up_offset = c.mul(p->up_offset, 2),
+                gate_pre_offset = c.mul(pre ? p->gate_pre_offset : 0, pe), up_pre_offset = c.mul(pre ? p->up_pre_offset : 0, pe),
+                out_offset = c.mul(p->out_offset, e);
+  UK_REQUIRE(c.ok && "operand extents fit int64");
+  UK_REQUIRE(p->M == 1 || p->lhs_stride0 >= 0);
+  UK_REQUIRE(p->N == 1 || (p->gate_stride0 >= 0 && p->up_stride0 >= 0));
+  UK_REQUIRE(!pre || p->M == 1 || (p->gate_pre_stride0 >= 0 && p->up_pre_stride0 >= 0));
+  UK_REQUIRE(rows_apart(out_region));
+  UK_REQUIRE(!store || (rows_apart(gate_pre_region) && rows_apart(up_pre_region)));
+
+  hipStream_t stream = tl_stream;
+  Stager stager;
+  Operand o_lhs{offset_pointer(p->lhs_buffer, lhs_offset), as_copied(lhs_region), true};
+  Operand o_gate{offset_pointer(p->gate_buffer, gate_offset), as_copied(gate_region), true};
+  Operand o_up{offset_pointer(p->up_buffer, up_offset), as_copied(up_region), true};
+  Operand o_gate_pre{offset_pointer(p->gate_pre_buffer, gate_pre_offset), as_copied(gate_pre_region), load};
+  Operand o_up_pre{offset_pointer(p->up_pre_buffer, up_pre_offset), as_copied(up_pre_region), load};
+  Operand o_out{offset_pointer(p->out_buffer, out_offset), out_region, false};
+  UK_REQUIRE(given(o_lhs, p->lhs_buffer));
+  UK_REQUIRE(given(o_gate, p->gate_buffer));
+  UK_REQUIRE(given(o_up, p->up_buffer));
+  UK_REQUIRE(given(o_gate_pre, p->gate_pre_buffer));
+  UK_REQUIRE(given(o_up_pre, p->up_pre_buffer));
+  UK_REQUIRE(given(o_out, p->out_buffer));
+  Operand* const operands[] = {&o_lhs, &o_gate, &o_up, &o_gate_pre, &o_up_pre, &o_out};
+  for (int i = 0; i < 5; ++i) UK_REQUIRE(!overlap(o_out, *operands[i]));
+  for (int i = 0; store && i < 3; ++i) UK_REQUIRE(!overlap(o_gate_pre, *operands[i]) && !overlap(o_up_pre, *operands[i]));
+  UK_REQUIRE(!store || !overlap(o_gate_pre, o_up_pre));
+  if (!stage_operands(stager, operands, 6, stream)) {
+    abandon(stager, stream);
+    return;
+  }
+  uk::GatedArgs a;
+  a.lhs = (const uint8_t*)o_lhs.dev; a.gate = (const uint8_t*)o_gate.dev; a.up = (const uint8_t*)o_up.dev;
+  a.gate_pre = pre ? written(o_gate_pre) : nullptr; a.up_pre = pre ? written(o_up_pre) : nullptr;
+  a.out = written(o_out);
+  a.lhs_stride0 = p->lhs_stride0; a.gate_stride0 = p->gate_stride0; a.up_stride0 = p->up_stride0;
+  a.gate_pre_stride0 = pre ? p->gate_pre_stride0 : 0; a.up_pre_stride0 = pre ? p->up_pre_stride0 : 0;
+  a.out_stride0 = p->out_stride0;
+  a.M = p->M; a.N = p->N; a.K = p->K0 == 0 ? 0 : p->K;
+  a.M0 = p->M0; a.N0 = p->N0; a.K0 = p->K0;
+  a.type = type; a.out_type = out_type; a.pre_type = pre_type;
+  a.activation = activation_of(p->flags);
+  a.pre_load = load; a.pre_store = store;
+  if (!launch_ok(uk::launch_gated_mmt4d(a, stream, &tl_last_kernel), "gated_mmt4d")) {
+    abandon(stager, stream);
+    return;
+  }
+  const Operand* const outs[] = {&o_out, &o_gate_pre, &o_up_pre};
+  finish(stager, stream, outs, store ? 3 : 1);
+}
+
+namespace {
+
+// What a backward call's checks and the size of its workspace have in common; null: refused, or (`empty`) nothing to do.
+bool gated_backward_args(const iree_uk_mi355x_gated_mmt4d_backward_params_t* p, uk::GatedBackwardArgs* a, bool* empty) {
+  *empty = false;
+  UK_REQUIRE_TRUE(p != nullptr);
+  UK_REQUIRE_TRUE(gated_flags_known(p->flags, IREE_UK_MI355X_FLAG_GATED_MMT4D_ACCUMULATE));
+  UK_REQUIRE_TRUE(tile_counts_in_range(p->M, p->N, p->K, p->M0, p->N0, p->K0));
+  const uint32_t flag = p->flags & IREE_UK_MI355X_FLAG_GATED_MMT4D_TYPE_MASK;
+  const bool of_lhs = p->lhs_grad_buffer, of_gate = p->gate_grad_buffer, of_up = p->up_grad_buffer;
+  *a = uk::GatedBackwardArgs();
+  a->lhs_grad = (uint8_t*)p->lhs_grad_buffer; a->gate_grad = (uint8_t*)p->gate_grad_buffer; a->up_grad = (uint8_t*)p->up_grad_buffer;
+  a->lhs_stride0 = p->lhs_stride0; a->gate_stride0 = p->gate_stride0; a->up_stride0 = p->up_stride0;
+  a->gate_pre_stride0 = p->gate_pre_stride0; a->up_pre_stride0 = p->up_pre_stride0; a->out_grad_stride0 = p->out_grad_stride0;
+  a->lhs_grad_stride0 = of_lhs ? p->lhs_grad_stride0 : 0;
+  a->gate_grad_stride0 = of_gate ? p->gate_grad_stride0 : 0;
+  a->up_grad_stride0 = of_up ? p->up_grad_stride0 : 0;
+  // (Without rows there are sums over none, without columns too.)
+  const bool rows = p->M > 0 && p->M0 > 0, cols = p->N > 0 && p->N0 > 0;
+  a->M = rows ? p->M : 0; a->N = cols ? p->N : 0; a->K = p->K;
+  a->M0 = p->M0; a->N0 = p->N0; a->K0 = p->K0;
+  a->type = operand_type_of(flag); a->out_type = result_type_of(flag);
+  a->pre_type = p->flags & IREE_UK_MI355X_FLAG_GATED_MMT4D_PRE_F32 ? uk::Float::kF32 : a->type;
+  a->activation = activation_of(p->flags);
+  a->accumulate = p->flags & IREE_UK_MI355X_FLAG_GATED_MMT4D_ACCUMULATE;
+  *empty = p->K == 0 || p->K0 == 0 || (!rows && !cols) || !(of_lhs || of_gate || of_up) || (!rows && (a->accumulate || !(of_gate || of_up))) ||
+           (!cols && !of_lhs);
+  return true;
+}
+
+}  // namespace
+
+UK_API iree_uk_index_t iree_uk_mi355x_gated_mmt4d_backward_workspace(const iree_uk_mi355x_gated_mmt4d_backward_params_t* p) {
+  uk::GatedBackwardArgs a;
+  bool empty;
+  if (!gated_backward_args(p, &a, &empty) || empty) return 0;
+  const int64_t bytes = uk::gated_backward_workspace(a);
+  if (bytes < 0) {
+    report_failure(__FILE__, __LINE__, __func__, "the workspace fits int64");
+    return 0;
+  }
+  return bytes;
+}
+
+UK_API void iree_uk_mi355x_gated_mmt4d_backward_p(const iree_uk_mi355x_gated_mmt4d_backward_params_t* p) {
+  tl_last_kernel = "";
+  uk::GatedBackwardArgs a;
+  bool empty;
+  if (!gated_backward_args(p, &a, &empty) || empty) return;
+  const bool of_lhs = a.lhs_grad, of_gate = a.gate_grad, of_up = a.up_grad, of_weights = of_gate || of_up;
+  const int64_t needed = uk::gated_backward_workspace(a);
+  UK_REQUIRE(needed >= 0 && "the workspace fits int64");
+  UK_REQUIRE(p->workspace_size >= needed);
+  UK_REQUIRE(needed == 0 || p->workspace_buffer != nullptr);
+  UK_REQUIRE((uintptr_t)p->workspace_buffer % 256 == 0 || needed == 0);
+
+  Checked c;
+  const int e = uk::float_bytes(a.out_type), pe = uk::float_bytes(a.pre_type);
+  const int64_t k = p->K, m0 = p->M0, n0 = p->N0, k0 = p->K0;
+  const RowRegion lhs_region = tiled_region(c, of_weights ? a.M : 0, k, m0, k0, a.lhs_stride0, 2);
+  const RowRegion gate_region = tiled_region(c, of_lhs ? a.N : 0, k, n0, k0, a.gate_stride0, 2);
+  const RowRegion up_region = tiled_region(c, of_lhs ? a.N : 0, k, n0, k0, a.up_stride0, 2);
+  const RowRegion gate_pre_region = tiled_region(c, a.M, a.N, m0, n0, a.gate_pre_stride0, pe);
+  const RowRegion up_pre_region = tiled_region(c, a.M, a.N, m0, n0, a.up_pre_stride0, pe);
+  const RowRegion out_grad_region = tiled_region(c, a.M, a.N, m0, n0, a.out_grad_stride0, e);
+  const RowRegion lhs_grad_region = tiled_region(c, of_lhs ? a.M : 0, k, m0, k0, a.lhs_grad_stride0, e);
+  const RowRegion gate_grad_region = tiled_region(c, of_gate ? a.N : 0, k, n0, k0, a.gate_grad_stride0, e);
+  const RowRegion up_grad_region = tiled_region(c, of_up ? a.N : 0, k, n0, k0, a.up_grad_stride0, e);
+  const int64_t lhs_offset = c.mul(p->lhs_offset, 2), gate_offset = c.mul(p->gate_offset, 2), up_offset = c.mul(p->up_offset, 2),
+                gate_pre_offset = c.mul(p->gate_pre_offset, pe), up_pre_offset = c.mul(p->up_pre_offset, pe),
+                out_grad_offset = c.mul(p->out_grad_offset, e), lhs_grad_offset = c.mul(of_lhs ? p->lhs_grad_offset : 0, e),
+                gate_grad_offset = c.mul(of_gate ? p->gate_grad_offset : 0, e), up_grad_offset = c.mul(of_up ? p->up_grad_offset : 0, e);
+  UK_REQUIRE(c.ok && "operand extents fit int64");
+  UK_REQUIRE(a.M <= 1 || (a.lhs_stride0 >= 0 && a.gate_pre_stride0 >= 0 && a.up_pre_stride0 >= 0 && a.out_grad_stride0 >= 0));
+  UK_REQUIRE(a.N <= 1 || (a.gate_stride0 >= 0 && a.up_stride0 >= 0));
+  UK_REQUIRE(rows_apart(lhs_grad_region));
+  UK_REQUIRE(rows_apart(gate_grad_region));
+  UK_REQUIRE(rows_apart(up_grad_region));
+
+  hipStream_t stream = tl_stream;
+  Stager stager;
+  Operand o_lhs{offset_pointer(p->lhs_buffer, lhs_offset), as_copied(lhs_region), true};
+  Operand o_gate{offset_pointer(p->gate_buffer, gate_offset), as_copied(gate_region), true};
+  Operand o_up{offset_pointer(p->up_buffer, up_offset), as_copied(up_region), true};
+  Operand o_gate_pre{offset_pointer(p->gate_pre_buffer, gate_pre_offset), as_copied(gate_pre_region), true};
+  Operand o_up_pre{offset_pointer(p->up_pre_buffer, up_pre_offset), as_copied(up_pre_region), true};
+  Operand o_out_grad{offset_pointer(p->out_grad_buffer, out_grad_offset), as_copied(out_grad_region), true};
+  Operand o_lhs_grad{offset_pointer(p->lhs_grad_buffer, lhs_grad_offset), lhs_grad_region, false};
+  Operand o_gate_grad{offset_pointer(p->gate_grad_buffer, gate_grad_offset), gate_grad_region, a.accumulate};
+  Operand o_up_grad{offset_pointer(p->up_grad_buffer, up_grad_offset), up_grad_region, a.accumulate};
+  Operand o_workspace{p->workspace_buffer, make_region(c, needed > 0 ? 1 : 0, needed, needed), false};
+  Operand* const operands[] = {&o_lhs, &o_gate, &o_up, &o_gate_pre, &o_up_pre, &o_out_grad,
+                               &o_lhs_grad, &o_gate_grad, &o_up_grad, &o_workspace};
+  const void* const buffers[] = {p->lhs_buffer, p->gate_buffer, p->up_buffer, p->gate_pre_buffer, p->up_pre_buffer, p->out_grad_buffer};
+  for (int i = 0; i < 6; ++i) UK_REQUIRE(given(*operands[i], buffers[i]));
+  for (int i = 6; i < 10; ++i)
+    for (int j = 0; j < i; ++j) UK_REQUIRE(!overlap(*operands[i], *operands[j]));
+  if (!stage_operands(stager, operands, 10, stream)) {
+    abandon(stager, stream);
+    return;
+  }
+  a.lhs = (const uint8_t*)o_lhs.dev; a.gate = (const uint8_t*)o_gate.dev; a.up = (const uint8_t*)o_up.dev;
+  a.gate_pre = (const uint8_t*)o_gate_pre.dev; a.up_pre = (const uint8_t*)o_up_pre.dev;
+  a.out_grad = (const uint8_t*)o_out_grad.dev;
+  a.lhs_grad = of_lhs ? written(o_lhs_grad) : nullptr;
+  a.gate_grad = of_gate ? written(o_gate_grad) : nullptr;
+  a.up_grad = of_up ? written(o_up_grad) : nullptr;
+  a.workspace = written(o_workspace);
+  if (!launch_ok(uk::launch_gated_backward(a, stream, &tl_last_kernel), "gated_mmt4d_backward")) {
+    abandon(stager, stream);
+    return;
+  }
+  const Operand* const outs[] = {&o_lhs_grad, &o_gate_grad, &o_up_grad};
+  finish(stager, stream, outs, 3);
+}
+
+namespace {
+
+bool adapter_args(const iree_uk_mi355x_adapter_mmt4d_params_t* p, uk::AdapterArgs* a, bool* empty) {
+  *empty = false;
+  UK_REQUIRE_TRUE(p != nullptr);
+  const uint32_t flag = p->flags & IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_TYPE_MASK;
+  UK_REQUIRE_TRUE(!(p->flags & ~(uint32_t)(IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_TYPE_MASK | IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_ACCUMULATE)));
+  UK_REQUIRE_TRUE(flag >= IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_TYPE_F16F16F32 && flag <= IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_TYPE_BF16BF16BF16);
+  UK_REQUIRE_TRUE(tile_counts_in_range(p->M, p->N, p->K, p->M0, p->N0, p->K0));
+  UK_REQUIRE_TRUE(p->M * p->M0 <= 0x7FFFFFFF);
+  UK_REQUIRE_TRUE(in_unsigned_range(p->rank, 15));
+  UK_REQUIRE_TRUE(in_unsigned_range(p->count, 31));
+  *a = uk::AdapterArgs();
+  a->lhs_stride0 = p->lhs_stride0; a->out_stride0 = p->out_stride0;
+  a->down_stride0 = p->down_stride0; a->down_stride1 = p->down_stride1;
+  a->up_stride0 = p->up_stride0; a->up_stride1 = p->up_stride1;
+  a->M = p->M; a->N = p->N; a->K = p->K0 == 0 ? 0 : p->K;
+  a->M0 = p->M0; a->N0 = p->N0; a->K0 = p->K0;
+  a->rank = p->rank; a->count = p->count;
+  if (a->K == 0 || a->rank == 0) a->count = 0;  // (nobody has an adapter)
+  a->type = operand_type_of(flag); a->out_type = result_type_of(flag);
+  a->accumulate = p->flags & IREE_UK_MI355X_FLAG_ADAPTER_MMT4D_ACCUMULATE;
+  *empty = p->M == 0 || p->N == 0 || p->M0 == 0 || p->N0 == 0 || (a->accumulate && a->count == 0);
+  return true;
+}
+
+}  // namespace
+
+UK_API iree_uk_index_t iree_uk_mi355x_adapter_mmt4d_workspace(const iree_uk_mi355x_adapter_mmt4d_params_t* p) {
+  uk::AdapterArgs a;
+  bool empty;
+  if (!adapter_args(p, &a, &empty) || empty) return 0;
+  const int64_t bytes = uk::adapter_workspace(a);
+  if (bytes < 0) {
+    report_failure(__FILE__, __LINE__, __func__, "the workspace fits int64");
+    return 0;
+  }
+  return bytes;
+}
+
+UK_API void iree_uk_mi355x_adapter_mmt4d_p(const iree_uk_mi355x_adapter_mmt4d_params_t* p) {
+  tl_last_kernel = "";
+  uk::AdapterArgs a;
+  bool empty;
+  if (!adapter_args(p, &a, &empty) || empty) return;
+  const int64_t needed = uk::adapter_workspace(a);
+  UK_REQUIRE(needed >= 0 && "the workspace fits int64");
+  UK_REQUIRE(p->workspace_size >= needed);
+  UK_REQUIRE(needed == 0 || p->workspace_buffer != nullptr);
+  UK_REQUIRE((uintptr_t)p->workspace_buffer % 256 == 0 || needed == 0);
+
+  Checked c;
+  const int e = uk::float_bytes(a.out_type);
+  const bool any = a.count > 0;
+  const int64_t depth = c.mul(a.K, a.K0), cols = a.N * a.N0, rows = a.M * a.M0;
+  UK_REQUIRE(!any || (p->down_stride0 >= 0 && p->down_stride1 >= 0 && p->up_stride0 >= 0 && p->up_stride1 >= 0));
+  const RowRegion lhs_region = tiled_region(c, any ? a.M : 0, a.K, a.M0, a.K0, a.lhs_stride0, 2);
+  const RowRegion down_region =
+      make_region(c, any ? a.count : 0, c.mul(c.add(c.mul(a.rank - 1, any ? a.down_stride1 : 0), depth), 2), c.mul(any ? a.down_stride0 : 0, 2));
+  const RowRegion up_region =
+      make_region(c, any ? a.count : 0, c.mul(c.add(c.mul(cols - 1, any ? a.up_stride1 : 0), a.rank), 2), c.mul(any ? a.up_stride0 : 0, 2));
+  const RowRegion index_region = make_region(c, any ? 1 : 0, rows * 4, 0);
+  const RowRegion scales_region = make_region(c, any && p->scales_buffer ? 1 : 0, a.count * 4, 0);
+  const RowRegion out_region = tiled_region(c, a.M, a.N, a.M0, a.N0, a.out_stride0, e);
+  const int64_t lhs_offset = c.mul(p->lhs_offset, 2), down_offset = c.mul(p->down_offset, 2), up_offset = c.mul(p->up_offset, 2),
+                index_offset = c.mul(p->index_offset, 4), scales_offset = c.mul(p->scales_buffer ? p->scales_offset : 0, 4),
+                out_offset = c.mul(p->out_offset, e);
+  UK_REQUIRE(c.ok && "operand extents fit int64");
+  UK_REQUIRE(a.M == 1 || a.lhs_stride0 >= 0);
+  UK_REQUIRE(rows_apart(out_region));
+
+  hipStream_t stream = tl_stream;
+  Stager stager;
+  Operand o_lhs{offset_pointer(p->lhs_buffer, lhs_offset), as_copied(lhs_region), true};
+  Operand o_down{offset_pointer(p->down_buffer, down_offset), as_copied(down_region), true};
+  Operand o_up{offset_pointer(p->up_buffer, up_offset), as_copied(up_region), true};
+  Operand o_index{offset_pointer(p->index_buffer, index_offset), index_region, true};
+  Operand o_scales{offset_pointer(p->scales_buffer, scales_offset), scales_region, true};
+  Operand o_out{offset_pointer(p->out_buffer, out_offset), out_region, a.accumulate};
+  Operand o_workspace{p->workspace_buffer, make_region(c, needed > 0 ? 1 : 0, needed, needed), false};
+  Operand* const operands[] = {&o_lhs, &o_down, &o_up, &o_index, &o_scales, &o_out, &o_workspace};
+  const void* const buffers[] = {p->lhs_buffer, p->down_buffer, p->up_buffer, p->index_buffer, p->scales_buffer, p->out_buffer};
+  for (int i = 0; i < 6; ++i) UK_REQUIRE(given(*operands[i], buffers[i]));
+  UK_REQUIRE((uintptr_t)o_index.ptr % 4 == 0 && (uintptr_t)o_scales.ptr % 4 == 0);
+  for (int i = 5; i < 7; ++i)
+    for (int j = 0; j < i; ++j) UK_REQUIRE(!overlap(*operands[i], *operands[j]));
+  if (!stage_operands(stager, operands, 7, stream)) {
+    abandon(stager, stream);
+    return;
+  }
+  a.lhs = (const uint8_t*)o_lhs.dev; a.down = (const uint8_t*)o_down.dev; a.up = (const uint8_t*)o_up.dev;
+  a.index = (const int32_t*)o_index.dev;
+  a.scales = any && p->scales_buffer ? (const float*)o_scales.dev : nullptr;
+  a.out = written(o_out);
+  a.workspace = written(o_workspace);
+  if (!launch_ok(uk::launch_adapter_mmt4d(a, stream, &tl_last_kernel), "adapter_mmt4d")) {
+    abandon(stager, stream);
+    return;
+  }
+  finish(stager, stream, o_out);
 }
 
 //===----------------------------------------------------------------------===//

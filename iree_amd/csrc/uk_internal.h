@@ -110,6 +110,58 @@ struct RmsNormArgs {
   bool stream_sum;  // past the caches; the launcher's
 };
 
+// Gated products: operands of one 16-bit type, strides in elements of the buffer's type.
+enum class Activation { kSilu = 0, kGelu = 1, kSigmoid = 2 };
+struct GatedArgs {
+  const uint8_t* lhs;
+  const uint8_t* gate;
+  const uint8_t* up;
+  uint8_t* gate_pre;  // or null, both
+  uint8_t* up_pre;
+  uint8_t* out;
+  int64_t lhs_stride0, gate_stride0, up_stride0, gate_pre_stride0, up_pre_stride0, out_stride0;
+  int64_t M, N, K;
+  int32_t M0, N0, K0;
+  Float type, out_type, pre_type;
+  Activation activation;
+  bool pre_load, pre_store;
+};
+
+struct GatedBackwardArgs {
+  const uint8_t* lhs;
+  const uint8_t* gate;
+  const uint8_t* up;
+  const uint8_t* gate_pre;
+  const uint8_t* up_pre;
+  const uint8_t* out_grad;
+  uint8_t* lhs_grad;   // each of them or null
+  uint8_t* gate_grad;
+  uint8_t* up_grad;
+  uint8_t* workspace;
+  int64_t lhs_stride0, gate_stride0, up_stride0, gate_pre_stride0, up_pre_stride0, out_grad_stride0;
+  int64_t lhs_grad_stride0, gate_grad_stride0, up_grad_stride0;
+  int64_t M, N, K;
+  int32_t M0, N0, K0;
+  Float type, out_type, pre_type;
+  Activation activation;
+  bool accumulate;
+};
+
+struct AdapterArgs {
+  const uint8_t* lhs;
+  const uint8_t* down;
+  const uint8_t* up;
+  const int32_t* index;
+  const float* scales;  // or null
+  uint8_t* out;
+  uint8_t* workspace;
+  int64_t lhs_stride0, down_stride0, down_stride1, up_stride0, up_stride1, out_stride0;
+  int64_t M, N, K, rank, count;
+  int32_t M0, N0, K0;
+  Float type, out_type;
+  bool accumulate;
+};
+
 // Enqueues a kernel that takes one argument struct. (Half a hundred nanoseconds each of the triple-bracket form's
 // configuration stack and of hipGetLastError are left out: the call itself returns the launch's status.)
 template <typename Args>
@@ -158,6 +210,13 @@ hipError_t launch_mx_pack(const MxPackArgs& a, hipStream_t stream, const char** 
 hipError_t launch_mx_unpack(const MxUnpackArgs& a, hipStream_t stream, const char** name);
 hipError_t launch_mx_mmt4d(const MxMmt4dArgs& a, hipStream_t stream, const char** name);
 hipError_t launch_rms_norm(const RmsNormArgs& a, hipStream_t stream, const char** name);
+
+hipError_t launch_gated_mmt4d(const GatedArgs& a, hipStream_t stream, const char** name);
+// (Of a workspace's bytes: -1 where they do not fit 64 bits. Pointers other than which gradients there are do not count.)
+hipError_t launch_gated_backward(const GatedBackwardArgs& a, hipStream_t stream, const char** name);
+int64_t gated_backward_workspace(const GatedBackwardArgs& a);
+hipError_t launch_adapter_mmt4d(const AdapterArgs& a, hipStream_t stream, const char** name);
+int64_t adapter_workspace(const AdapterArgs& a);
 
 // Copies between pinned host memory and the device as kernels on the stream (host_copy.hip), 16 bytes at a time: both
 // sides are 16-byte aligned and may be touched up to the next multiple of 16 bytes. A download sets flag b to
