@@ -1,0 +1,41 @@
+// The block kernels of gated products, one translation unit for each type.
+#ifndef IREE_AMD_CSRC_GATED_MMT4D_BLOCK_H_
+#define IREE_AMD_CSRC_GATED_MMT4D_BLOCK_H_
+
+#include "gated_mmt4d.h"
+#include "product16_block.h"
+
+namespace uk {
+namespace {
+
+template <Float T>
+hipError_t launch_gated_block(const GatedProduct& g, int tile, hipStream_t stream) {
+  BlockProduct<GatedResults> p;
+  p.lhs = g.lhs;
+  p.rhs = g.gate;
+  p.second = g.up;
+  p.second_stride0 = g.up_stride0;
+  p.depth = g.depth;
+  p.epilogue = g.results;
+  // Weights that no cache holds and that a tile or two of rows read once go past the caches: 64 rows x 28672 x 8192 (940 MB) 165 -> 148
+  // us in 64x128 tiles. (From 235 MB, 64 x 14336 x 4096, in 64x64 ones: 47.7 -> 44.9 us where other calls have filled the caches in
+  // between, but 35.5 -> 43.2 where they hold them.)
+  const bool stream_rhs = g.lhs.rows <= 128 && 4 * (int64_t)g.gate.rows * g.depth > (256ll << 20);
+  switch (tile) {  // kGatedTiles
+    case 0: return launch_block_tile<T, 4, 4, 4>(p, stream);
+    case 1: return launch_block_tile<T, 3, 4, 4>(p, stream);
+    case 2: return launch_block_tile<T, 2, 4, 3>(p, stream);
+    case 3: return launch_block_tile<T, 2, 3, 4>(p, stream);
+    case 4: return stream_rhs ? launch_block_tile<T, 2, 2, 5, true>(p, stream) : launch_block_tile<T, 2, 2, 5>(p, stream);
+    case 5: return stream_rhs ? launch_block_tile<T, 1, 4, 4, true>(p, stream) : launch_block_tile<T, 1, 4, 4>(p, stream);
+    case 6: return stream_rhs ? launch_block_tile<T, 1, 3, 5, true>(p, stream) : launch_block_tile<T, 1, 3, 5>(p, stream);
+    case 7: return stream_rhs ? launch_block_tile<T, 1, 2, 6, true>(p, stream) : launch_block_tile<T, 1, 2, 6>(p, stream);
+    case 8: return stream_rhs ? launch_block_tile<T, 1, 1, 8, true>(p, stream) : launch_block_tile<T, 1, 1, 8>(p, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+}  // namespace uk
+
+#endif  // IREE_AMD_CSRC_GATED_MMT4D_BLOCK_H_
