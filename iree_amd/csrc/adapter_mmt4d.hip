@@ -97,16 +97,23 @@ template <typename F>
 __device__ __forceinline__ uint32_t of_adapters(const AdapterProduct& p, uint32_t first, uint32_t slot, int lane, F f) {
   const uint32_t row = first + (lane & 15);
   const int32_t named = row < p.lhs.rows ? p.index[row] : -1;
-  uint32_t left = (uint32_t)__builtin_amdgcn_ballot_w64(named >= 0 && (uint32_t)named < p.count) & 0xFFFF;
-  const uint32_t without = ~left & 0xFFFF;
-  while (left != 0) {
-    const int32_t of = __builtin_amdgcn_readlane(named, __builtin_ctz(left));
-    const uint32_t same = (uint32_t)__builtin_amdgcn_ballot_w64(named == of) & left;
-    left &= ~same;
-    if (slot == 0) f((uint32_t)of, same);
-    slot = slot == 0 ? p.slots - 1 : slot - 1;
+  const uint32_t with = (uint32_t)__builtin_amdgcn_ballot_w64(named >= 0 && (uint32_t)named < p.count) & 0xFFFF;
+  // The first rows of adapters: nobody before has the same. (Lanes compare with the fifteen in front of them; -1 where there is none, and such a row has no adapter.)
+  bool again = false;
+  int32_t before = named;
+#pragma unroll
+  for (int back = 1; back < 16; ++back) {
+    before = __builtin_amdgcn_update_dpp(-1, before, 0x111, 0xF, 0xF, false);  // (of the lane in front, within sixteen)
+    again |= before == named;
   }
-  return without;
+  uint32_t firsts = (uint32_t)__builtin_amdgcn_ballot_w64(!again) & with;
+  for (; slot != 0 && firsts != 0; --slot) firsts &= firsts - 1;
+  while (firsts != 0) {
+    const int32_t of = __builtin_amdgcn_readlane(named, __builtin_ctz(firsts));
+    f((uint32_t)of, (uint32_t)__builtin_amdgcn_ballot_w64(named == of) & with);
+    for (uint32_t i = 0; i < p.slots && firsts != 0; ++i) firsts &= firsts - 1;
+  }
+  return ~with & 0xFFFF;
 }
 
 // Sums of 16 rows with 16 * RT ranks over a split's part of K, which the wavefronts share four chunks of 32 at a time; they meet in
@@ -190,93 +197,129 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_down_kernel(const Adapter
   }
 }
 
-// 16 rows times 16 * kFragments columns a wavefront. Sums and products are f32: v_mfma_f32_16x16x4, lane (r, g) with V ranks from V g on
-// of each 4 V, of row r of the sums and of column r.
-template <Float T, int V, bool ALIGNED>
+// 16 rows times 16 * F columns a wavefront, of four. Sums and products are f32: v_mfma_f32_16x16x4, lane (r, g) with V ranks from V g on
+// of each 4 V, of row r of the sums and of column r; RANKS times 4 V ranks at a time. The splits' sums are added on their way into LDS,
+// where all four have them from, and only those of rows that have the adapter are read: sixteen rows' sums of 64 ranks and two splits
+// are 8 KiB, twice what 32 columns of `up` are. Addresses are a part that is the wavefront's (scalar) and 32 bits that are the lane's.
+//
+// FAST: columns come in whole sixteens that lie next to each other, aligned, and an adapter's row of `up` in whole, aligned Vs. (As two
+// branches of one kernel the slow one's registers halved the number of wavefronts on a compute unit.)
+template <Float T, Float OUT, int V, int RANKS, int F, bool FAST>
 __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterProduct p) {
+  constexpr int SIZE = OUT == Float::kF32 ? 4 : 2, GROUP = 4 * V * RANKS, PITCH = GROUP + 4;  // (rows 4 banks apart)
+  __shared__ float sums[16 * PITCH];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   for (uint32_t unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
     // unit = (tile * slots + slot) * parts + block of columns
     const uint32_t upper = divide(unit, p.parts, p.parts_reciprocal), part = unit - upper * p.parts;
     const uint32_t tile = divide(upper, p.slots, p.slots_reciprocal), slot = upper - tile * p.slots;
-    const uint32_t first = tile * 16, first_col = (part * 4 + wave) * (16 * kFragments);
-    if (first_col >= p.cols) continue;
+    const uint32_t first = tile * 16, first_col = (part * 4 + wave) * (16 * F);
     const uint32_t row = first + r < p.lhs.rows ? first + r : p.lhs.rows - 1;
-    const int64_t out_row = layout_row(p.out_at, row);
-    auto store = [&](int f, p16_v4f32 v) {
-      const uint32_t col = first_col + 16 * f + 4 * g;
-      if (p.runs && col + 4 <= p.cols) {
-        const int64_t at = out_row + layout_col(p.out_at, col);
-        float x[4] = {v[0], v[1], v[2], v[3]}, old[4];
-        if (p.out_type == Float::kF32) {
-          if (p.accumulate) {
-            load_run<Float::kF32, 4>(p.out, at, old);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] += old[e];
-          }
-          store_run<Float::kF32, 4>(p.out, at, x);
-        } else {
-          if (p.accumulate) {
-            load_run<T, 4>(p.out, at, old);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] += old[e];
-          }
-          store_run<T, 4>(p.out, at, x);
-        }
-        return;
-      }
+    uint8_t* const out = p.out + layout_row(p.out_at, first) * SIZE;
+    const uint32_t out_row = (uint32_t)(layout_row(p.out_at, row) - layout_row(p.out_at, first));  // elements
+    // Four results, of fragment f, as they lie in memory.
+    typedef uint32_t Words __attribute__((ext_vector_type(SIZE)));
+    auto four_at = [&](int f) {
+      uint8_t* const fragment = out + layout_col(p.out_at, first_col + 16 * f) * SIZE;
+      return (Words*)__builtin_assume_aligned(fragment + (out_row + 4 * g) * SIZE, 4 * SIZE);
+    };
+    auto store_one_by_one = [&](int f, p16_v4f32 v) {
 #pragma unroll 1
       for (int e = 0; e < 4; ++e) {
-        if (col + e >= p.cols) continue;
-        const int64_t at = out_row + layout_col(p.out_at, col + e);
-        const float old = !p.accumulate ? 0 : p.out_type == Float::kF32 ? element<Float::kF32>(p.out, at) : element<T>(p.out, at);
-        if (p.out_type == Float::kF32) ((float*)p.out)[at] = old + v[e];
-        else ((uint16_t*)p.out)[at] = mx_narrow<T>(old + v[e]);
+        const uint32_t col = first_col + 16 * f + 4 * g + e;
+        if (col >= p.cols) continue;
+        const int64_t at = out_row + layout_col(p.out_at, col);
+        const float x = v[e] + (p.accumulate ? element<OUT>(out, at) : 0);
+        if constexpr (OUT == Float::kF32) ((float*)out)[at] = x;
+        else ((uint16_t*)out)[at] = mx_narrow<OUT>(x);
       }
     };
     const uint32_t without = of_adapters(p, first, slot, lane, [&](uint32_t of, uint32_t same) {
-      const uint8_t* up[kFragments];
+      const bool mine = (same >> r & 1) != 0;
+      typedef uint16_t Run __attribute__((ext_vector_type(V)));
+      const uint8_t* const up = p.up + of * p.up_stride0;
+      Words old[F] = {};
+      if (FAST && p.accumulate && mine) {
 #pragma unroll
-      for (int f = 0; f < kFragments; ++f) {
-        const uint32_t col = first_col + 16 * f + r;
-        up[f] = p.up + of * p.up_stride0 + (int64_t)(col < p.cols ? col : p.cols - 1) * p.up_stride1;
-      }
-      p16_v4f32 acc[kFragments] = {};
-      for (uint32_t from = 0; from < p.rank; from += 4 * V) {
-        const uint32_t rank = from + V * g;
-        float sum[V] = {};
-        for (uint32_t s = 0; s < p.splits; ++s) {
-          const float* at = p.sums + ((int64_t)s * p.lhs.rows + row) * p.pitch + rank;
-#pragma unroll
-          for (int e = 0; e < V; e += 4) {
-            const p16_v4f32 v = *(const p16_v4f32*)(at + e);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[e + i] += v[i];
-          }
-        }
-#pragma unroll
-        for (int f = 0; f < kFragments; ++f) {
-          uint16_t w[V];
-          if (ALIGNED && rank + V <= p.rank) {
-            __builtin_memcpy(w, __builtin_assume_aligned(up[f] + 2 * rank, 2 * V), 2 * V);
-          } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) w[e] = rank + e < p.rank ? ((const uint16_t*)up[f])[rank + e] : 0;
-          }
-#pragma unroll
-          for (int e = 0; e < V; ++e) acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(mx_widen<T>(w[e]), sum[e], acc[f], 0, 0, 0);
-        }
+        for (int f = 0; f < F; ++f)
+          if (first_col + 16 * f < p.cols) old[f] = *four_at(f);
       }
       const float scale = p.scales ? p.scales[of] : 1;
-      if ((same >> r & 1) != 0) {
+      p16_v4f32 acc[F] = {};
+      for (uint32_t rank0 = 0; rank0 < p.rank; rank0 += GROUP) {
+        Run w[RANKS][F];
 #pragma unroll
-        for (int f = 0; f < kFragments; ++f) store(f, acc[f] * scale);
+        for (int f = 0; f < F; ++f) {
+          const uint32_t col = first_col + 16 * f + r;
+          const uint32_t at = (col < p.cols ? col : p.cols - 1) * (uint32_t)p.up_stride1 + 2 * (rank0 + V * g);
+#pragma unroll
+          for (int c = 0; c < RANKS; ++c) {
+            const uint32_t rank = rank0 + 4 * V * c + V * g;
+            w[c][f] = Run(0);
+            if constexpr (FAST) {
+              if (rank < p.rank) w[c][f] = *(const Run*)(up + at + 8 * V * c);
+            } else {
+#pragma unroll
+              for (int e = 0; e < V; ++e)
+                if (rank + e < p.rank) w[c][f][e] = ((const uint16_t*)(up + at + 8 * V * c))[e];
+            }
+          }
+        }
+        // Four ranks of a row each thread. (The pitch is a multiple of 32 ranks; what lies behind it is not there.)
+        const uint32_t of_row = threadIdx.x / (GROUP / 4), four = 4 * (threadIdx.x % (GROUP / 4));
+        if (of_row < 16 && (same >> of_row & 1) != 0 && rank0 + four < p.pitch) {
+          const float* at = p.sums + (int64_t)(first + of_row) * p.pitch + rank0 + four;
+          const int64_t split = (int64_t)p.lhs.rows * p.pitch;
+          p16_v4f32 v = {0, 0, 0, 0};
+          for (uint32_t s = 0; s < p.splits; s += 4) {  // (four under way at a time)
+            p16_v4f32 part[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) part[i] = s + i < p.splits ? *(const p16_v4f32*)(at + (s + i) * split) : p16_v4f32{0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) v += part[i];
+          }
+          *(p16_v4f32*)(sums + of_row * PITCH + four) = v;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < RANKS; ++c)
+#pragma unroll
+          for (int e = 0; e < V; e += 4) {
+            const p16_v4f32 sum = *(const p16_v4f32*)(sums + r * PITCH + 4 * V * c + V * g + e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int f = 0; f < F; ++f)
+                acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(mx_widen<T>(w[c][f][e + i]), sum[i], acc[f], 0, 0, 0);
+          }
+        __syncthreads();
+      }
+      if (!mine) return;
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        p16_v4f32 v = acc[f] * scale;
+        if constexpr (!FAST) {
+          store_one_by_one(f, v);
+        } else if (first_col + 16 * f < p.cols) {
+          if constexpr (OUT == Float::kF32) {
+            v += __builtin_bit_cast(p16_v4f32, old[f]);
+            *four_at(f) = __builtin_bit_cast(Words, v);
+          } else {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = v[e] + mx_widen<OUT>((uint16_t)(old[f][e / 2] >> (16 * (e & 1))));
+            *four_at(f) = Words{mx_narrow_pair<OUT>(x[0], x[1]), mx_narrow_pair<OUT>(x[2], x[3])};
+          }
+        }
       }
     });
     if (!p.accumulate && slot == 0 && (without >> r & 1) != 0 && first + r < p.lhs.rows) {
-#pragma unroll
-      for (int f = 0; f < kFragments; ++f) store(f, p16_v4f32{0, 0, 0, 0});
+#pragma unroll 1
+      for (int f = 0; f < F; ++f) {
+        if constexpr (!FAST) store_one_by_one(f, p16_v4f32{0, 0, 0, 0});
+        else if (first_col + 16 * f < p.cols) *four_at(f) = Words(0);
+      }
     }
   }
 }
@@ -291,6 +334,10 @@ uint32_t splits_of(int64_t rows, int64_t depth, int64_t rank) {
 int64_t pitch_of(int64_t rank) { return (rank + 31) / 32 * 32; }
 
 bool multiple(const void* p, int64_t to) { return (uintptr_t)p % to == 0; }
+
+// Fragments of columns of a wavefront that multiplies by `up`.
+int up_fragments(int64_t rank) { return rank <= 32 ? 4 : 2; }
+int64_t column_parts(int64_t cols, int64_t rank) { return (cols + 64 * up_fragments(rank) - 1) / (64 * up_fragments(rank)); }
 
 // The problem as the kernels on the matrix pipe take it; false: they do not.
 bool as_product(const AdapterArgs& a, AdapterProduct* p) {
@@ -313,7 +360,9 @@ bool as_product(const AdapterArgs& a, AdapterProduct* p) {
   p->splits = splits_of(rows, depth, a.rank);
   p->accumulate = a.accumulate;
   const int e = float_bytes(a.out_type);
-  p->runs = runs_of(p->out_at, a.out, a.M, e, 4, 4 * e);
+  p->runs = runs_of(p->out_at, a.out, a.M, e, 16, 4 * e);
+  // (32 bits from an adapter's start to a column of `up`, and from a tile's first result to its last.)
+  if (p->up_stride1 > (1ll << 31) / cols || (a.M > 1 && a.out_stride0 > (1ll << 28) / 17) || (int64_t)p->out_at.tile * a.N > (1ll << 28)) return false;
   // Adapters of a tile side by side where there are few tiles.
   const int64_t slots = 128 / tiles, most = a.count < 16 ? a.count : 16;
   p->slots = (uint32_t)(slots < 1 ? 1 : slots > most ? most : slots);
@@ -338,20 +387,26 @@ hipError_t launch_down(const AdapterProduct& p, hipStream_t stream) {
   return launch_units(adapter_down_kernel<T, kFragments>, p, (fragments + kFragments - 1) / kFragments * p.splits, 64 * kWaves, stream);
 }
 
+template <Float T, Float OUT, bool FAST>
+hipError_t launch_up_of(const AdapterProduct& p, int64_t parts, hipStream_t stream) {
+  if (p.rank <= 16) return launch_units(adapter_up_kernel<T, OUT, 4, 1, 4, FAST>, p, parts, 256, stream);
+  if (p.rank <= 32) return launch_units(adapter_up_kernel<T, OUT, 8, 1, 4, FAST>, p, parts, 256, stream);
+  return launch_units(adapter_up_kernel<T, OUT, 8, 2, 2, FAST>, p, parts, 256, stream);
+}
 template <Float T>
 hipError_t launch_up(const AdapterProduct& p, hipStream_t stream) {
-  const int64_t parts = ((int64_t)p.cols + 64 * kFragments - 1) / (64 * kFragments);
+  const int64_t parts = column_parts(p.cols, p.rank);
   const int v = p.rank <= 16 ? 4 : 8;
-  const bool aligned = multiple(p.up, 2 * v) && (p.count <= 1 || p.up_stride0 % (2 * v) == 0) && (p.cols <= 1 || p.up_stride1 % (2 * v) == 0);
-  if (v == 4) return launch_units(aligned ? adapter_up_kernel<T, 4, true> : adapter_up_kernel<T, 4, false>, p, parts, 256, stream);
-  return launch_units(aligned ? adapter_up_kernel<T, 8, true> : adapter_up_kernel<T, 8, false>, p, parts, 256, stream);
+  const bool fast = p.runs && p.cols % 16 == 0 && p.rank % v == 0 && multiple(p.up, 2 * v) && (p.count <= 1 || p.up_stride0 % (2 * v) == 0) &&
+                    (p.cols <= 1 || p.up_stride1 % (2 * v) == 0);
+  if (p.out_type == Float::kF32) return fast ? launch_up_of<T, Float::kF32, true>(p, parts, stream) : launch_up_of<T, Float::kF32, false>(p, parts, stream);
+  return fast ? launch_up_of<T, T, true>(p, parts, stream) : launch_up_of<T, T, false>(p, parts, stream);
 }
 
 // Whether the pieces of work of both launches are fewer than 2^31.
 bool countable(const AdapterProduct& p) {
-  const int64_t tiles = ((int64_t)p.lhs.rows + 15) / 16, blocks = (p.rank + 15) / 16;
-  const int64_t parts = ((int64_t)p.cols + 64 * kFragments - 1) / (64 * kFragments), most = (1ll << 31) / (tiles * p.slots);
-  return blocks * p.splits < most && parts < most;
+  const int64_t tiles = ((int64_t)p.lhs.rows + 15) / 16, blocks = (p.rank + 15) / 16, most = (1ll << 31) / (tiles * p.slots);
+  return blocks * p.splits < most && column_parts(p.cols, p.rank) < most;
 }
 
 }  // namespace
