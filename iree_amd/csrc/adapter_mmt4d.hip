@@ -87,6 +87,7 @@ struct AdapterProduct {
   Layout out_at;
   Float out_type;
   uint32_t depth, rank, count, cols, pitch, splits;
+  uint32_t turns;           // blocks of columns that a wavefront multiplies by `up`, one after the other
   uint32_t slots, units;    // of a launch: workgroups' pieces of work
   uint32_t parts, parts_reciprocal, slots_reciprocal;
   int32_t accumulate, runs;
@@ -197,37 +198,68 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_down_kernel(const Adapter
   }
 }
 
-// 16 rows times 16 * F columns a wavefront, of four. Sums and products are f32: v_mfma_f32_16x16x4, lane (r, g) with V ranks from V g on
-// of each 4 V, of row r of the sums and of column r; RANKS times 4 V ranks at a time. The splits' sums are added on their way into LDS,
-// where all four have them from, and only those of rows that have the adapter are read: sixteen rows' sums of 64 ranks and two splits
-// are 8 KiB, twice what 32 columns of `up` are. Addresses are a part that is the wavefront's (scalar) and 32 bits that are the lane's.
+// A sum in f32 as two or three 16-bit floats that add up to it: bf16 takes the 24 bits of its mantissa eight at a time, exactly; f16
+// the nearest, then the nearest to what that leaves, which is 2^-24 of it off at most, a sum having been brought into f16's range with
+// the others of its row first (`unit`, a power of two).
+template <Float T> constexpr int kSumParts = T == Float::kF16 ? 2 : 3;
+template <Float T>
+__device__ __forceinline__ void split_sum(float v, uint16_t (&part)[3]) {
+  if constexpr (T == Float::kBf16) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const uint32_t bits = __builtin_bit_cast(uint32_t, v);
+      part[i] = (uint16_t)(bits >> 16);
+      const float rest = v - __builtin_bit_cast(float, bits & 0xFFFF0000u);
+      v = rest == rest ? rest : 0;  // (of an infinity nothing is left)
+    }
+  } else {
+    part[0] = mx_narrow<T>(v);
+    const float rest = v - mx_widen<T>(part[0]);
+    part[1] = mx_narrow<T>(rest == rest ? rest : 0);
+    part[2] = 0;
+  }
+}
+
+// 16 rows times 16 * F columns a wavefront and turn. The rank sums are multiplied as 16-bit floats of which they are the sums, with
+// v_mfma_f32_16x16x32: of up to 16 ranks (HALF) two parts are one instruction's 32, lane (r, g) with eight from 8 (g & 1) on, of row r
+// of the sums and of column r. Otherwise a part of 32 CHUNKS ranks is CHUNKS instructions. (On v_mfma_f32_16x16x4, with `up` widened to
+// f32, 64 rows of 64 adapters x 14336, rank 16, took 17.5 us and not 14.0, of which the matrix instructions 3 and the widening and what
+// runs in front of a wavefront's first load most of the rest.)
 //
-// FAST: columns come in whole sixteens that lie next to each other, aligned, and an adapter's row of `up` in whole, aligned Vs. (As two
-// branches of one kernel the slow one's registers halved the number of wavefronts on a compute unit.)
-template <Float T, Float OUT, int V, int RANKS, int F, bool FAST>
+// MANY: more ranks than that, whose sums are taken anew in every turn.
+//
+// The splits' sums are added on their way into LDS, where a workgroup's four wavefronts have them from; only those of rows that have the
+// adapter are read. The next turn's `up` and results are on their way while one's are multiplied.
+//
+// FAST: columns come in whole sixteens that lie next to each other, aligned, and an adapter's row of `up` in whole eights, aligned. (As
+// two branches of one kernel the slow one's registers halved the number of wavefronts on a compute unit.)
+template <Float T, Float OUT, bool HALF, int CHUNKS, int F, bool FAST, bool MANY>
 __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterProduct p) {
-  constexpr int SIZE = OUT == Float::kF32 ? 4 : 2, GROUP = 4 * V * RANKS, PITCH = GROUP + 4;  // (rows 4 banks apart)
+  constexpr int SIZE = OUT == Float::kF32 ? 4 : 2, GROUP = HALF ? 16 : 32 * CHUNKS, PITCH = GROUP + 4;  // (rows 4 banks apart)
+  constexpr int PARTS = HALF ? (kSumParts<T> + 1) / 2 : kSumParts<T> * CHUNKS;  // operands of 32 values
   __shared__ float sums[16 * PITCH];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
+  const uint32_t own_rank = HALF ? 8 * (g & 1) : 8 * g;  // of a chunk's, the lane's first
   for (uint32_t unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
     // unit = (tile * slots + slot) * parts + block of columns
     const uint32_t upper = divide(unit, p.parts, p.parts_reciprocal), part = unit - upper * p.parts;
     const uint32_t tile = divide(upper, p.slots, p.slots_reciprocal), slot = upper - tile * p.slots;
-    const uint32_t first = tile * 16, first_col = (part * 4 + wave) * (16 * F);
+    const uint32_t first = tile * 16, first_col = (part * 4 + wave) * (16 * F * p.turns);
+    const uint32_t end_col = first_col + 16 * F * p.turns < p.cols ? first_col + 16 * F * p.turns : p.cols;
     const uint32_t row = first + r < p.lhs.rows ? first + r : p.lhs.rows - 1;
     uint8_t* const out = p.out + layout_row(p.out_at, first) * SIZE;
     const uint32_t out_row = (uint32_t)(layout_row(p.out_at, row) - layout_row(p.out_at, first));  // elements
-    // Four results, of fragment f, as they lie in memory.
+    // Four results, of the fragment at `col`, as they lie in memory.
     typedef uint32_t Words __attribute__((ext_vector_type(SIZE)));
-    auto four_at = [&](int f) {
-      uint8_t* const fragment = out + layout_col(p.out_at, first_col + 16 * f) * SIZE;
+    auto four_at = [&](uint32_t col) {
+      uint8_t* const fragment = out + layout_col(p.out_at, col) * SIZE;
       return (Words*)__builtin_assume_aligned(fragment + (out_row + 4 * g) * SIZE, 4 * SIZE);
     };
-    auto store_one_by_one = [&](int f, p16_v4f32 v) {
+    auto store_one_by_one = [&](uint32_t from, p16_v4f32 v) {
 #pragma unroll 1
       for (int e = 0; e < 4; ++e) {
-        const uint32_t col = first_col + 16 * f + 4 * g + e;
+        const uint32_t col = from + 4 * g + e;
         if (col >= p.cols) continue;
         const int64_t at = out_row + layout_col(p.out_at, col);
         const float x = v[e] + (p.accumulate ? element<OUT>(out, at) : 0);
@@ -237,88 +269,162 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterProduct p)
     };
     const uint32_t without = of_adapters(p, first, slot, lane, [&](uint32_t of, uint32_t same) {
       const bool mine = (same >> r & 1) != 0;
-      typedef uint16_t Run __attribute__((ext_vector_type(V)));
       const uint8_t* const up = p.up + of * p.up_stride0;
+      uint4 w[CHUNKS][F], t[PARTS];
       Words old[F] = {};
-      if (FAST && p.accumulate && mine) {
-#pragma unroll
-        for (int f = 0; f < F; ++f)
-          if (first_col + 16 * f < p.cols) old[f] = *four_at(f);
-      }
-      const float scale = p.scales ? p.scales[of] : 1;
-      p16_v4f32 acc[F] = {};
-      for (uint32_t rank0 = 0; rank0 < p.rank; rank0 += GROUP) {
-        Run w[RANKS][F];
+      float unit_of_row = 1;
+      auto load_up = [&](uint4 (&to)[CHUNKS][F], uint32_t col0, uint32_t rank0) {
 #pragma unroll
         for (int f = 0; f < F; ++f) {
-          const uint32_t col = first_col + 16 * f + r;
-          const uint32_t at = (col < p.cols ? col : p.cols - 1) * (uint32_t)p.up_stride1 + 2 * (rank0 + V * g);
+          const uint32_t col = col0 + 16 * f + r;
+          const uint32_t at = (col < p.cols ? col : p.cols - 1) * (uint32_t)p.up_stride1 + 2 * (rank0 + own_rank);
 #pragma unroll
-          for (int c = 0; c < RANKS; ++c) {
-            const uint32_t rank = rank0 + 4 * V * c + V * g;
-            w[c][f] = Run(0);
+          for (int c = 0; c < CHUNKS; ++c) {
+            const int exist = (int)p.rank - (int)(rank0 + 32 * c + own_rank);
+            to[c][f] = make_uint4(0, 0, 0, 0);
             if constexpr (FAST) {
-              if (rank < p.rank) w[c][f] = *(const Run*)(up + at + 8 * V * c);
+              if (exist > 0) to[c][f] = *(const uint4*)(up + at + 64 * c);
             } else {
-#pragma unroll
-              for (int e = 0; e < V; ++e)
-                if (rank + e < p.rank) w[c][f][e] = ((const uint16_t*)(up + at + 8 * V * c))[e];
+              to[c][f] = last_piece_anywhere(up + at + 64 * c, exist);
             }
           }
         }
+      };
+      auto load_old = [&](Words (&to)[F], uint32_t col0) {
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+          if (FAST && p.accumulate && mine && col0 + 16 * f < end_col) to[f] = *four_at(col0 + 16 * f);
+      };
+      // The sums of ranks from rank0 on, as operands.
+      auto take_sums = [&](uint32_t rank0) {
         // Four ranks of a row each thread. (The pitch is a multiple of 32 ranks; what lies behind it is not there.)
-        const uint32_t of_row = threadIdx.x / (GROUP / 4), four = 4 * (threadIdx.x % (GROUP / 4));
-        if (of_row < 16 && (same >> of_row & 1) != 0 && rank0 + four < p.pitch) {
-          const float* at = p.sums + (int64_t)(first + of_row) * p.pitch + rank0 + four;
-          const int64_t split = (int64_t)p.lhs.rows * p.pitch;
+#pragma unroll
+        for (int n = 0; n < (16 * GROUP / 4 + 255) / 256; ++n) {
+          const uint32_t number = threadIdx.x + 256 * n, of_row = number / (GROUP / 4), four = 4 * (number % (GROUP / 4));
+          if (of_row >= 16) continue;
           p16_v4f32 v = {0, 0, 0, 0};
-          for (uint32_t s = 0; s < p.splits; s += 4) {  // (four under way at a time)
-            p16_v4f32 part[4];
+          if ((same >> of_row & 1) != 0 && rank0 + four < p.pitch) {
+            const float* at = p.sums + (int64_t)(first + of_row) * p.pitch + rank0 + four;
+            const int64_t split = (int64_t)p.lhs.rows * p.pitch;
+            for (uint32_t s = 0; s < p.splits; s += 4) {  // (four under way at a time)
+              p16_v4f32 part[4];
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) part[i] = s + i < p.splits ? *(const p16_v4f32*)(at + (s + i) * split) : p16_v4f32{0, 0, 0, 0};
+              for (uint32_t i = 0; i < 4; ++i) part[i] = s + i < p.splits ? *(const p16_v4f32*)(at + (s + i) * split) : p16_v4f32{0, 0, 0, 0};
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) v += part[i];
+              for (uint32_t i = 0; i < 4; ++i) v += part[i];
+            }
           }
           *(p16_v4f32*)(sums + of_row * PITCH + four) = v;
         }
         __syncthreads();
+        float v[CHUNKS][8], largest = 0;
 #pragma unroll
-        for (int c = 0; c < RANKS; ++c)
+        for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-          for (int e = 0; e < V; e += 4) {
-            const p16_v4f32 sum = *(const p16_v4f32*)(sums + r * PITCH + 4 * V * c + V * g + e);
+          for (int e = 0; e < 8; e += 4) {
+            const p16_v4f32 four = *(const p16_v4f32*)(sums + r * PITCH + 32 * c + own_rank + e);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int f = 0; f < F; ++f)
-                acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(mx_widen<T>(w[c][f][e + i]), sum[i], acc[f], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+              v[c][e + i] = four[i];
+              largest = __builtin_fmaxf(largest, __builtin_fabsf(four[i]));
+            }
           }
         __syncthreads();
-      }
-      if (!mine) return;
+        if constexpr (T == Float::kF16) {
+          // To below 2^15, with the row's other ranks. (What is not finite, and zeros, as they are.)
+          largest = __builtin_fmaxf(largest, __shfl_xor(largest, 16));
+          largest = __builtin_fmaxf(largest, __shfl_xor(largest, 32));
+          const int field = (int)(__builtin_bit_cast(uint32_t, largest) >> 23);
+          const int by = field == 255 || field < 24 ? 0 : 127 + 14 - field;
+          unit_of_row = ldexpf(1.0f, -by);
 #pragma unroll
-      for (int f = 0; f < F; ++f) {
-        p16_v4f32 v = acc[f] * scale;
-        if constexpr (!FAST) {
-          store_one_by_one(f, v);
-        } else if (first_col + 16 * f < p.cols) {
-          if constexpr (OUT == Float::kF32) {
-            v += __builtin_bit_cast(p16_v4f32, old[f]);
-            *four_at(f) = __builtin_bit_cast(Words, v);
-          } else {
-            float x[4];
+          for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = v[e] + mx_widen<OUT>((uint16_t)(old[f][e / 2] >> (16 * (e & 1))));
-            *four_at(f) = Words{mx_narrow_pair<OUT>(x[0], x[1]), mx_narrow_pair<OUT>(x[2], x[3])};
+            for (int e = 0; e < 8; ++e) v[c][e] = ldexpf(v[c][e], by);
+        }
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          uint32_t words[3][4];
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            uint16_t even[3], odd[3];
+            split_sum<T>(v[c][e], even);
+            split_sum<T>(v[c][e + 1], odd);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) words[i][e / 2] = (uint32_t)even[i] | (uint32_t)odd[i] << 16;
           }
+          auto operand = [&](int i) { return make_uint4(words[i][0], words[i][1], words[i][2], words[i][3]); };
+          if constexpr (HALF) {
+            const uint4 a = operand(0), b = operand(1), d = operand(2), none = make_uint4(0, 0, 0, 0);
+            t[0] = g < 2 ? a : b;
+            if constexpr (PARTS > 1) t[1] = g < 2 ? d : none;
+          } else {
+#pragma unroll
+            for (int i = 0; i < kSumParts<T>; ++i) t[c * kSumParts<T> + i] = operand(i);
+          }
+        }
+      };
+      p16_v4f32 acc[F];
+      auto multiply = [&](const uint4 (&by)[CHUNKS][F]) {
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i)
+#pragma unroll
+          for (int f = 0; f < F; ++f) acc[f] = mfma16_16<T>(by[HALF ? 0 : i / kSumParts<T>][f], t[i], acc[f]);
+      };
+      load_up(w, first_col < p.cols ? first_col : 0, 0);
+      load_old(old, first_col);
+      const float scale = p.scales ? p.scales[of] : 1;
+      if constexpr (!MANY) take_sums(0);
+      // (Everyone goes round as often, for the sums' sake.)
+      for (uint32_t turn = 0; turn < p.turns; ++turn) {
+        const uint32_t col0 = first_col + 16 * F * turn, next_col = col0 + 16 * F < end_col ? col0 + 16 * F : 0;
+#pragma unroll
+        for (int f = 0; f < F; ++f) acc[f] = p16_v4f32{0, 0, 0, 0};
+        if constexpr (MANY) {
+          p16_v4f32 total[F] = {};
+          for (uint32_t rank0 = 0; rank0 < p.rank; rank0 += GROUP) {
+            take_sums(rank0);
+            multiply(w);
+            const bool last = rank0 + GROUP >= p.rank;
+            load_up(w, last ? next_col : col0 < p.cols ? col0 : 0, last ? 0 : rank0 + GROUP);
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+              total[f] += acc[f] * unit_of_row;
+              acc[f] = p16_v4f32{0, 0, 0, 0};
+            }
+          }
+#pragma unroll
+          for (int f = 0; f < F; ++f) acc[f] = total[f];
+        } else {
+          multiply(w);
+          if (turn + 1 < p.turns) load_up(w, next_col, 0);
+        }
+        if (mine) {
+#pragma unroll
+          for (int f = 0; f < F; ++f) {
+            const uint32_t col = col0 + 16 * f;
+            if (col >= end_col) continue;
+            p16_v4f32 v = acc[f] * (MANY ? scale : unit_of_row * scale);
+            if constexpr (!FAST) {
+              store_one_by_one(col, v);
+            } else if constexpr (OUT == Float::kF32) {
+              v += __builtin_bit_cast(p16_v4f32, old[f]);
+              *four_at(col) = __builtin_bit_cast(Words, v);
+            } else {
+              float x[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = v[e] + mx_widen<OUT>((uint16_t)(old[f][e / 2] >> (16 * (e & 1))));
+              *four_at(col) = Words{mx_narrow_pair<OUT>(x[0], x[1]), mx_narrow_pair<OUT>(x[2], x[3])};
+            }
+          }
+          if (turn + 1 < p.turns) load_old(old, col0 + 16 * F);
         }
       }
     });
     if (!p.accumulate && slot == 0 && (without >> r & 1) != 0 && first + r < p.lhs.rows) {
-#pragma unroll 1
-      for (int f = 0; f < F; ++f) {
-        if constexpr (!FAST) store_one_by_one(f, p16_v4f32{0, 0, 0, 0});
-        else if (first_col + 16 * f < p.cols) *four_at(f) = Words(0);
+      for (uint32_t col = first_col; col < end_col; col += 16) {
+        if constexpr (!FAST) store_one_by_one(col, p16_v4f32{0, 0, 0, 0});
+        else *four_at(col) = Words(0);
       }
     }
   }
@@ -335,9 +441,16 @@ int64_t pitch_of(int64_t rank) { return (rank + 31) / 32 * 32; }
 
 bool multiple(const void* p, int64_t to) { return (uintptr_t)p % to == 0; }
 
-// Fragments of columns of a wavefront that multiplies by `up`.
+// Fragments of columns of a wavefront's turn, and turns: as many as leave some 4096 wavefronts, sixteen to a compute unit.
 int up_fragments(int64_t rank) { return rank <= 32 ? 4 : 2; }
-int64_t column_parts(int64_t cols, int64_t rank) { return (cols + 64 * up_fragments(rank) - 1) / (64 * up_fragments(rank)); }
+uint32_t turns_of(int64_t rows, int64_t slots, int64_t cols, int64_t rank) {
+  const int64_t across = (cols + 16 * up_fragments(rank) - 1) / (16 * up_fragments(rank)), t = (rows + 15) / 16 * slots * across / 4096;
+  return (uint32_t)(t < 1 ? 1 : t > 8 ? 8 : t);
+}
+int64_t column_parts(const AdapterProduct& p) {
+  const int64_t of_group = 64 * (int64_t)up_fragments(p.rank) * p.turns;
+  return (p.cols + of_group - 1) / of_group;
+}
 
 // The problem as the kernels on the matrix pipe take it; false: they do not.
 bool as_product(const AdapterArgs& a, AdapterProduct* p) {
@@ -367,6 +480,7 @@ bool as_product(const AdapterArgs& a, AdapterProduct* p) {
   const int64_t slots = 128 / tiles, most = a.count < 16 ? a.count : 16;
   p->slots = (uint32_t)(slots < 1 ? 1 : slots > most ? most : slots);
   p->slots_reciprocal = reciprocal_of(p->slots);
+  p->turns = turns_of(rows, p->slots, cols, a.rank);
   return true;
 }
 
@@ -389,16 +503,16 @@ hipError_t launch_down(const AdapterProduct& p, hipStream_t stream) {
 
 template <Float T, Float OUT, bool FAST>
 hipError_t launch_up_of(const AdapterProduct& p, int64_t parts, hipStream_t stream) {
-  if (p.rank <= 16) return launch_units(adapter_up_kernel<T, OUT, 4, 1, 4, FAST>, p, parts, 256, stream);
-  if (p.rank <= 32) return launch_units(adapter_up_kernel<T, OUT, 8, 1, 4, FAST>, p, parts, 256, stream);
-  return launch_units(adapter_up_kernel<T, OUT, 8, 2, 2, FAST>, p, parts, 256, stream);
+  if (p.rank <= 16) return launch_units(adapter_up_kernel<T, OUT, true, 1, 4, FAST, false>, p, parts, 256, stream);
+  if (p.rank <= 32) return launch_units(adapter_up_kernel<T, OUT, false, 1, 4, FAST, false>, p, parts, 256, stream);
+  if (p.rank <= 64) return launch_units(adapter_up_kernel<T, OUT, false, 2, 2, FAST, false>, p, parts, 256, stream);
+  return launch_units(adapter_up_kernel<T, OUT, false, 2, 2, FAST, true>, p, parts, 256, stream);
 }
 template <Float T>
 hipError_t launch_up(const AdapterProduct& p, hipStream_t stream) {
-  const int64_t parts = column_parts(p.cols, p.rank);
-  const int v = p.rank <= 16 ? 4 : 8;
-  const bool fast = p.runs && p.cols % 16 == 0 && p.rank % v == 0 && multiple(p.up, 2 * v) && (p.count <= 1 || p.up_stride0 % (2 * v) == 0) &&
-                    (p.cols <= 1 || p.up_stride1 % (2 * v) == 0);
+  const int64_t parts = column_parts(p);
+  const bool fast = p.runs && p.cols % 16 == 0 && p.rank % 8 == 0 && multiple(p.up, 16) && (p.count <= 1 || p.up_stride0 % 16 == 0) &&
+                    (p.cols <= 1 || p.up_stride1 % 16 == 0);
   if (p.out_type == Float::kF32) return fast ? launch_up_of<T, Float::kF32, true>(p, parts, stream) : launch_up_of<T, Float::kF32, false>(p, parts, stream);
   return fast ? launch_up_of<T, T, true>(p, parts, stream) : launch_up_of<T, T, false>(p, parts, stream);
 }
@@ -406,7 +520,7 @@ hipError_t launch_up(const AdapterProduct& p, hipStream_t stream) {
 // Whether the pieces of work of both launches are fewer than 2^31.
 bool countable(const AdapterProduct& p) {
   const int64_t tiles = ((int64_t)p.lhs.rows + 15) / 16, blocks = (p.rank + 15) / 16, most = (1ll << 31) / (tiles * p.slots);
-  return blocks * p.splits < most && column_parts(p.cols, p.rank) < most;
+  return blocks * p.splits < most && column_parts(p) < most;
 }
 
 }  // namespace

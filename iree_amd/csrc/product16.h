@@ -102,6 +102,14 @@ __device__ __forceinline__ uint4 last_piece(const uint8_t* at, int exist) {
   return make_uint4((uint32_t)low, (uint32_t)(low >> 32), (uint32_t)high, (uint32_t)(high >> 32));
 }
 
+// The same at an address that is a multiple of 2 only. (Loads of 16 bytes need no alignment here.)
+__device__ __forceinline__ uint4 last_piece_anywhere(const uint8_t* at, int exist) {
+  if (exist < 8) return last_piece(at, exist);
+  uint4 v;
+  __builtin_memcpy(&v, at, 16);
+  return v;
+}
+
 // COUNT (4 or 8) consecutive elements at an address that is a multiple of their size, of 16 bytes at most.
 template <Float T, int COUNT>
 __device__ __forceinline__ void load_run(const uint8_t* p, int64_t at, float (&v)[COUNT]) {
