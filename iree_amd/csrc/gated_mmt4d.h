@@ -7,7 +7,8 @@
 namespace uk {
 
 struct GatedResults {
-  static constexpr bool kPaired = true;
+  static constexpr bool kPaired = true, kInTurn = false;
+  static constexpr int kResults = 1;
   uint8_t *out, *gate_pre, *up_pre;  // the latter two null: none
   Layout out_at, gate_at, up_at;
   Curve curve;
@@ -19,7 +20,7 @@ struct GatedResults {
   // 32, gates in the first half of its registers and ups in the second.
   template <Float T, int AM, int BN>
   __device__ __forceinline__ void store(const p16_v16f32 (&acc)[AM][BN], uint32_t row0, uint32_t col0, uint32_t rows, uint32_t cols,
-                                        int lane) const {
+                                        int lane, uint32_t) const {
     const int r = lane & 31, half = lane >> 5;
 #pragma unroll
     for (int i = 0; i < AM; ++i) {
@@ -65,17 +66,7 @@ struct GatedResults {
       if (out_type == Float::kF32) put_four<T>(Float::kF32, out, out_row + layout_col(out_at, from), h + 4 * q);
     }
     if (out_type == Float::kF32) return;
-    // The two lanes of a row exchange halves, and each has eight consecutive columns.
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      typedef uint32_t v2u32 __attribute__((ext_vector_type(2)));
-      const v2u32 both = __builtin_bit_cast(v2u32, __builtin_amdgcn_permlane32_swap(mx_narrow_pair<T>(h[2 * e], h[2 * e + 1]),
-                                                                                    mx_narrow_pair<T>(h[4 + 2 * e], h[5 + 2 * e]), false, false));
-      w[e] = both[0];
-      w[2 + e] = both[1];
-    }
-    *(uint4*)((uint16_t*)out + out_row + layout_col(out_at, col + 8 * half)) = make_uint4(w[0], w[1], w[2], w[3]);
+    *(uint4*)((uint16_t*)out + out_row + layout_col(out_at, col + 8 * half)) = eight_of_two_lanes<T>(h);
   }
   template <Float T>
   __device__ __forceinline__ void add_four(const uint8_t* p, int64_t at, float* v) const {

@@ -10,11 +10,12 @@ namespace {
 
 template <Float T>
 hipError_t launch_gated_block(const GatedProduct& g, int tile, hipStream_t stream) {
-  BlockProduct<GatedResults> p;
+  BlockProduct<GatedResults, Operand16, Operand16> p;
   p.lhs = g.lhs;
   p.rhs = g.gate;
   p.second = g.up;
   p.second_stride0 = g.up_stride0;
+  p.lhs_second = 0;
   p.depth = g.depth;
   p.epilogue = g.results;
   // Weights that no cache holds and that a tile or two of rows read once go past the caches: 64 rows x 28672 x 8192 (940 MB) 165 -> 148

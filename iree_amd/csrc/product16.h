@@ -17,6 +17,14 @@ struct Operand16 {
   uint32_t row_bytes, piece1, piece2;
 };
 
+// An operand whose rows' values of one k lie next to each other: element (k, row) in panel k / tile_rows, row_bytes apart within it, and
+// then as a matrix of tiles has its columns (tiles n0 wide, tile_bytes apart). tile_rows is 1, 2, 4, .. 32, n0 a multiple of 8.
+struct Strided16 {
+  const uint8_t* data;
+  int64_t stride0;  // bytes from a panel to the next
+  uint32_t rows, log2_tile_rows, row_bytes, n0, n0_reciprocal, tile_bytes;
+};
+
 // A result or another matrix laid out like it: element (row, col) at row / tile_rows * stride0 + (col / n0) * tile + (row %
 // tile_rows) * n0 + col % n0.
 struct Layout {
@@ -48,6 +56,23 @@ inline bool as_operand16(const uint8_t* data, int64_t stride0, int64_t panels, i
   o->row_bytes = m0 == 1 ? 0 : 2 * k0;
   o->piece1 = k0 == 8 ? 16 * m0 : 16;
   o->piece2 = k0 == 32 ? 32 : 32 * m0;
+  return true;
+}
+// The same matrix [panels][K][M0][K0] with its first dimension contracted. (32 of its rows within 31 bits of each other.)
+inline bool as_strided16(const uint8_t* data, int64_t stride0, int64_t panels, int64_t M0, int64_t K, int64_t K0, Strided16* o) {
+  const int64_t cols = K * K0, n0 = M0 == 1 ? cols : K0;
+  if (cols == 0 || cols > 0x7FFFFFFF - 512 || n0 % 8 != 0 || M0 > 32 || (M0 & (M0 - 1)) != 0) return false;
+  if ((uintptr_t)data % 16 != 0 || (panels > 1 && stride0 % 8 != 0)) return false;
+  const int64_t apart = panels > 1 ? 2 * stride0 : 0;
+  if (apart * (32 / M0) + 2 * M0 * cols >= 1ll << 31) return false;
+  o->data = data;
+  o->stride0 = apart;
+  o->rows = (uint32_t)cols;
+  o->log2_tile_rows = (uint32_t)__builtin_ctz((unsigned)M0);
+  o->row_bytes = M0 == 1 ? 0 : (uint32_t)(2 * K0);
+  o->n0 = (uint32_t)n0;
+  o->n0_reciprocal = reciprocal_of(o->n0);
+  o->tile_bytes = M0 == 1 ? 0 : (uint32_t)(2 * M0 * K0);
   return true;
 }
 // Whether rows up to `apart` apart lie within 31 bits of each other.
@@ -132,6 +157,22 @@ __device__ __forceinline__ void store_run(uint8_t* p, int64_t at, const float (&
     for (int i = 0; i < COUNT; i += 2) w[i / 2] = mx_narrow_pair<T>(v[i], v[i + 1]);
     __builtin_memcpy(__builtin_assume_aligned((uint16_t*)p + at, 2 * COUNT), w, 2 * COUNT);
   }
+}
+
+// Of sixteen columns of a row two lanes, 32 apart, have 4 half to + 3 and 8 + 4 half to + 3. They exchange halves, and each returns
+// eight consecutive ones, from 8 half on, rounded.
+template <Float T>
+__device__ __forceinline__ uint4 eight_of_two_lanes(const float (&v)[8]) {
+  typedef uint32_t v2u32 __attribute__((ext_vector_type(2)));
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const v2u32 both = __builtin_bit_cast(v2u32, __builtin_amdgcn_permlane32_swap(mx_narrow_pair<T>(v[2 * e], v[2 * e + 1]),
+                                                                                  mx_narrow_pair<T>(v[4 + 2 * e], v[5 + 2 * e]), false, false));
+    w[e] = both[0];
+    w[2 + e] = both[1];
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 }  // namespace uk

@@ -1,17 +1,22 @@
 // Products of 16-bit floats of many rows: block tiles through LDS.
 //
 // A workgroup of four wavefronts (2 x 2) multiplies 64 AM rows of the lhs with 64 BN rows of the rhs, each wavefront AM x BN
-// fragments of v_mfma_f32_32x32x16. K goes by in chunks of 32 values, 64 bytes of a row, which travel global memory -> LDS without
-// passing through registers into a ring of STAGES stages.
+// fragments of v_mfma_f32_32x32x16. K goes by in chunks of 32 values, which travel global memory -> LDS without passing through
+// registers into a ring of STAGES stages.
 //
-// LDS holds a chunk's rows one after the other, a row's 16-byte pieces exchanged among themselves so that the lanes that a read
-// serves together find theirs in different banks. Loads write LDS in lane order, so it is the global address of a lane that is
-// chosen; four neighbouring lanes still read one row's 64 bytes.
+// An operand is of one of two kinds. Operand16: a row's K is contiguous, 64 bytes a chunk. LDS holds a chunk's rows one after the
+// other, a row's 16-byte pieces exchanged among themselves so that the lanes that a read serves together find theirs in different
+// banks. Strided16: the rows' values of one k are contiguous. LDS holds a chunk's 32 ks one after the other, 128 bytes for each 64
+// rows, and the transposing read hands a lane four ks of its row: sixteen lanes read 32 bytes of each of four ks, which lie in
+// different banks because a k's 32-byte units are exchanged among themselves. Loads write LDS in lane order, so it is the global
+// address of a lane that is chosen; neighbouring lanes still read neighbouring pieces.
 //
 // The rhs fragment is the instruction's row operand, so that a lane ends up with four consecutive columns of one row of the result.
 //
-// An epilogue E takes the accumulators. With E::kPaired the rhs are two matrices of the same layout: of each 32 rows in LDS the
-// first 16 are the first's, the others the second's of the same numbers, so that a lane has both products of a column.
+// An epilogue E takes the accumulators, and says what the rhs is. E::kPaired: two matrices of the same layout side by side: of each 32
+// rows in LDS the first 16 are the first's, the others the second's of the same numbers, so that a lane has both products of a
+// column. E::kInTurn: two matrices one behind the other along K, the lhs's K being twice as long (its second half `lhs_second` bytes
+// behind its first).
 #ifndef IREE_AMD_CSRC_PRODUCT16_BLOCK_H_
 #define IREE_AMD_CSRC_PRODUCT16_BLOCK_H_
 
@@ -21,12 +26,14 @@
 
 namespace uk {
 
-template <typename E>
+template <typename E, typename A, typename B>
 struct BlockProduct {
-  Operand16 lhs, rhs;
-  const uint8_t* second;  // of a pair: the other rhs
+  A lhs;
+  B rhs;
+  const uint8_t* second;  // the other rhs
   int64_t second_stride0;
-  uint32_t depth;         // 32 at least
+  int64_t lhs_second;
+  uint32_t depth;         // of one rhs
   uint32_t tile_rows, tile_cols, band_reciprocal;
   E epilogue;
 };
@@ -35,8 +42,8 @@ namespace {
 
 extern __shared__ uint4 ring[];
 
-// 64 x 16 bytes to LDS byte offset `lds` (of the wavefront) from `base` + the lane's `offset`, past the caches or through them. The compiler does not see that they
-// write LDS and keeps no order between them and reads: wait_and_meet does.
+// 64 x 16 bytes to LDS byte offset `lds` (of the wavefront) from `base` + the lane's `offset`, past the caches or through them. The
+// compiler does not see that they write LDS and keeps no order between them and reads: wait_and_meet does.
 template <bool STREAM = false>
 __device__ __forceinline__ void load_pieces(uint32_t lds, uint32_t offset, const uint8_t* base) {
   if constexpr (STREAM)
@@ -75,12 +82,99 @@ __device__ __forceinline__ void each_of(F f) {
 // A row's piece `c` lies at piece c ^ exchanged(row).
 __device__ __forceinline__ uint32_t exchanged(uint32_t row) { return ((row >> 2) & 3) ^ (row & 2); }
 
+// One side of a tile: 64 W rows from `first` on, loaded 16 bytes a lane, W loads a wavefront for a chunk. `number` of a load: 0 to 4 W -
+// 1; `row_number`: the sixteen rows that it has (of a pair half of them are another matrix's).
+template <int W>
+__device__ __forceinline__ const uint8_t* first_of(const Operand16& o, const uint8_t* data, int64_t stride0, uint32_t first) {
+  return uniform_pointer(data + (int64_t)divide(first, o.tile_rows, o.tile_reciprocal) * stride0);
+}
+template <int W>
+__device__ __forceinline__ uint32_t piece_of(const Operand16&, uint32_t number, int lane) {
+  return (lane % 4) ^ exchanged(number * 16 + lane / 4);
+}
+// A lane's offset from there. Rows behind the last are read as the last.
+template <int W>
+__device__ __forceinline__ uint32_t offset_of(const Operand16& o, int64_t stride0, uint32_t first, uint32_t number, uint32_t row_number,
+                                              int lane, uint32_t depth) {
+  uint32_t row = first + row_number * 16 + lane / 4, piece = piece_of<W>(o, number, lane);
+  row = row < o.rows ? row : o.rows - 1;
+  if (8 * piece >= depth) piece = 0;  // (less than a chunk of K: it is loaded for nothing, and only what is there)
+  const uint32_t panel = divide(row, o.tile_rows, o.tile_reciprocal), first_panel = divide(first, o.tile_rows, o.tile_reciprocal);
+  return (uint32_t)((int64_t)(panel - first_panel) * stride0) + (row - panel * o.tile_rows) * o.row_bytes + (piece & 1) * o.piece1 +
+         (piece >> 1) * o.piece2;
+}
+// The lane's piece of what K has behind `full` whole chunks, `rest` values.
+template <int W>
+__device__ __forceinline__ uint4 rest_of(const Operand16& o, const uint8_t* at, uint32_t number, int lane, uint32_t rest) {
+  return last_piece(at, (int)rest - 8 * (int)piece_of<W>(o, number, lane));
+}
+__device__ __forceinline__ int64_t chunk_step(const Operand16& o) { return 64 * (int64_t)o.tile_rows; }
+
+__device__ __forceinline__ uint32_t column_bytes(const Strided16& o, uint32_t row) {
+  const uint32_t tile = divide(row, o.n0, o.n0_reciprocal);
+  return tile * o.tile_bytes + 2 * (row - tile * o.n0);
+}
+template <int W>
+__device__ __forceinline__ const uint8_t* first_of(const Strided16& o, const uint8_t* data, int64_t, uint32_t first) {
+  return uniform_pointer(data + column_bytes(o, first));
+}
+template <int W>
+__device__ __forceinline__ uint32_t k_of(uint32_t number, int lane) { return (number * 64 + lane) / (8 * W); }
+template <int W>
+__device__ __forceinline__ uint32_t offset_of(const Strided16& o, int64_t stride0, uint32_t first, uint32_t number, uint32_t, int lane,
+                                              uint32_t depth) {
+  uint32_t k = k_of<W>(number, lane);
+  const uint32_t at = (number * 64 + lane) % (8 * W), piece = 2 * ((at >> 1) ^ (k & 3)) + (at & 1);
+  const uint32_t row = first + 8 * piece < o.rows ? first + 8 * piece : o.rows - 8;
+  if (k >= depth) k = 0;
+  return (k >> o.log2_tile_rows) * (uint32_t)stride0 + (k & ((1u << o.log2_tile_rows) - 1)) * o.row_bytes + column_bytes(o, row) -
+         column_bytes(o, first);
+}
+template <int W>
+__device__ __forceinline__ uint4 rest_of(const Strided16&, const uint8_t* at, uint32_t number, int lane, uint32_t rest) {
+  return k_of<W>(number, lane) < rest ? *(const uint4*)at : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ int64_t chunk_step(const Strided16& o) { return o.stride0 * (32 >> o.log2_tile_rows); }
+
+// Reads of a fragment of 32 rows: lane (r, g) has row r of it and, of a step's 16 ks, 8 g to 8 g + 7. kReads of them; where a lane's
+// first one is in a chunk, `half`: the wavefront's of two.
+template <typename O> constexpr int kReads = std::is_same<O, Strided16>::value ? 2 : 1;
+template <int W>
+__device__ __forceinline__ uint32_t read_at(const Operand16&, int half, int lane) {
+  const int r = lane & 31, g = lane >> 5;
+  return (half * 32 * W + r) * 64 + 16 * (g ^ exchanged(r));
+}
+template <int W>
+__device__ __forceinline__ uint32_t read_at(const Strided16&, int half, int lane) {
+  const int q = lane >> 4, i = lane & 15;
+  return (8 * (q >> 1) + (i >> 2)) * (128 * W) + ((2 * W * half + (q & 1)) ^ (i >> 2)) * 32 + (i & 3) * 8;
+}
+// Read H of fragment F in step S.
+template <int W, int F, int S, int H>
+__device__ __forceinline__ void read_piece(const Operand16&, const uint8_t* side, uint32_t at, uint4& to) {
+  to = *(const uint4*)(side + F * 2048 + (at ^ (32 * S)));
+}
+template <int W, int F, int S, int H>
+__device__ __forceinline__ void read_piece(const Strided16&, const uint8_t* side, uint32_t at, uint4& to) {
+  typedef short v4i16 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4i16* Pointer;
+  const uint8_t* const from = side + (at ^ (64 * (F & 1))) + 128 * (F >> 1) + (16 * S + 4 * H) * (128 * W);
+  const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Pointer)(v4i16*)const_cast<uint8_t*>(from)));
+  if constexpr (H == 0) {
+    to.x = v.x;
+    to.y = v.y;
+  } else {
+    to.z = v.x;
+    to.w = v.y;
+  }
+}
+
 constexpr int block_lds_bytes(int am, int bn, int stages) { return stages * 64 * (am + bn) * 64; }
 
-template <Float T, int AM, int BN, int STAGES, bool STREAM, typename E>
+template <Float T, int AM, int BN, int STAGES, bool STREAM, typename E, typename A, typename B>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AM * BN <= 8 && block_lds_bytes(AM, BN, STAGES) <= 80 * 1024 ? 2 : 1, 2)))
-void product16_block_kernel(const BlockProduct<E> p) {
-  constexpr bool PAIRED = E::kPaired;
+void product16_block_kernel(const BlockProduct<E, A, B> p) {
+  constexpr bool PAIRED = E::kPaired, IN_TURN = E::kInTurn;
   constexpr int ROWS = 64 * AM, COLS = 64 * BN, RESULTS = PAIRED ? COLS / 2 : COLS;
   constexpr int A_BYTES = ROWS * 64, STAGE = A_BYTES + COLS * 64;
   constexpr int A_LOADS = AM, B_LOADS = BN, LOADS = A_LOADS + B_LOADS;  // of a wavefront, for a chunk
@@ -91,41 +185,39 @@ void product16_block_kernel(const BlockProduct<E> p) {
   if ((blockIdx.x >> 3) >= per_xcd || linear >= tiles) return;
   int tile_row, tile_col;
   tile_of_number(linear, p.tile_rows, p.tile_cols, p.band_reciprocal, &tile_row, &tile_col);
-  const uint32_t first_row = (uint32_t)tile_row * ROWS, first_col = (uint32_t)tile_col * RESULTS;
+  // (Tiles of an epilogue's second result come behind those of its first.)
+  uint32_t result = 0;
+  if constexpr (E::kResults > 1) {
+    result = (uint32_t)tile_row >= p.epilogue.tile_rows_of_first ? 1 : 0;
+    tile_row -= result * p.epilogue.tile_rows_of_first;
+  }
+  const uint32_t first_row = (uint32_t)tile_row * ROWS;
+  const uint32_t first_col = (uint32_t)tile_col * RESULTS;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave_m = wave >> 1, wave_n = wave & 1;
-  const int r = lane & 31, g = lane >> 5;
 
-  // Loads: offsets of a lane from the panel that the tile begins in. Rows behind the last are read as the last.
-  const uint32_t lhs_panel = divide(first_row, p.lhs.tile_rows, p.lhs.tile_reciprocal);
-  const uint32_t rhs_panel = divide(first_col, p.rhs.tile_rows, p.rhs.tile_reciprocal);
-  const uint8_t* lhs = uniform_pointer(p.lhs.data + (int64_t)lhs_panel * p.lhs.stride0);
-  const uint8_t* const rhs_first = uniform_pointer(p.rhs.data + (int64_t)rhs_panel * p.rhs.stride0);
-  const uint8_t* const rhs_second = PAIRED ? uniform_pointer(p.second + (int64_t)rhs_panel * p.second_stride0) : rhs_first;
-  auto row_offset = [](const Operand16& o, int64_t stride0, uint32_t row, uint32_t first_panel, uint32_t piece) {
-    row = row < o.rows ? row : o.rows - 1;
-    const uint32_t panel = divide(row, o.tile_rows, o.tile_reciprocal);
-    return (uint32_t)((int64_t)(panel - first_panel) * stride0) + (row - panel * o.tile_rows) * o.row_bytes + (piece & 1) * o.piece1 +
-           (piece >> 1) * o.piece2;
-  };
-  // A load has sixteen rows in LDS; of a pair they are the first's or the second's.
+  // Loads. Of a pair a load has sixteen rows of the first or of the second.
+  const uint8_t* lhs = first_of<AM>(p.lhs, p.lhs.data + (E::kResults > 1 ? result * p.lhs_second : 0), p.lhs.stride0, first_row);
+  const uint8_t* const lhs_first = lhs;
+  const uint8_t* const rhs_first = first_of<BN>(p.rhs, p.rhs.data, p.rhs.stride0, first_col);
+  const uint8_t* const rhs_second = PAIRED || IN_TURN ? first_of<BN>(p.rhs, p.second, p.second_stride0, first_col) : rhs_first;
   auto is_second = [&](int i) { return PAIRED && ((wave * B_LOADS + i) & 1) != 0; };
-  uint32_t a_from[A_LOADS], b_from[B_LOADS];
-  auto a_piece_of = [&](int i) { return (lane % 4) ^ exchanged((wave * A_LOADS + i) * 16 + lane / 4); };
-  auto b_piece_of = [&](int i) { return (lane % 4) ^ exchanged((wave * B_LOADS + i) * 16 + lane / 4); };
   auto a_offset = [&](int i) {
-    return row_offset(p.lhs, p.lhs.stride0, first_row + (wave * A_LOADS + i) * 16 + lane / 4, lhs_panel, a_piece_of(i));
+    const uint32_t number = wave * A_LOADS + i;
+    return offset_of<AM>(p.lhs, p.lhs.stride0, first_row, number, number, lane, p.depth);
   };
   auto b_offset = [&](int i) {
-    const uint32_t number = wave * B_LOADS + i, row = first_col + (PAIRED ? number / 2 : number) * 16 + lane / 4;
-    return row_offset(p.rhs, is_second(i) ? p.second_stride0 : p.rhs.stride0, row, rhs_panel, b_piece_of(i));
+    const uint32_t number = wave * B_LOADS + i;
+    return offset_of<BN>(p.rhs, is_second(i) ? p.second_stride0 : p.rhs.stride0, first_col, number, PAIRED ? number / 2 : number, lane, p.depth);
   };
+  uint32_t a_from[A_LOADS], b_from[B_LOADS];
 #pragma unroll
   for (int i = 0; i < A_LOADS; ++i) a_from[i] = a_offset(i);
 #pragma unroll
   for (int i = 0; i < B_LOADS; ++i) b_from[i] = b_offset(i);
-  const uint32_t lhs_step = 64 * p.lhs.tile_rows, rhs_step = 64 * p.rhs.tile_rows;
+  const int64_t lhs_step = chunk_step(p.lhs);
+  int64_t rhs_step = chunk_step(p.rhs);
   // Of loads 0, 2, .. and of loads 1, 3, .. (of a pair the one's and the other's, in turn)
   const uint8_t *rhs_even = is_second(0) ? rhs_second : rhs_first, *rhs_odd = is_second(1) ? rhs_second : rhs_first;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)ring;
@@ -136,27 +228,40 @@ void product16_block_kernel(const BlockProduct<E> p) {
     else load_pieces<STREAM>(at + A_BYTES + (wave * B_LOADS + I - A_LOADS) * 1024, b_from[I - A_LOADS], (I - A_LOADS) % 2 ? rhs_odd : rhs_even);
   };
   // Behind the last chunk it is the last that is loaded again: no step is unlike the others.
-  const uint32_t full = p.depth >> 5, rest = p.depth & 31, chunks = full + (rest != 0);
+  const uint32_t full = p.depth >> 5, rest = p.depth & 31;
+  const uint32_t by_registers = rest == 0 ? 0 : IN_TURN ? 2 : 1, chunks = (IN_TURN ? 2 : 1) * full + by_registers;
   uint32_t loading = 1;
   auto to_next_chunk = [&] {
-    const bool more = loading++ < full;
-    lhs += more ? lhs_step : 0;
-    rhs_even += more ? rhs_step : 0;
-    if constexpr (PAIRED && BN > 1) rhs_odd += more ? rhs_step : 0;
-    else rhs_odd = rhs_even;
+    if constexpr (IN_TURN) {
+      const bool turn = loading == full, more = loading++ < 2 * full;
+      lhs = turn ? lhs_first + p.lhs_second : lhs + (more ? lhs_step : 0);
+      rhs_even = turn ? rhs_second : rhs_even + (more ? rhs_step : 0);
+      if (turn) {
+        B other = p.rhs;
+        other.stride0 = p.second_stride0;
+        rhs_step = chunk_step(other);
+#pragma unroll
+        for (int i = 0; i < B_LOADS; ++i)
+          b_from[i] = offset_of<BN>(other, other.stride0, first_col, wave * B_LOADS + i, wave * B_LOADS + i, lane, p.depth);
+      }
+    } else {
+      const bool more = loading++ < full;
+      lhs += more ? lhs_step : 0;
+      rhs_even += more ? rhs_step : 0;
+      if constexpr (PAIRED && BN > 1) rhs_odd += more ? rhs_step : 0;
+    }
+    if constexpr (!PAIRED || BN == 1) rhs_odd = rhs_even;
   };
 
-  // Reads: a lane has row r of a fragment and, of the step's 16 values, piece g.
   const uint8_t* lds = (const uint8_t*)ring;
-  const uint32_t a_row = (wave_m * 32 * AM + r) * 64, b_row = A_BYTES + (wave_n * 32 * BN + r) * 64;
-  const uint32_t piece = 16 * (g ^ exchanged(r));
+  const uint32_t a_read = read_at<AM>(p.lhs, wave_m, lane), b_read = read_at<BN>(p.rhs, wave_n, lane);
   uint4 a[2][AM], b[2][BN];
-  constexpr int READS = AM + BN;
+  constexpr int A_READS = AM * kReads<A>, READS = A_READS + BN * kReads<B>;
   // Read number I of step S of the chunk at `at`.
   auto read = [&](const uint8_t* at, auto step, auto number) {
     constexpr int S = decltype(step)::value, I = decltype(number)::value;
-    if constexpr (I < AM) a[S][I] = *(const uint4*)(at + a_row + I * 2048 + (piece ^ (32 * S)));
-    else b[S][I - AM] = *(const uint4*)(at + b_row + (I - AM) * 2048 + (piece ^ (32 * S)));
+    if constexpr (I < A_READS) read_piece<AM, I / kReads<A>, S, I % kReads<A>>(p.lhs, at, a_read, a[S][I / kReads<A>]);
+    else read_piece<BN, (I - A_READS) / kReads<B>, S, (I - A_READS) % kReads<B>>(p.rhs, at + A_BYTES, b_read, b[S][(I - A_READS) / kReads<B>]);
   };
   p16_v16f32 acc[AM][BN] = {};
   // A step's MFMAs, and R reads and L loads (numbered) dealt out among them: a wavefront issues in order, what stands in front of
@@ -180,25 +285,36 @@ void product16_block_kernel(const BlockProduct<E> p) {
   typedef std::integral_constant<int, EARLY> EarlyLoads;
   typedef std::integral_constant<int, LOADS - EARLY> LateLoads;
 
-  // What K has behind its last whole chunk comes first, by way of registers, zeros behind it: the loop knows whole chunks only.
-  if (rest != 0) {
-    auto by_registers = [&](const uint8_t* at, uint32_t to, uint32_t c) {
-      *(uint4*)((uint8_t*)ring + to + 16 * lane) = last_piece(at, (int)rest - 8 * (int)c);
-    };
+  // What K (of one rhs, and of the other in turn) has behind its last whole chunk comes first, by way of registers, zeros behind it:
+  // the loop knows whole chunks only.
+  for (uint32_t s = 0; s < by_registers; ++s) {
+    const uint8_t* const of_lhs = lhs_first + (s == 0 ? 0 : p.lhs_second) + (int64_t)full * lhs_step;
+    B other = p.rhs;
+    other.stride0 = p.second_stride0;
+    const uint8_t* const of_second = rhs_second + (int64_t)full * chunk_step(other);
+    const uint8_t* const of_rhs = s == 0 ? rhs_first + (int64_t)full * chunk_step(p.rhs) : of_second;
+    uint8_t* const stage = (uint8_t*)ring + s * STAGE;
 #pragma unroll 1
-    for (int i = 0; i < A_LOADS; ++i)
-      by_registers(lhs + (uint64_t)full * lhs_step + a_offset(i), (wave * A_LOADS + i) * 1024, a_piece_of(i));
+    for (int i = 0; i < A_LOADS; ++i) {
+      const uint32_t number = wave * A_LOADS + i;
+      *(uint4*)(stage + number * 1024 + 16 * lane) =
+          rest_of<AM>(p.lhs, of_lhs + offset_of<AM>(p.lhs, p.lhs.stride0, first_row, number, number, lane, rest), number, lane, rest);
+    }
 #pragma unroll 1
-    for (int i = 0; i < B_LOADS; ++i)
-      by_registers((is_second(i) ? rhs_second : rhs_first) + (uint64_t)full * rhs_step + b_offset(i), A_BYTES + (wave * B_LOADS + i) * 1024,
-                   b_piece_of(i));
+    for (int i = 0; i < B_LOADS; ++i) {
+      const uint32_t number = wave * B_LOADS + i;
+      const bool second = is_second(i) || s != 0;
+      const uint32_t offset = offset_of<BN>(p.rhs, second ? p.second_stride0 : p.rhs.stride0, first_col, number, PAIRED ? number / 2 : number, lane, rest);
+      *(uint4*)(stage + A_BYTES + number * 1024 + 16 * lane) =
+          rest_of<BN>(p.rhs, (is_second(i) ? of_second : of_rhs) + offset, number, lane, rest);
+    }
   }
   // A chunk: its first step's MFMAs, among them its second step's reads; then the next chunk has come for everyone and this one's
   // stage is free; the second step's MFMAs, among them the next chunk's first reads. The loads of the chunk that goes into the
   // freed stage are dealt out over the two steps behind it.
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) {
-    if (s == 0 && rest != 0) continue;
+    if ((uint32_t)s < by_registers) continue;
     each_of<LOADS>([&](auto i) { load(lds0 + s * STAGE, i); });
     to_next_chunk();
   }
@@ -222,20 +338,24 @@ void product16_block_kernel(const BlockProduct<E> p) {
   for (int i = 0; i < AM; ++i)
 #pragma unroll
     for (int j = 0; j < BN; ++j) asm volatile("" : "+a"(acc[i][j]));
-  p.epilogue.template store<T, AM, BN>(acc, first_row + wave_m * 32 * AM, first_col + wave_n * (RESULTS / 2), p.lhs.rows, p.rhs.rows, lane);
+  p.epilogue.template store<T, AM, BN>(acc, first_row + wave_m * 32 * AM, first_col + wave_n * (RESULTS / 2), p.lhs.rows, p.rhs.rows, lane, result);
   // (The last loads have reached LDS before it is given to another workgroup.)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <Float T, int AM, int BN, int STAGES, bool STREAM = false, typename E>
-hipError_t launch_block_tile(BlockProduct<E> p, hipStream_t stream) {
+template <Float T, int AM, int BN, int STAGES, bool STREAM = false, typename E, typename A, typename B>
+hipError_t launch_block_tile(BlockProduct<E, A, B> p, hipStream_t stream) {
   constexpr int RESULTS = E::kPaired ? 32 * BN : 64 * BN, LDS = block_lds_bytes(AM, BN, STAGES);
   static_assert(LDS <= 160 * 1024, "LDS");
   p.tile_rows = (p.lhs.rows + 64 * AM - 1) / (64 * AM);
+  if constexpr (E::kResults > 1) {
+    p.epilogue.tile_rows_of_first = p.tile_rows;
+    p.tile_rows *= p.epilogue.results;
+  }
   p.tile_cols = (p.rhs.rows + RESULTS - 1) / RESULTS;
   p.band_reciprocal = band_reciprocal(p.tile_cols);
   const unsigned tiles = p.tile_rows * p.tile_cols;
-  void (*kernel)(const BlockProduct<E>) = product16_block_kernel<T, AM, BN, STAGES, STREAM, E>;
+  void (*kernel)(const BlockProduct<E, A, B>) = product16_block_kernel<T, AM, BN, STAGES, STREAM, E, A, B>;
   const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (e != hipSuccess) return e;
   return launch_kernel(kernel, (tiles + 7) / 8 * 8, 256, LDS, stream, p);
