@@ -7,25 +7,25 @@
 
 namespace uk {
 
-// Gradients on their way to memory: of one matrix, or of two of the same layout (but for their strides).
+// Gradients on their way to memory: copies of one layout (but for their strides), of which the first two have addresses of their own and
+// all of a lhs gradient's parts lie `apart` bytes behind each other.
 struct GradResults {
   uint8_t* out[2];
   int64_t stride0[2];
+  int64_t apart;
   Layout at;
   Float type;
   int32_t accumulate;
   int32_t runs;                // eight (f32: four) columns from a multiple of that on lie next to each other, aligned
   uint32_t rows;               // of each
-  uint32_t tile_rows_of_first;
-  uint32_t results;
+  uint32_t copies, tile_rows_of_copy, tile_rows_reciprocal;
 
   template <Float T, int AM, int BN>
   __device__ __forceinline__ void store_all(const p16_v16f32 (&acc)[AM][BN], uint32_t row0, uint32_t col0, uint32_t cols, int lane,
-                                            uint32_t result) const {
+                                            uint8_t* to, int64_t of_stride0) const {
     const int r = lane & 31, half = lane >> 5;
     Layout l = at;
-    l.stride0 = result ? stride0[1] : stride0[0];
-    uint8_t* const to = result ? out[1] : out[0];
+    l.stride0 = of_stride0;
 #pragma unroll
     for (int i = 0; i < AM; ++i) {
       const uint32_t row = row0 + 32 * i + r;
@@ -81,21 +81,19 @@ struct GradResults {
   }
 };
 struct LhsGrad : GradResults {
-  static constexpr bool kPaired = false, kInTurn = true;
-  static constexpr int kResults = 1;
+  static constexpr bool kPaired = false, kInTurn = true, kCopies = true;
   template <Float T, int AM, int BN>
   __device__ __forceinline__ void store(const p16_v16f32 (&acc)[AM][BN], uint32_t row0, uint32_t col0, uint32_t, uint32_t cols, int lane,
-                                        uint32_t) const {
-    store_all<T>(acc, row0, col0, cols, lane, 0);
+                                        uint32_t copy) const {
+    store_all<T>(acc, row0, col0, cols, lane, out[0] + copy * apart, stride0[0]);
   }
 };
 struct WeightGrads : GradResults {
-  static constexpr bool kPaired = false, kInTurn = false;
-  static constexpr int kResults = 2;
+  static constexpr bool kPaired = false, kInTurn = false, kCopies = true;
   template <Float T, int AM, int BN>
   __device__ __forceinline__ void store(const p16_v16f32 (&acc)[AM][BN], uint32_t row0, uint32_t col0, uint32_t, uint32_t cols, int lane,
-                                        uint32_t result) const {
-    store_all<T>(acc, row0, col0, cols, lane, result);
+                                        uint32_t copy) const {
+    store_all<T>(acc, row0, col0, cols, lane, copy ? out[1] : out[0], copy ? stride0[1] : stride0[0]);
   }
 };
 

@@ -7,7 +7,8 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// The workspace: [rows][2 * cols] of the operands' type, a row's dg then its du, each filled up with zeros to a multiple of eight.
+// The workspace: [rows][2 * cols] of the operands' type, a row's dg then its du, each filled up with zeros to a multiple of eight;
+// behind it, where lhs_grad's sums over the columns are split, [splits][rows][depth] of f32.
 struct Sizes {
   int64_t rows, cols, depth, pitch;
   explicit Sizes(const GatedBackwardArgs& a)
@@ -144,29 +145,39 @@ GradResults results_of(const GatedBackwardArgs& a, const Layout& at, uint8_t* fi
   other.stride0 = stride1;
   r.runs = runs_of(at, first, panels, e, 16 / e, 16) && (!second || runs_of(other, second, panels, e, 16 / e, 16));
   r.rows = (uint32_t)rows;
-  r.tile_rows_of_first = 0;
-  r.results = second ? 2 : 1;
+  r.apart = 0;
+  r.copies = second ? 2 : 1;
+  r.tile_rows_of_copy = r.tile_rows_reciprocal = 0;
   return r;
 }
 
-// Which tile: the least of the times that a model gives, in microseconds: a start, and chunks of K times what one of them takes with one
-// workgroup on a compute unit and, where LDS and registers hold two, with two; more than that follow each other. Fitted to the times of
-// every tile in 260 problems from 16 to 4096 rows, 64 to 28672 columns, K of 64 to 14336; over these the tile taken is slower than the
-// best one by 0.6 % (lhs) and 1.6 % (weights) in the mean. -1: none can.
+// Which tile, and how many parts K is split into: the least of the times that a model gives, in microseconds: a start, and chunks of K
+// times what one of them takes with one workgroup on a compute unit and, where LDS and registers hold two, with two; more than that
+// follow each other. Fitted to the times of every tile in 260 problems from 16 to 4096 rows, 64 to 28672 columns, K of 64 to 14336; over
+// these the tile taken is slower than the best one by 0.6 % (lhs) and 1.6 % (weights) in the mean. lhs_grad's K is both weights' rows
+// and its results few where the rows are: 19 x 18592 x 448 takes 25.7 us in 28 parts and 188 in one, 100 x 12176 x 3504 45 and 125, 508
+// x 9526 x 325 33 and 105. Over 120 problems of 1 to 4096 rows timed with every tile and ten numbers of parts, what is taken is slower
+// than the best by 2.2 % in the mean. tile -1: none can.
 struct Times { float start, one, two, start_again; };  // two = 0: one workgroup on a compute unit
-int choose_tile(const Times* times, int64_t rows, int64_t cols, int64_t chunks, int64_t results) {
-  int best = -1;
+struct Choice { int tile, splits; };
+Choice choose(const Times* times, int64_t rows, int64_t cols, int64_t chunks, int64_t copies, int64_t most_splits) {
+  Choice best = {-1, 1};
   float least = 0;
   for (int i = 0; i < (int)(sizeof kGradTiles / sizeof kGradTiles[0]); ++i) {
     const GradTile& t = kGradTiles[i];
-    const int64_t tiles = (rows + t.rows - 1) / t.rows * ((cols + t.cols - 1) / t.cols) * results, rounds = (tiles + 255) / 256;
-    if (tiles > (1 << 23)) continue;  // (a grid has fewer than 2^32 threads)
+    const int64_t of_one = (rows + t.rows - 1) / t.rows * ((cols + t.cols - 1) / t.cols) * copies;
     const Times& of = times[i];
-    const float steps = (float)chunks * (of.two == 0 ? rounds * of.one : (rounds >> 1) * of.two + (rounds & 1) * of.one);
-    const float cost = of.start + (rounds - 1) * of.start_again + steps;
-    if (best < 0 || cost < least) {
-      least = cost;
-      best = i;
+    for (int64_t splits = 1; splits <= most_splits; ++splits) {
+      const int64_t tiles = of_one * splits, rounds = (tiles + 255) / 256;
+      if (tiles > (1 << 23)) continue;  // (a grid has fewer than 2^32 threads)
+      // (The parts of sums are written and read, in a launch more.)
+      const float parts = splits == 1 ? 0 : 2 + (float)splits * (float)(rows * cols) * 1.5e-6f;
+      const float steps = (float)chunks / (float)splits * (of.two == 0 ? rounds * of.one : (rounds >> 1) * of.two + (rounds & 1) * of.one);
+      const float cost = of.start + (rounds - 1) * of.start_again + steps + parts;
+      if (best.tile < 0 || cost < least) {
+        least = cost;
+        best = {i, (int)splits};
+      }
     }
   }
   return best;
@@ -175,6 +186,49 @@ constexpr Times kLhsGradTimes[] = {{16.2f, .491f, 0, 21.5f},   {11.3f, .299f, 0,
                                    {7.7f, .157f, .418f, 1.1f}, {7.6f, .159f, .361f, 1.3f}, {6.6f, .137f, .246f, .9f}};
 constexpr Times kWeightGradTimes[] = {{17.3f, .522f, 0, 15.6f},   {11.9f, .323f, 0, 8.5f},   {11.6f, .303f, .747f, 4.1f}, {8.8f, .196f, .448f, 2.4f},
                                       {7.4f, .171f, .303f, 1.6f}, {7.3f, .164f, .313f, 1.6f}, {6.3f, .141f, .210f, 1.1f}};
+
+// lhs_grad's. A split has sixteen chunks at least, and all of them 64 MiB of sums at most.
+Choice choose_lhs_grad(const Sizes& s) {
+  if (s.rows < 1 || s.cols < 1 || s.depth < 1 || s.rows > INT32_MAX || s.cols > INT32_MAX || s.depth > INT32_MAX) return {-1, 1};
+  const int64_t whole = 2 * (s.cols / 32), of_sums = s.rows > (1 << 24) / s.depth ? 1 : (1 << 24) / (s.rows * s.depth);
+  const int64_t most = whole / 16 < of_sums ? whole / 16 : of_sums;
+  return choose(kLhsGradTimes, s.rows, s.depth, 2 * ((s.cols + 31) / 32), 1, most < 1 ? 1 : most > 32 ? 32 : most);
+}
+int64_t grads_bytes(const Sizes& s) { return (s.rows * s.pitch * 2 + 255) / 256 * 256; }
+
+// The sums of lhs_grad's splits, in their order: a thread for four of a row.
+struct SumArgs {
+  const float* parts;
+  uint8_t* out;
+  Layout at;
+  int64_t results, apart;  // fours; floats from a split to the next
+  uint32_t cols, fours;    // of a row
+  int32_t splits, runs;
+  Float type;
+};
+template <Float T>
+__global__ __launch_bounds__(kThreads) void gated_lhs_grad_sums(const SumArgs p) {
+  for (int64_t n = (int64_t)blockIdx.x * kThreads + threadIdx.x; n < p.results; n += (int64_t)gridDim.x * kThreads) {
+    const uint32_t row = (uint32_t)(n / p.fours), col = 4 * (uint32_t)(n - (int64_t)row * p.fours);
+    const float* const from = p.parts + (int64_t)row * p.cols + col;
+    float v[4];
+    load_run<Float::kF32, 4>((const uint8_t*)from, 0, v);
+    for (int32_t s = 1; s < p.splits; ++s) {
+      float more[4];
+      load_run<Float::kF32, 4>((const uint8_t*)(from + s * p.apart), 0, more);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += more[e];
+    }
+    const int64_t row_at = layout_row(p.at, row);
+    if (p.runs) {
+      if (p.type == Float::kF32) store_run<Float::kF32, 4>(p.out, row_at + layout_col(p.at, col), v);
+      else store_run<T, 4>(p.out, row_at + layout_col(p.at, col), v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) put_element(p.type, p.out, row_at + layout_col(p.at, col + e), v[e]);
+    }
+  }
+}
 
 // false: the general kernel takes it.
 bool launch_lhs_grad(const GatedBackwardArgs& a, const Sizes& s, hipStream_t stream, hipError_t* e) {
@@ -189,9 +243,37 @@ bool launch_lhs_grad(const GatedBackwardArgs& a, const Sizes& s, hipStream_t str
   p.lhs_second = s.pitch;  // (half of a row's bytes)
   p.depth = (uint32_t)s.cols;
   p.results = results_of(a, layout_of(a.lhs_grad_stride0, a.M0, a.K, a.K0), a.lhs_grad, nullptr, a.lhs_grad_stride0, 0, s.rows, a.M, false);
-  const int tile = choose_tile(kLhsGradTimes, s.rows, s.depth, 2 * ((s.cols + 31) / 32), 1);
-  if (tile < 0) return false;
-  *e = a.type == Float::kF16 ? launch_lhs_grad_f16(p, tile, stream) : launch_lhs_grad_bf16(p, tile, stream);
+  const Choice c = choose_lhs_grad(s);
+  if (c.tile < 0) return false;
+  const Layout at = p.results.at;
+  const bool f16 = a.type == Float::kF16;
+  if (c.splits > 1) {  // (the depth is a multiple of eight)
+    uint8_t* const parts = a.workspace + grads_bytes(s);
+    p.results.out[0] = parts;
+    p.results.at = layout_of(s.depth, 1, s.depth, 1);
+    p.results.stride0[0] = s.depth;
+    p.results.type = Float::kF32;
+    p.results.runs = 1;
+    p.results.apart = s.rows * s.depth * 4;
+    p.results.copies = (uint32_t)c.splits;
+  }
+  *e = f16 ? launch_lhs_grad_f16(p, c.tile, stream) : launch_lhs_grad_bf16(p, c.tile, stream);
+  if (c.splits == 1 || *e != hipSuccess) return true;
+  SumArgs g;
+  g.parts = (const float*)(a.workspace + grads_bytes(s));
+  g.out = a.lhs_grad;
+  g.at = at;
+  g.cols = (uint32_t)s.depth;
+  g.fours = g.cols / 4;
+  g.results = s.rows * g.fours;
+  g.apart = s.rows * s.depth;
+  g.splits = c.splits;
+  const int size = float_bytes(a.out_type);
+  g.runs = runs_of(at, a.lhs_grad, a.M, size, 4, 4 * size);
+  g.type = a.out_type;
+  const int64_t groups = (g.results + kThreads - 1) / kThreads;
+  *e = launch_kernel(f16 ? gated_lhs_grad_sums<Float::kF16> : gated_lhs_grad_sums<Float::kBf16>, (unsigned)(groups < (1 << 22) ? groups : 1 << 22),
+                     kThreads, 0, stream, g);
   return true;
 }
 bool launch_weight_grads(const GatedBackwardArgs& a, const Sizes& s, hipStream_t stream, hipError_t* e) {
@@ -207,9 +289,9 @@ bool launch_weight_grads(const GatedBackwardArgs& a, const Sizes& s, hipStream_t
   uint8_t* const second = a.gate_grad ? a.up_grad : nullptr;
   const int64_t stride0 = a.gate_grad ? a.gate_grad_stride0 : a.up_grad_stride0;
   p.results = results_of(a, layout_of(stride0, a.N0, a.K, a.K0), first, second, stride0, a.up_grad_stride0, s.cols, a.N, a.accumulate);
-  const int tile = choose_tile(kWeightGradTimes, s.cols, s.depth, (s.rows + 31) / 32, p.results.results);
-  if (tile < 0) return false;
-  *e = a.type == Float::kF16 ? launch_weight_grad_f16(p, tile, stream) : launch_weight_grad_bf16(p, tile, stream);
+  const Choice c = choose(kWeightGradTimes, s.cols, s.depth, (s.rows + 31) / 32, p.results.copies, 1);
+  if (c.tile < 0) return false;
+  *e = a.type == Float::kF16 ? launch_weight_grad_f16(p, c.tile, stream) : launch_weight_grad_bf16(p, c.tile, stream);
   return true;
 }
 
@@ -242,8 +324,13 @@ bool launch_first(const GatedBackwardArgs& a, const Sizes& s, hipStream_t stream
 int64_t gated_backward_workspace(const GatedBackwardArgs& a) {
   const Sizes s(a);
   int64_t bytes;
-  if (__builtin_mul_overflow(s.rows, 2 * s.pitch, &bytes) || bytes > INT64_MAX - 256) return -1;
-  return (bytes + 255) / 256 * 256;
+  if (__builtin_mul_overflow(s.rows, 2 * s.pitch, &bytes) || bytes > INT64_MAX - (1ll << 30)) return -1;
+  bytes = grads_bytes(s);
+  if (a.lhs_grad) {
+    const int splits = choose_lhs_grad(s).splits;
+    if (splits > 1) bytes += splits * s.rows * s.depth * 4;
+  }
+  return bytes;
 }
 
 hipError_t launch_gated_backward(const GatedBackwardArgs& a, hipStream_t stream, const char** name) {

@@ -7,8 +7,7 @@
 namespace uk {
 
 struct GatedResults {
-  static constexpr bool kPaired = true, kInTurn = false;
-  static constexpr int kResults = 1;
+  static constexpr bool kPaired = true, kInTurn = false, kCopies = false;
   uint8_t *out, *gate_pre, *up_pre;  // the latter two null: none
   Layout out_at, gate_at, up_at;
   Curve curve;

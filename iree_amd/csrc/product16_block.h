@@ -16,13 +16,15 @@
 // An epilogue E takes the accumulators, and says what the rhs is. E::kPaired: two matrices of the same layout side by side: of each 32
 // rows in LDS the first 16 are the first's, the others the second's of the same numbers, so that a lane has both products of a
 // column. E::kInTurn: two matrices one behind the other along K, the lhs's K being twice as long (its second half `lhs_second` bytes
-// behind its first).
+// behind its first). E::kCopies: the grid's rows of tiles come several times over, for another lhs and result (`lhs_second` behind the
+// first) or, in turn, for another part of K.
 #ifndef IREE_AMD_CSRC_PRODUCT16_BLOCK_H_
 #define IREE_AMD_CSRC_PRODUCT16_BLOCK_H_
 
 #include <type_traits>
 
 #include "product16.h"
+#include "product16_walk.h"
 
 namespace uk {
 
@@ -185,11 +187,11 @@ void product16_block_kernel(const BlockProduct<E, A, B> p) {
   if ((blockIdx.x >> 3) >= per_xcd || linear >= tiles) return;
   int tile_row, tile_col;
   tile_of_number(linear, p.tile_rows, p.tile_cols, p.band_reciprocal, &tile_row, &tile_col);
-  // (Tiles of an epilogue's second result come behind those of its first.)
-  uint32_t result = 0;
-  if constexpr (E::kResults > 1) {
-    result = (uint32_t)tile_row >= p.epilogue.tile_rows_of_first ? 1 : 0;
-    tile_row -= result * p.epilogue.tile_rows_of_first;
+  // (An epilogue's copies: a second result's tiles, or another part of K's, come behind those of the first.)
+  uint32_t copy = 0;
+  if constexpr (E::kCopies) {
+    copy = divide((uint32_t)tile_row, p.epilogue.tile_rows_of_copy, p.epilogue.tile_rows_reciprocal);
+    tile_row -= copy * p.epilogue.tile_rows_of_copy;
   }
   const uint32_t first_row = (uint32_t)tile_row * ROWS;
   const uint32_t first_col = (uint32_t)tile_col * RESULTS;
@@ -198,7 +200,7 @@ void product16_block_kernel(const BlockProduct<E, A, B> p) {
   const int wave_m = wave >> 1, wave_n = wave & 1;
 
   // Loads. Of a pair a load has sixteen rows of the first or of the second.
-  const uint8_t* lhs = first_of<AM>(p.lhs, p.lhs.data + (E::kResults > 1 ? result * p.lhs_second : 0), p.lhs.stride0, first_row);
+  const uint8_t* lhs = first_of<AM>(p.lhs, p.lhs.data + (E::kCopies && !IN_TURN ? copy * p.lhs_second : 0), p.lhs.stride0, first_row);
   const uint8_t* const lhs_first = lhs;
   const uint8_t* const rhs_first = first_of<BN>(p.rhs, p.rhs.data, p.rhs.stride0, first_col);
   const uint8_t* const rhs_second = PAIRED || IN_TURN ? first_of<BN>(p.rhs, p.second, p.second_stride0, first_col) : rhs_first;
@@ -229,23 +231,41 @@ void product16_block_kernel(const BlockProduct<E, A, B> p) {
   };
   // Behind the last chunk it is the last that is loaded again: no step is unlike the others.
   const uint32_t full = p.depth >> 5, rest = p.depth & 31;
-  const uint32_t by_registers = rest == 0 ? 0 : IN_TURN ? 2 : 1, chunks = (IN_TURN ? 2 : 1) * full + by_registers;
-  uint32_t loading = 1;
-  auto to_next_chunk = [&] {
-    if constexpr (IN_TURN) {
-      const bool turn = loading == full, more = loading++ < 2 * full;
-      lhs = turn ? lhs_first + p.lhs_second : lhs + (more ? lhs_step : 0);
-      rhs_even = turn ? rhs_second : rhs_even + (more ? rhs_step : 0);
-      if (turn) {
-        B other = p.rhs;
-        other.stride0 = p.second_stride0;
-        rhs_step = chunk_step(other);
+  uint32_t by_registers = rest == 0 ? 0 : 1;
+  ChunkWalk walk = {0, full, full};
+  if constexpr (IN_TURN) {
+    by_registers = copy == 0 ? 2 * by_registers : 0;
+    walk.at = first_of_split(2 * full, copy, p.epilogue.copies);
+    walk.end = first_of_split(2 * full, copy + 1, p.epilogue.copies);
+  }
+  const uint32_t chunks = walk.end - walk.at + by_registers;
+  // Of the second rhs offsets and steps are others where its stride is.
+  auto to_second = [&] {
+    B other = p.rhs;
+    other.stride0 = p.second_stride0;
+    rhs_step = chunk_step(other);
+    rhs_even = rhs_second;
 #pragma unroll
-        for (int i = 0; i < B_LOADS; ++i)
-          b_from[i] = offset_of<BN>(other, other.stride0, first_col, wave * B_LOADS + i, wave * B_LOADS + i, lane, p.depth);
-      }
+    for (int i = 0; i < B_LOADS; ++i)
+      b_from[i] = offset_of<BN>(other, other.stride0, first_col, wave * B_LOADS + i, wave * B_LOADS + i, lane, p.depth);
+    lhs = lhs_first + p.lhs_second;
+  };
+  if constexpr (IN_TURN) {
+    uint32_t skipped = walk.at;
+    if (walk.at != 0 && walk.at >= full) {
+      to_second();
+      skipped -= full;
+    }
+    lhs += skipped * lhs_step;
+    rhs_even += skipped * rhs_step;
+    rhs_odd = rhs_even;
+  }
+  auto to_next_chunk = [&] {
+    const ChunkWalk::Step step = walk.next();
+    if (IN_TURN && step == ChunkWalk::kSecondHalf) {
+      to_second();
     } else {
-      const bool more = loading++ < full;
+      const bool more = step != ChunkWalk::kStay;
       lhs += more ? lhs_step : 0;
       rhs_even += more ? rhs_step : 0;
       if constexpr (PAIRED && BN > 1) rhs_odd += more ? rhs_step : 0;
@@ -338,7 +358,7 @@ void product16_block_kernel(const BlockProduct<E, A, B> p) {
   for (int i = 0; i < AM; ++i)
 #pragma unroll
     for (int j = 0; j < BN; ++j) asm volatile("" : "+a"(acc[i][j]));
-  p.epilogue.template store<T, AM, BN>(acc, first_row + wave_m * 32 * AM, first_col + wave_n * (RESULTS / 2), p.lhs.rows, p.rhs.rows, lane, result);
+  p.epilogue.template store<T, AM, BN>(acc, first_row + wave_m * 32 * AM, first_col + wave_n * (RESULTS / 2), p.lhs.rows, p.rhs.rows, lane, copy);
   // (The last loads have reached LDS before it is given to another workgroup.)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
@@ -348,9 +368,10 @@ hipError_t launch_block_tile(BlockProduct<E, A, B> p, hipStream_t stream) {
   constexpr int RESULTS = E::kPaired ? 32 * BN : 64 * BN, LDS = block_lds_bytes(AM, BN, STAGES);
   static_assert(LDS <= 160 * 1024, "LDS");
   p.tile_rows = (p.lhs.rows + 64 * AM - 1) / (64 * AM);
-  if constexpr (E::kResults > 1) {
-    p.epilogue.tile_rows_of_first = p.tile_rows;
-    p.tile_rows *= p.epilogue.results;
+  if constexpr (E::kCopies) {
+    p.epilogue.tile_rows_of_copy = p.tile_rows;
+    p.epilogue.tile_rows_reciprocal = reciprocal_of(p.tile_rows);
+    p.tile_rows *= p.epilogue.copies;
   }
   p.tile_cols = (p.rhs.rows + RESULTS - 1) / RESULTS;
   p.band_reciprocal = band_reciprocal(p.tile_cols);

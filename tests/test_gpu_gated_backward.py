@@ -64,6 +64,17 @@ def test_activations_types_and_accumulation(gpu_lib, m, n, k, tile, type, activa
     check_case(gpu_lib, m, n, k, tile, type, type if out == "same" else out, pre_type, activation, accumulate)
 
 
+# Few rows and a long K of lhs_grad (the gate's and up's rows): it is split, and its parts added.
+SPLIT = [(1, 2080, 64, (1, 16, 16)), (17, 1200, 264, (1, 16, 8)), (40, 4096, 128, (1, 1, 8)), (64, 3001, 200, (16, 16, 16)),
+         (100, 2048, 512, (4, 8, 8)), (130, 5000, 72, (1, 32, 24))]
+
+
+@pytest.mark.parametrize("type,out,accumulate", [("bf16", "bf16", False), ("f16", "f32", True)])
+@pytest.mark.parametrize("m,n,k,tile", SPLIT)
+def test_split_sums(gpu_lib, m, n, k, tile, type, out, accumulate):  # noqa: F811
+    check_case(gpu_lib, m, n, k, tile, type, out, type, "silu", accumulate, which="l" if n == 4096 else "lgu")
+
+
 @pytest.mark.parametrize("which", ["l", "g", "u", "gu", "lu"])
 @pytest.mark.parametrize("m,n,k,tile", [PROBLEMS[i] for i in (7, 9, 12)])
 def test_some_of_the_gradients(gpu_lib, m, n, k, tile, which):  # noqa: F811
