@@ -153,12 +153,13 @@ GradResults results_of(const GatedBackwardArgs& a, const Layout& at, uint8_t* fi
 
 // Which tile, and how many parts K is split into: the least of the times that a model gives, in microseconds: a start, and chunks of K
 // times what one of them takes with one workgroup on a compute unit and, where LDS and registers hold two, with two; more than that
-// follow each other. Fitted to the times of every tile in 260 problems from 16 to 4096 rows, 64 to 28672 columns, K of 64 to 14336; over
-// these the tile taken is slower than the best one by 0.6 % (lhs) and 1.6 % (weights) in the mean. lhs_grad's K is both weights' rows
-// and its results few where the rows are: 19 x 18592 x 448 takes 25.7 us in 28 parts and 188 in one, 100 x 12176 x 3504 45 and 125, 508
-// x 9526 x 325 33 and 105. Over 120 problems of 1 to 4096 rows timed with every tile and ten numbers of parts, what is taken is slower
-// than the best by 2.2 % in the mean. tile -1: none can.
-struct Times { float start, one, two, start_again; };  // two = 0: one workgroup on a compute unit
+// follow each other. With all compute units busy, clocks and memory hold a chunk to `busy` for each 256 workgroups at least. Fitted to
+// the times of every tile in 260 problems from 16 to 4096 rows, 64 to 28672 columns, K of 64 to 14336, and, for lhs_grad, of every tile
+// with up to ten numbers of parts in 120 of 1 to 4096 rows; over these what is taken is slower than the best by 0.7 % (lhs) and 1.3 %
+// (weights) in the mean. lhs_grad's K is both weights' rows, and its results are few where the rows are: 19 x 18592 x 448 takes 25.7 us
+// in 28 parts and 188 in one, 100 x 12176 x 3504 45 and 125, 508 x 9526 x 325 33 and 105, 2048 x 8192 x 4096 245 in two and 283 in one
+// (of smaller tiles). tile -1: none can.
+struct Times { float start, one, two, start_again, busy; };  // two = 0: one workgroup on a compute unit
 struct Choice { int tile, splits; };
 Choice choose(const Times* times, int64_t rows, int64_t cols, int64_t chunks, int64_t copies, int64_t most_splits) {
   Choice best = {-1, 1};
@@ -172,7 +173,8 @@ Choice choose(const Times* times, int64_t rows, int64_t cols, int64_t chunks, in
       if (tiles > (1 << 23)) continue;  // (a grid has fewer than 2^32 threads)
       // (The parts of sums are written and read, in a launch more.)
       const float parts = splits == 1 ? 0 : 2 + (float)splits * (float)(rows * cols) * 1.5e-6f;
-      const float steps = (float)chunks / (float)splits * (of.two == 0 ? rounds * of.one : (rounds >> 1) * of.two + (rounds & 1) * of.one);
+      const float in_turn = (float)chunks / (float)splits * (of.two == 0 ? rounds * of.one : (rounds >> 1) * of.two + (rounds & 1) * of.one);
+      const float busy = (float)of_one * (float)chunks / 256 * of.busy, steps = in_turn > busy ? in_turn : busy;
       const float cost = of.start + (rounds - 1) * of.start_again + steps + parts;
       if (best.tile < 0 || cost < least) {
         least = cost;
@@ -182,10 +184,12 @@ Choice choose(const Times* times, int64_t rows, int64_t cols, int64_t chunks, in
   }
   return best;
 }
-constexpr Times kLhsGradTimes[] = {{16.2f, .491f, 0, 21.5f},   {11.3f, .299f, 0, 11.7f},  {11.4f, .334f, .834f, 4.3f}, {9.1f, .220f, .555f, 2.3f},
-                                   {7.7f, .157f, .418f, 1.1f}, {7.6f, .159f, .361f, 1.3f}, {6.6f, .137f, .246f, .9f}};
-constexpr Times kWeightGradTimes[] = {{17.3f, .522f, 0, 15.6f},   {11.9f, .323f, 0, 8.5f},   {11.6f, .303f, .747f, 4.1f}, {8.8f, .196f, .448f, 2.4f},
-                                      {7.4f, .171f, .303f, 1.6f}, {7.3f, .164f, .313f, 1.6f}, {6.3f, .141f, .210f, 1.1f}};
+constexpr Times kLhsGradTimes[] = {{16.2f, .491f, 0, 21.5f, .45f},   {11.3f, .299f, 0, 11.7f, .66f},   {11.4f, .334f, .834f, 4.3f, .53f},
+                                   {9.1f, .220f, .555f, 2.3f, .24f}, {7.7f, .157f, .418f, 1.1f, .29f}, {7.6f, .159f, .361f, 1.3f, .17f},
+                                   {6.6f, .137f, .246f, .9f, .13f}};
+constexpr Times kWeightGradTimes[] = {{17.3f, .522f, 0, 15.6f, .92f},   {11.9f, .323f, 0, 8.5f, .57f},    {11.6f, .303f, .747f, 4.1f, .49f},
+                                      {8.8f, .196f, .448f, 2.4f, .27f}, {7.4f, .171f, .303f, 1.6f, .10f}, {7.3f, .164f, .313f, 1.6f, .17f},
+                                      {6.3f, .141f, .210f, 1.1f, .12f}};
 
 // lhs_grad's. A split has sixteen chunks at least, and all of them 64 MiB of sums at most.
 Choice choose_lhs_grad(const Sizes& s) {

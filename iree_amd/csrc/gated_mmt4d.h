@@ -148,9 +148,10 @@ struct GatedTile {
   int rows, cols;
   const char* name;
 };
-constexpr GatedTile kGatedTiles[] = {{256, 128, "gated_mmt4d_256x128"}, {192, 128, "gated_mmt4d_192x128"}, {128, 128, "gated_mmt4d_128x128"},
-                                     {128, 96, "gated_mmt4d_128x96"},   {128, 64, "gated_mmt4d_128x64"},   {64, 128, "gated_mmt4d_64x128"},
-                                     {64, 96, "gated_mmt4d_64x96"},     {64, 64, "gated_mmt4d_64x64"},     {64, 32, "gated_mmt4d_64x32"}};
+constexpr GatedTile kGatedTiles[] = {{256, 128, "gated_mmt4d_256x128"}, {256, 96, "gated_mmt4d_256x96"},   {192, 96, "gated_mmt4d_192x96"},
+                                     {192, 128, "gated_mmt4d_192x128"}, {128, 128, "gated_mmt4d_128x128"}, {128, 96, "gated_mmt4d_128x96"},
+                                     {128, 64, "gated_mmt4d_128x64"},   {64, 128, "gated_mmt4d_64x128"},   {64, 96, "gated_mmt4d_64x96"},
+                                     {64, 64, "gated_mmt4d_64x64"},     {64, 32, "gated_mmt4d_64x32"}};
 // The kernels for few rows (gated_mmt4d_few.hip): fragments of 16 rows and of 16 results a row that a workgroup multiplies, and
 // whether the lhs goes through LDS.
 struct GatedFewShape {

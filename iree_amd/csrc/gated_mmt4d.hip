@@ -111,9 +111,10 @@ struct Choice {
 };
 Choice choose(const GatedProduct& p) {
   struct Times { float start, one, two, start_again, memory; };  // two = 0: one workgroup on a compute unit; memory: TB/s
-  static const Times kTimes[] = {{11.8f, .499f, 0, 19.9f, 4.14f},    {9.8f, .409f, 0, 15.3f, 5.56f},   {7.3f, .325f, .888f, 3.4f, 5.47f},
-                                 {6.2f, .265f, .725f, 2.4f, 6.17f},  {5.0f, .208f, .555f, 1.7f, 6.81f}, {5.2f, .254f, .613f, 1.8f, 6.93f},
-                                 {4.5f, .200f, .480f, 1.5f, 7.11f},  {3.9f, .150f, .360f, 1.1f, 7.72f}, {3.1f, .124f, .229f, .8f, 8.12f}};
+  static const Times kTimes[] = {{11.8f, .499f, 0, 19.9f, 4.14f},   {9.4f, .412f, 0, 14.1f, 4.81f},    {7.8f, .345f, 0, 11.3f, 5.75f},
+                                 {9.8f, .409f, 0, 15.3f, 5.56f},    {7.3f, .325f, .888f, 3.4f, 5.47f}, {6.2f, .265f, .725f, 2.4f, 6.17f},
+                                 {5.0f, .208f, .555f, 1.7f, 6.81f}, {5.2f, .254f, .613f, 1.8f, 6.93f}, {4.5f, .200f, .480f, 1.5f, 7.11f},
+                                 {3.9f, .150f, .360f, 1.1f, 7.72f}, {3.1f, .124f, .229f, .8f, 8.12f}};
   static_assert(sizeof kTimes / sizeof kTimes[0] == sizeof kGatedTiles / sizeof kGatedTiles[0], "one for each tile");
   const int64_t rows = p.lhs.rows, cols = p.gate.rows;
   const float chunks = (float)((p.depth + 31) / 32), bytes = (float)cols * chunks * 128e-6f;  // of the weights, MB

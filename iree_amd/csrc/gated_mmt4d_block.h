@@ -24,14 +24,16 @@ hipError_t launch_gated_block(const GatedProduct& g, int tile, hipStream_t strea
   const bool stream_rhs = g.lhs.rows <= 128 && 4 * (int64_t)g.gate.rows * g.depth > (256ll << 20);
   switch (tile) {  // kGatedTiles
     case 0: return launch_block_tile<T, 4, 4, 4>(p, stream);
-    case 1: return launch_block_tile<T, 3, 4, 4>(p, stream);
-    case 2: return launch_block_tile<T, 2, 4, 3>(p, stream);
-    case 3: return launch_block_tile<T, 2, 3, 4>(p, stream);
-    case 4: return stream_rhs ? launch_block_tile<T, 2, 2, 5, true>(p, stream) : launch_block_tile<T, 2, 2, 5>(p, stream);
-    case 5: return stream_rhs ? launch_block_tile<T, 1, 4, 4, true>(p, stream) : launch_block_tile<T, 1, 4, 4>(p, stream);
-    case 6: return stream_rhs ? launch_block_tile<T, 1, 3, 5, true>(p, stream) : launch_block_tile<T, 1, 3, 5>(p, stream);
-    case 7: return stream_rhs ? launch_block_tile<T, 1, 2, 6, true>(p, stream) : launch_block_tile<T, 1, 2, 6>(p, stream);
-    case 8: return stream_rhs ? launch_block_tile<T, 1, 1, 8, true>(p, stream) : launch_block_tile<T, 1, 1, 8>(p, stream);
+    case 1: return launch_block_tile<T, 4, 3, 4>(p, stream);
+    case 2: return launch_block_tile<T, 3, 3, 4>(p, stream);
+    case 3: return launch_block_tile<T, 3, 4, 4>(p, stream);
+    case 4: return launch_block_tile<T, 2, 4, 3>(p, stream);
+    case 5: return launch_block_tile<T, 2, 3, 4>(p, stream);
+    case 6: return stream_rhs ? launch_block_tile<T, 2, 2, 5, true>(p, stream) : launch_block_tile<T, 2, 2, 5>(p, stream);
+    case 7: return stream_rhs ? launch_block_tile<T, 1, 4, 4, true>(p, stream) : launch_block_tile<T, 1, 4, 4>(p, stream);
+    case 8: return stream_rhs ? launch_block_tile<T, 1, 3, 5, true>(p, stream) : launch_block_tile<T, 1, 3, 5>(p, stream);
+    case 9: return stream_rhs ? launch_block_tile<T, 1, 2, 6, true>(p, stream) : launch_block_tile<T, 1, 2, 6>(p, stream);
+    case 10: return stream_rhs ? launch_block_tile<T, 1, 1, 8, true>(p, stream) : launch_block_tile<T, 1, 1, 8>(p, stream);
   }
   return hipErrorInvalidValue;
 }
