@@ -15,6 +15,7 @@ struct Operand16 {
   int64_t stride0;  // bytes from a panel to the next
   uint32_t rows, tile_rows, tile_reciprocal;
   uint32_t row_bytes, piece1, piece2;
+  uint32_t log2_pieces;  // of a chunk's pieces of a row lie next to each other: 4, 2 or 1
 };
 
 // An operand whose rows' values of one k lie next to each other: element (k, row) in panel k / tile_rows, row_bytes apart within it, and
@@ -56,6 +57,7 @@ inline bool as_operand16(const uint8_t* data, int64_t stride0, int64_t panels, i
   o->row_bytes = m0 == 1 ? 0 : 2 * k0;
   o->piece1 = k0 == 8 ? 16 * m0 : 16;
   o->piece2 = k0 == 32 ? 32 : 32 * m0;
+  o->log2_pieces = k0 == 32 ? 2 : k0 == 16 ? 1 : 0;
   return true;
 }
 // The same matrix [panels][K][M0][K0] with its first dimension contracted. (32 of its rows within 31 bits of each other.)

@@ -4,9 +4,10 @@
 // fragments of v_mfma_f32_32x32x16. K goes by in chunks of 32 values, which travel global memory -> LDS without passing through
 // registers into a ring of STAGES stages.
 //
-// An operand is of one of two kinds. Operand16: a row's K is contiguous, 64 bytes a chunk. LDS holds a chunk's rows one after the
-// other, a row's 16-byte pieces exchanged among themselves so that the lanes that a read serves together find theirs in different
-// banks. Strided16: the rows' values of one k are contiguous. LDS holds a chunk's 32 ks one after the other, 128 bytes for each 64
+// An operand is of one of two kinds. Operand16: a row's K comes in pieces of 16 bytes, four a chunk. LDS holds a chunk's rows sixteen
+// by sixteen: one after the other where a row's pieces lie next to each other, these exchanged among themselves so that the lanes that a
+// read serves together find theirs in different banks; else as the tiles have them, two pieces of sixteen rows and the two others, or
+// a piece of each and then the next, which is no read's conflict. Strided16: the rows' values of one k are contiguous. LDS holds a chunk's 32 ks one after the other, 128 bytes for each 64
 // rows, and the transposing read hands a lane four ks of its row: sixteen lanes read 32 bytes of each of four ks, which lie in
 // different banks because a k's 32-byte units are exchanged among themselves. Loads write LDS in lane order, so it is the global
 // address of a lane that is chosen; neighbouring lanes still read neighbouring pieces.
@@ -81,7 +82,7 @@ __device__ __forceinline__ void each_of(F f) {
   each_between<0, N>(f);
 }
 
-// A row's piece `c` lies at piece c ^ exchanged(row).
+// Where four pieces of a row lie next to each other, piece `c` lies at c ^ exchanged(row) in LDS.
 __device__ __forceinline__ uint32_t exchanged(uint32_t row) { return ((row >> 2) & 3) ^ (row & 2); }
 
 // One side of a tile: 64 W rows from `first` on, loaded 16 bytes a lane, W loads a wavefront for a chunk. `number` of a load: 0 to 4 W -
@@ -90,15 +91,22 @@ template <int W>
 __device__ __forceinline__ const uint8_t* first_of(const Operand16& o, const uint8_t* data, int64_t stride0, uint32_t first) {
   return uniform_pointer(data + (int64_t)divide(first, o.tile_rows, o.tile_reciprocal) * stride0);
 }
-template <int W>
-__device__ __forceinline__ uint32_t piece_of(const Operand16&, uint32_t number, int lane) {
-  return (lane % 4) ^ exchanged(number * 16 + lane / 4);
+// Which of the sixteen rows and which piece of it a lane loads: neighbouring lanes have neighbouring pieces.
+__device__ __forceinline__ uint32_t row_of_lane(const Operand16& o, int lane) { return (lane >> o.log2_pieces) & 15; }
+__device__ __forceinline__ uint32_t piece_of_lane(const Operand16& o, int lane) {
+  const uint32_t next = lane & ((1u << o.log2_pieces) - 1);
+  return o.log2_pieces == 2 ? next ^ exchanged(lane >> 2) : next + ((uint32_t)lane >> (4 + o.log2_pieces) << o.log2_pieces);
 }
+// Where in LDS that is, of sixteen rows: row r's piece g, g < 2; two pieces further on it is at at ^ of_next_step().
+__device__ __forceinline__ uint32_t place_of(const Operand16& o, uint32_t r, uint32_t g) {
+  return o.log2_pieces == 2 ? r * 64 + 16 * (g ^ exchanged(r)) : o.log2_pieces == 1 ? r * 32 + 16 * g : g * 256 + 16 * r;
+}
+__device__ __forceinline__ uint32_t of_next_step(const Operand16& o) { return o.log2_pieces == 2 ? 32 : 512; }
 // A lane's offset from there. Rows behind the last are read as the last.
 template <int W>
-__device__ __forceinline__ uint32_t offset_of(const Operand16& o, int64_t stride0, uint32_t first, uint32_t number, uint32_t row_number,
+__device__ __forceinline__ uint32_t offset_of(const Operand16& o, int64_t stride0, uint32_t first, uint32_t, uint32_t row_number,
                                               int lane, uint32_t depth) {
-  uint32_t row = first + row_number * 16 + lane / 4, piece = piece_of<W>(o, number, lane);
+  uint32_t row = first + row_number * 16 + row_of_lane(o, lane), piece = piece_of_lane(o, lane);
   row = row < o.rows ? row : o.rows - 1;
   if (8 * piece >= depth) piece = 0;  // (less than a chunk of K: it is loaded for nothing, and only what is there)
   const uint32_t panel = divide(row, o.tile_rows, o.tile_reciprocal), first_panel = divide(first, o.tile_rows, o.tile_reciprocal);
@@ -107,8 +115,8 @@ __device__ __forceinline__ uint32_t offset_of(const Operand16& o, int64_t stride
 }
 // The lane's piece of what K has behind `full` whole chunks, `rest` values.
 template <int W>
-__device__ __forceinline__ uint4 rest_of(const Operand16& o, const uint8_t* at, uint32_t number, int lane, uint32_t rest) {
-  return last_piece(at, (int)rest - 8 * (int)piece_of<W>(o, number, lane));
+__device__ __forceinline__ uint4 rest_of(const Operand16& o, const uint8_t* at, uint32_t, int lane, uint32_t rest) {
+  return last_piece(at, (int)rest - 8 * (int)piece_of_lane(o, lane));
 }
 __device__ __forceinline__ int64_t chunk_step(const Operand16& o) { return 64 * (int64_t)o.tile_rows; }
 
@@ -142,9 +150,9 @@ __device__ __forceinline__ int64_t chunk_step(const Strided16& o) { return o.str
 // first one is in a chunk, `half`: the wavefront's of two.
 template <typename O> constexpr int kReads = std::is_same<O, Strided16>::value ? 2 : 1;
 template <int W>
-__device__ __forceinline__ uint32_t read_at(const Operand16&, int half, int lane) {
+__device__ __forceinline__ uint32_t read_at(const Operand16& o, int half, int lane) {
   const int r = lane & 31, g = lane >> 5;
-  return (half * 32 * W + r) * 64 + 16 * (g ^ exchanged(r));
+  return half * 2048 * W + (r >> 4) * 1024 + place_of(o, r & 15, g);
 }
 template <int W>
 __device__ __forceinline__ uint32_t read_at(const Strided16&, int half, int lane) {
@@ -153,8 +161,8 @@ __device__ __forceinline__ uint32_t read_at(const Strided16&, int half, int lane
 }
 // Read H of fragment F in step S.
 template <int W, int F, int S, int H>
-__device__ __forceinline__ void read_piece(const Operand16&, const uint8_t* side, uint32_t at, uint4& to) {
-  to = *(const uint4*)(side + F * 2048 + (at ^ (32 * S)));
+__device__ __forceinline__ void read_piece(const Operand16& o, const uint8_t* side, uint32_t at, uint4& to) {
+  to = *(const uint4*)(side + F * 2048 + (S == 0 ? at : at ^ of_next_step(o)));
 }
 template <int W, int F, int S, int H>
 __device__ __forceinline__ void read_piece(const Strided16&, const uint8_t* side, uint32_t at, uint4& to) {
