@@ -57,7 +57,7 @@ PROBLEMS = [
     (777, 544, 328, 64, 11, (1, 16, 32), "runs"), (600, 100, 200, 16, 40, (1, 16, 16), "mixed"), (40, 50, 70, 5, 4, (5, 7, 6), "mixed"),
     (9, 30, 500, 300, 3, (3, 5, 16), "all"), (20, 20, 1030, 2, 5, (2, 4, 24), "runs"), (12, 31, 7, 3, 2, (1, 1, 1), "mixed"),
     (90, 257, 2056, 16, 5, (1, 1, 2056), "mixed"), (33, 64, 128, 256, 4, (1, 16, 16), "runs"), (48, 100, 64, 20, 2, (1, 4, 16), "one"),
-    (530, 48, 40, 12, 3, (1, 16, 8), "runs"),
+    (530, 48, 40, 12, 3, (1, 16, 8), "runs"), (70, 90, 300, 45, 5, (1, 16, 16), "mixed"), (33, 100, 200, 64, 4, (1, 4, 16), "runs"),
 ]
 
 
