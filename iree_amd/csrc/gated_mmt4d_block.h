@@ -18,10 +18,11 @@ hipError_t launch_gated_block(const GatedProduct& g, int tile, hipStream_t strea
   p.lhs_second = 0;
   p.depth = g.depth;
   p.epilogue = g.results;
-  // Weights that no cache holds and that a tile or two of rows read once go past the caches: 64 rows x 28672 x 8192 (940 MB) 165 -> 148
-  // us in 64x128 tiles. (From 235 MB, 64 x 14336 x 4096, in 64x64 ones: 47.7 -> 44.9 us where other calls have filled the caches in
-  // between, but 35.5 -> 43.2 where they hold them.)
-  const bool stream_rhs = g.lhs.rows <= 128 && 4 * (int64_t)g.gate.rows * g.depth > (256ll << 20);
+  // Weights that a tile or two of rows read once go past the caches where the layer's three matrices (the third is as large as one of
+  // these) do not fit them, 256 MiB, and so are gone when the next token comes. 64 rows x 28672 x 8192, 940 MB, 165 -> 148 us in 64x128
+  // tiles; where other calls have filled the caches in between, 40 x 11008 x 4096 (180 MB) 38.1 -> 35.1, 64 x 14336 x 4096 47.1 -> 43.4 and
+  // 128 x 11008 x 4096 53.2 -> 50.2. The same call made again at once finds its weights there: 29 -> 35, 36 -> 43 and 33 -> 49.
+  const bool stream_rhs = g.lhs.rows <= 128 && 6 * (int64_t)g.gate.rows * g.depth > (256ll << 20);
   switch (tile) {  // kGatedTiles
     case 0: return launch_block_tile<T, 4, 4, 4>(p, stream);
     case 1: return launch_block_tile<T, 4, 3, 4>(p, stream);

@@ -79,9 +79,9 @@ def test_split_sums_are_tested(recorder):  # noqa: F811
         assert backward(recorder, m, n, k, tile, "l") == (0, 0), (m, n, k, tile)
 
 
-# From a large product on, weights that a tile or two of rows read go past the caches.
-@pytest.mark.parametrize("m,n,k,streams", [(1, 14336, 4096, False), (1, 28672, 8192, True), (64, 14336, 4096, False), (64, 28672, 8192, True),
-                                           (129, 28672, 8192, False)])
+# Large weights that few rows read go past the caches.
+@pytest.mark.parametrize("m,n,k,streams", [(1, 14336, 4096, True), (1, 2048, 2048, False), (1, 28672, 8192, True), (64, 14336, 4096, True), (64, 28672, 8192, True),
+                                           (100, 4100, 4096, False), (40, 11008, 4096, True), (129, 28672, 8192, False)])
 def test_weights_past_the_caches(recorder, m, n, k, streams):  # noqa: F811
     kernel, _ = gated(recorder, m, n, k, (1, 16, 16))
     past = re.search(r"few_kernelILNS_5FloatE\dELi\dELi\dELb(\d)|block_kernelILNS_5FloatE\dELi\dELi\dELi\dELb(\d)", kernel)
