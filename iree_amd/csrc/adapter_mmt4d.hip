@@ -73,7 +73,6 @@ hipError_t launch_over(void (*f16)(const AdapterKernelArgs), void (*bf16)(const 
 // rows, and a workgroup takes every SLOTS-th of them. A row has one adapter, so nobody else writes its results; what the matrix
 // instructions compute of the other rows is thrown away, and what is not finite there stays there.
 
-constexpr int kWaves = 8;      // of a workgroup that multiplies by `down`
 constexpr int kFragments = 4;  // of 16 columns that a wavefront multiplies by `up`, and of 16 ranks by `down`, at most
 
 struct AdapterProduct {
@@ -117,14 +116,32 @@ __device__ __forceinline__ uint32_t of_adapters(const AdapterProduct& p, uint32_
   return ~with & 0xFFFF;
 }
 
+extern __shared__ uint4 staged[];
+
+// 64 x 16 bytes to LDS byte offset `lds` (of the wavefront), unseen by the compiler.
+__device__ __forceinline__ void load_pieces(uint32_t lds, const uint8_t* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+}
+
+// Wavefronts of a workgroup that multiplies by `down`, and its LDS: 4 KB a wavefront for the lhs and for each 16 ranks.
+template <int RT> constexpr int kWaves = RT > 2 ? 4 : 8;
+template <int RT> constexpr int kDownLds = kWaves<RT> * (1 + RT) * 4096;
+
 // Sums of 16 rows with 16 * RT ranks over a split's part of K, which the wavefronts share four chunks of 32 at a time; they meet in
 // LDS, in the order of the wavefronts' numbers.
+//
+// A wavefront loads four chunks of sixteen rows, of the lhs and of `down`, into a part of LDS of its own, four rows a load: sixteen
+// lanes have 256 bytes of a row. (Straight into registers neighbouring lanes have different rows.) A row's piece c of 16 bytes lies at
+// c ^ r, for the banks' sake.
 template <Float T, int RT>
-__global__ __launch_bounds__(64 * kWaves) void adapter_down_kernel(const AdapterProduct p) {
-  __shared__ p16_v4f32 partial[kWaves][RT][64];
+__global__ __launch_bounds__(64 * kWaves<RT>) void adapter_down_kernel(const AdapterProduct p) {
+  constexpr int WAVES = kWaves<RT>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
   const uint32_t full = p.depth >> 5, rest = p.depth & 31;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)staged + wave * ((1 + RT) * 4096);
+  const uint8_t* const own = (const uint8_t*)staged + wave * ((1 + RT) * 4096) + r * 256;
+  p16_v4f32* const partial = (p16_v4f32*)staged;  // [WAVES][RT][64]
   for (uint32_t unit = blockIdx.x; unit < p.units; unit += gridDim.x) {
     // unit = (tile * slots + slot) * parts + (block of ranks * splits + split)
     const uint32_t upper = divide(unit, p.parts, p.parts_reciprocal), part = unit - upper * p.parts;
@@ -134,60 +151,54 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_down_kernel(const Adapter
     // (Splits begin with whole fours.)
     const uint32_t fours = (full + 3) / 4;
     const uint32_t from = (uint32_t)((uint64_t)fours * split / p.splits), to = (uint32_t)((uint64_t)fours * (split + 1) / p.splits);
-    const uint32_t row = first + r < p.lhs.rows ? first + r : p.lhs.rows - 1;
-    const uint32_t panel = divide(row, p.lhs.tile_rows, p.lhs.tile_reciprocal);
-    const uint8_t* const lhs = p.lhs.data + (int64_t)panel * p.lhs.stride0 + (row - panel * p.lhs.tile_rows) * p.lhs.row_bytes +
-                               (g & 1) * p.lhs.piece1 + (g >> 1) * p.lhs.piece2;
+    auto lhs_row = [&](uint32_t row) {
+      row = row < p.lhs.rows ? row : p.lhs.rows - 1;
+      const uint32_t panel = divide(row, p.lhs.tile_rows, p.lhs.tile_reciprocal);
+      return p.lhs.data + (int64_t)panel * p.lhs.stride0 + (row - panel * p.lhs.tile_rows) * p.lhs.row_bytes;
+    };
     const int64_t lhs_step = 64 * (int64_t)p.lhs.tile_rows;
     of_adapters(p, first, slot, lane, [&](uint32_t of, uint32_t same) {
-      const uint8_t* down[RT];
-#pragma unroll
-      for (int j = 0; j < RT; ++j) {
-        const uint32_t rank = first_rank + 16 * j + r;
-        down[j] = p.down + of * p.down_stride0 + (int64_t)(rank < p.rank ? rank : p.rank - 1) * p.down_stride1 + 16 * g;
-      }
+      auto down_row = [&](uint32_t rank) {
+        return p.down + of * p.down_stride0 + (int64_t)(rank < p.rank ? rank : p.rank - 1) * p.down_stride1;
+      };
       p16_v4f32 acc[RT] = {};
-      uint4 a[4], b[4][RT];
-      auto load = [&](int u, uint32_t four) {
-        const uint32_t chunk = 4 * four + u < full ? 4 * four + u : full - 1;
-        a[u] = *(const uint4*)(lhs + chunk * lhs_step);
+      for (uint32_t four = from + wave; four < to; four += WAVES) {
 #pragma unroll
-        for (int j = 0; j < RT; ++j) b[u][j] = *(const uint4*)(down[j] + (int64_t)chunk * 64);
-      };
-      auto multiply = [&](int u) {
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t of_sixteen = 4 * i + g, piece = (uint32_t)r ^ of_sixteen;
+          const uint32_t chunk = 4 * four + (piece >> 2) < full ? 4 * four + (piece >> 2) : full - 1;
+          load_pieces(lds0 + i * 1024, lhs_row(first + of_sixteen) + chunk * lhs_step + (piece & 1) * p.lhs.piece1 + (piece >> 1 & 1) * p.lhs.piece2);
 #pragma unroll
-        for (int j = 0; j < RT; ++j) acc[j] = mfma16_16<T>(b[u][j], a[u], acc[j]);
-      };
-      uint32_t four = from + wave;
-      if (four < to) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) load(u, four);
-        for (; four + kWaves < to; four += kWaves) {
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            multiply(u);
-            load(u, four + kWaves);
-          }
+          for (int j = 0; j < RT; ++j)
+            load_pieces(lds0 + (1 + j) * 4096 + i * 1024, down_row(first_rank + 16 * j + of_sixteen) + (int64_t)chunk * 64 + (piece & 3) * 16);
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (4 * four + u < full) multiply(u);
+        for (int u = 0; u < 4; ++u) {
+          if (4 * four + u >= full) continue;
+          const uint32_t at = 16 * ((4 * u + g) ^ r);
+          const uint4 a = *(const uint4*)(own + at);
+#pragma unroll
+          for (int j = 0; j < RT; ++j) acc[j] = mfma16_16<T>(*(const uint4*)(own + (1 + j) * 4096 + at), a, acc[j]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (before its place is loaded again)
       }
       // What K has behind its last whole chunk, zeros behind it.
-      if (rest != 0 && split == p.splits - 1 && wave == (int)((to - from) % kWaves)) {
+      if (rest != 0 && split == p.splits - 1 && wave == (int)((to - from) % WAVES)) {
         const int exist = (int)rest - 8 * g;
-        a[0] = last_piece(lhs + full * lhs_step, exist);
+        const uint4 a = last_piece(lhs_row(first + r) + full * lhs_step + (g & 1) * p.lhs.piece1 + (g >> 1) * p.lhs.piece2, exist);
 #pragma unroll
-        for (int j = 0; j < RT; ++j) b[0][j] = last_piece(down[j] + (int64_t)full * 64, exist);
-        multiply(0);
+        for (int j = 0; j < RT; ++j)
+          acc[j] = mfma16_16<T>(last_piece(down_row(first_rank + 16 * j + r) + (int64_t)full * 64 + 16 * g, exist), a, acc[j]);
       }
-#pragma unroll
-      for (int j = 0; j < RT; ++j) partial[wave][j][lane] = acc[j];
       __syncthreads();
-      for (int j = wave; j < RT; j += kWaves) {
-        p16_v4f32 v = partial[0][j][lane];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) v += partial[w][j][lane];
+      for (int j = 0; j < RT; ++j) partial[(wave * RT + j) * 64 + lane] = acc[j];
+      __syncthreads();
+      for (int j = wave; j < RT; j += WAVES) {
+        p16_v4f32 v = partial[j * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v += partial[(w * RT + j) * 64 + lane];
         const uint32_t rank = first_rank + 16 * j + 4 * g;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = rank + e < p.rank ? v[e] : 0;  // (ranks behind the last meet zeros, and are finite)
@@ -432,8 +443,9 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterProduct p)
 
 // How many parts K is split into: as many as leave every wavefront four chunks, while there are fewer workgroups than compute units.
 uint32_t splits_of(int64_t rows, int64_t depth, int64_t rank) {
+  const int waves = rank > 32 ? kWaves<kFragments> : kWaves<1>;
   const int64_t tiles = (rows + 15) / 16 * ((rank + 16 * kFragments - 1) / (16 * kFragments));
-  const int64_t most = depth / 32 / (4 * kWaves), wanted = (256 + tiles - 1) / tiles;
+  const int64_t most = depth / 32 / (4 * waves), wanted = (256 + tiles - 1) / tiles;
   const int64_t s = most < wanted ? most : wanted;
   return (uint32_t)(s < 1 ? 1 : s);
 }
@@ -485,28 +497,36 @@ bool as_product(const AdapterArgs& a, AdapterProduct* p) {
 }
 
 // One launch over tiles * slots * parts pieces of work.
-hipError_t launch_units(void (*kernel)(const AdapterProduct), AdapterProduct p, int64_t parts, unsigned threads, hipStream_t stream) {
+hipError_t launch_units(void (*kernel)(const AdapterProduct), AdapterProduct p, int64_t parts, unsigned threads, unsigned lds, hipStream_t stream) {
   const int64_t tiles = ((int64_t)p.lhs.rows + 15) / 16;
   p.parts = (uint32_t)parts;
   p.parts_reciprocal = reciprocal_of(p.parts);
   p.units = (uint32_t)(tiles * p.slots * parts);
-  return launch_kernel(kernel, p.units < (1u << 22) ? p.units : 1u << 22, threads, 0, stream, p);
+  return launch_kernel(kernel, p.units < (1u << 22) ? p.units : 1u << 22, threads, lds, stream, p);
 }
 
+template <Float T, int RT>
+hipError_t launch_down_of(const AdapterProduct& p, int64_t parts, hipStream_t stream) {
+  if (kDownLds<RT> > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)adapter_down_kernel<T, RT>, hipFuncAttributeMaxDynamicSharedMemorySize, kDownLds<RT>);
+    if (e != hipSuccess) return e;
+  }
+  return launch_units(adapter_down_kernel<T, RT>, p, parts, 64 * kWaves<RT>, kDownLds<RT>, stream);
+}
 template <Float T>
 hipError_t launch_down(const AdapterProduct& p, hipStream_t stream) {
   const int64_t fragments = (p.rank + 15) / 16;
-  if (fragments == 1) return launch_units(adapter_down_kernel<T, 1>, p, p.splits, 64 * kWaves, stream);
-  if (fragments == 2) return launch_units(adapter_down_kernel<T, 2>, p, p.splits, 64 * kWaves, stream);
-  return launch_units(adapter_down_kernel<T, kFragments>, p, (fragments + kFragments - 1) / kFragments * p.splits, 64 * kWaves, stream);
+  if (fragments == 1) return launch_down_of<T, 1>(p, p.splits, stream);
+  if (fragments == 2) return launch_down_of<T, 2>(p, p.splits, stream);
+  return launch_down_of<T, kFragments>(p, (fragments + kFragments - 1) / kFragments * p.splits, stream);
 }
 
 template <Float T, Float OUT, bool FAST>
 hipError_t launch_up_of(const AdapterProduct& p, int64_t parts, hipStream_t stream) {
-  if (p.rank <= 16) return launch_units(adapter_up_kernel<T, OUT, true, 1, 4, FAST, false>, p, parts, 256, stream);
-  if (p.rank <= 32) return launch_units(adapter_up_kernel<T, OUT, false, 1, 4, FAST, false>, p, parts, 256, stream);
-  if (p.rank <= 64) return launch_units(adapter_up_kernel<T, OUT, false, 2, 2, FAST, false>, p, parts, 256, stream);
-  return launch_units(adapter_up_kernel<T, OUT, false, 2, 2, FAST, true>, p, parts, 256, stream);
+  if (p.rank <= 16) return launch_units(adapter_up_kernel<T, OUT, true, 1, 4, FAST, false>, p, parts, 256, 0, stream);
+  if (p.rank <= 32) return launch_units(adapter_up_kernel<T, OUT, false, 1, 4, FAST, false>, p, parts, 256, 0, stream);
+  if (p.rank <= 64) return launch_units(adapter_up_kernel<T, OUT, false, 2, 2, FAST, false>, p, parts, 256, 0, stream);
+  return launch_units(adapter_up_kernel<T, OUT, false, 2, 2, FAST, true>, p, parts, 256, 0, stream);
 }
 template <Float T>
 hipError_t launch_up(const AdapterProduct& p, hipStream_t stream) {
