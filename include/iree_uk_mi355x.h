@@ -614,10 +614,14 @@ void iree_uk_mi355x_gated_mmt4d_p(const iree_uk_mi355x_gated_mmt4d_params_t* par
  * and du are rounded to the operands' type in between, which the matrix
  * instructions take; the sums over them are in f32 and rounded once. A gradient
  * whose buffer is NULL is not computed, and gate and up are not read without
- * lhs_grad, nor lhs without the gradients of the weights.
+ * lhs_grad, nor lhs without the gradients of the weights. The same call gives
+ * the same bits. The fast kernels ask gate and up, for lhs_grad, and lhs, for the
+ * others, to have tiles of 1, 2, 4, .. 32 rows and a multiple of 8 columns (one
+ * row tall: of 8 columns in all), and to be aligned as above.
  *   workspace: device memory of iree_uk_mi355x_gated_mmt4d_backward_workspace()
  *   bytes, 256-byte aligned, which is written before it is read and holds
- *   nothing afterwards. Calls that may run at the same time, graphs that hold
+ *   nothing afterwards: dg and du, and where lhs_grad has few rows parts of its
+ *   sums in f32. Calls that may run at the same time, graphs that hold
  *   them included, need workspaces of their own. (In synchronous mode it may be
  *   host memory like any other buffer; it is not touched then.) */
 void iree_uk_mi355x_gated_mmt4d_backward_p(const iree_uk_mi355x_gated_mmt4d_backward_params_t* params);
@@ -639,7 +643,12 @@ iree_uk_index_t iree_uk_mi355x_gated_mmt4d_backward_workspace(
  * rank sums included; the result is rounded once where it is f16 or bf16 (with
  * ACCUMULATE the destination's value is added before that). Rows may come in
  * any order; those of one adapter next to each other share the reads of it.
- * The same call gives the same bits.
+ * The same call gives the same bits, and a row's do not depend on the adapters
+ * of other rows. The fast kernels multiply a rank sum by `up` as two or three
+ * floats of its type that add up to it (of f16 within 2^-24 of it, or 2^-39 of
+ * the row's largest), so that an infinite value of `up` gives infinities or NaN.
+ * They take an lhs as above and a `down` whose address and strides are multiples
+ * of 16 bytes; `up` may lie anywhere, and is read faster aligned like that.
  *   workspace: as above, of iree_uk_mi355x_adapter_mmt4d_workspace() bytes. */
 void iree_uk_mi355x_adapter_mmt4d_p(const iree_uk_mi355x_adapter_mmt4d_params_t* params);
 iree_uk_index_t iree_uk_mi355x_adapter_mmt4d_workspace(const iree_uk_mi355x_adapter_mmt4d_params_t* params);
