@@ -244,6 +244,10 @@ __device__ __forceinline__ void split_sum(float v, uint16_t (&part)[3]) {
 // The splits' sums are added on their way into LDS, where a workgroup's four wavefronts have them from; only those of rows that have the
 // adapter are read. The next turn's `up` and results are on their way while one's are multiplied.
 //
+// 64 rows of 64 adapters x 14336, rank 16, take 14.0 us, 36 MB at 2.6 TB/s: a wavefront waits for its index, then for its sums, then has
+// three turns to make up for it. 2000 rows in runs x 4096, rank 64, take 23 us, of which the f32
+// results, read and written, are 65 MB. Results turned in LDS, so that four lanes have 64 bytes of a row, gained 4 % there and lost 10 % here.
+//
 // FAST: columns come in whole sixteens that lie next to each other, aligned, and an adapter's row of `up` in whole eights, aligned. (As
 // two branches of one kernel the slow one's registers halved the number of wavefronts on a compute unit.)
 template <Float T, Float OUT, bool HALF, int CHUNKS, int F, bool FAST, bool MANY>
@@ -456,7 +460,8 @@ int64_t pitch_of(int64_t rank) { return (rank + 31) / 32 * 32; }
 
 bool multiple(const void* p, int64_t to) { return (uintptr_t)p % to == 0; }
 
-// Fragments of columns of a wavefront's turn, and turns: as many as leave some 4096 wavefronts, sixteen to a compute unit.
+// Fragments of columns of a wavefront's turn, and turns: as many as leave some 4096 wavefronts, sixteen to a compute unit. (64 rows of 64
+// adapters, rank 16, and 2000 rows of 12, rank 64: 14.0 and 22.9 us; twice as many wavefronts 19.5 and 24.7; half as many, the latter 28.8.)
 int up_fragments(int64_t rank) { return rank <= 32 ? 4 : 2; }
 uint32_t turns_of(int64_t rows, int64_t slots, int64_t cols, int64_t rank) {
   const int64_t across = (cols + 16 * up_fragments(rank) - 1) / (16 * up_fragments(rank)), t = (rows + 15) / 16 * slots * across / 4096;

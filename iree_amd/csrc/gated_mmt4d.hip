@@ -104,7 +104,7 @@ bool block_covers(const GatedProduct& p) {
 // more than 16 rows the block kernels, which read the lhs less often, are left to decide.
 //
 // Fitted to the times of every kernel in 530 problems drawn from 1 to 4096 rows, 64 to 28672 columns, K of 64 to 14336, row-major and
-// tiled; over these the kernel taken is slower than the best one by 3.3 % in the mean, by more than 15 % in one of twenty.
+// tiled; over these the kernel taken is slower than the best one by 2.7 % in the mean, by more than 15 % in one of twenty.
 struct Choice {
   enum { kGeneric, kFew, kBlock } kernel;
   int number;
