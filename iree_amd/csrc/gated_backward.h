@@ -118,10 +118,14 @@ struct GradTile {
   int rows, cols;
 };
 constexpr GradTile kGradTiles[] = {{256, 256}, {256, 128}, {128, 256}, {128, 128}, {128, 64}, {64, 128}, {64, 64}};
+constexpr int kSmallestGradTile = 6;
 hipError_t launch_lhs_grad_f16(const LhsGradProduct& p, int tile, hipStream_t stream);
 hipError_t launch_lhs_grad_bf16(const LhsGradProduct& p, int tile, hipStream_t stream);
 hipError_t launch_weight_grad_f16(const WeightGradProduct& p, int tile, hipStream_t stream);
 hipError_t launch_weight_grad_bf16(const WeightGradProduct& p, int tile, hipStream_t stream);
+// Both in one launch, in tiles of 64x64.
+hipError_t launch_both_grads_f16(const LhsGradProduct& lhs, const WeightGradProduct& weights, hipStream_t stream);
+hipError_t launch_both_grads_bf16(const LhsGradProduct& lhs, const WeightGradProduct& weights, hipStream_t stream);
 
 }  // namespace uk
 

@@ -238,68 +238,61 @@ __global__ __launch_bounds__(kThreads) void gated_lhs_grad_sums(const SumArgs p)
 }
 
 // false: the general kernel takes it.
-bool launch_lhs_grad(const GatedBackwardArgs& a, const Sizes& s, hipStream_t stream, hipError_t* e) {
-  LhsGradProduct p;
+bool as_lhs_grad(const GatedBackwardArgs& a, const Sizes& s, LhsGradProduct* p, Choice* c) {
   Strided16 up;
   if (s.rows == 0 || s.cols == 0 || s.cols > 0x7FFFFFFF - 512) return false;
-  if (!as_operand16(a.workspace, s.pitch, s.rows, 1, s.cols, 1, &p.grads) || !near16(p.grads, 256) ||
-      !as_strided16(a.gate, a.gate_stride0, a.N, a.N0, a.K, a.K0, &p.gate) || !as_strided16(a.up, a.up_stride0, a.N, a.N0, a.K, a.K0, &up))
+  if (!as_operand16(a.workspace, s.pitch, s.rows, 1, s.cols, 1, &p->grads) || !near16(p->grads, 256) ||
+      !as_strided16(a.gate, a.gate_stride0, a.N, a.N0, a.K, a.K0, &p->gate) || !as_strided16(a.up, a.up_stride0, a.N, a.N0, a.K, a.K0, &up))
     return false;
-  p.up = up.data;
-  p.up_stride0 = up.stride0;
-  p.lhs_second = s.pitch;  // (half of a row's bytes)
-  p.depth = (uint32_t)s.cols;
-  p.results = results_of(a, layout_of(a.lhs_grad_stride0, a.M0, a.K, a.K0), a.lhs_grad, nullptr, a.lhs_grad_stride0, 0, s.rows, a.M, false);
-  const Choice c = choose_lhs_grad(s);
-  if (c.tile < 0) return false;
-  const Layout at = p.results.at;
-  const bool f16 = a.type == Float::kF16;
-  if (c.splits > 1) {  // (the depth is a multiple of eight)
-    uint8_t* const parts = a.workspace + grads_bytes(s);
-    p.results.out[0] = parts;
-    p.results.at = layout_of(s.depth, 1, s.depth, 1);
-    p.results.stride0[0] = s.depth;
-    p.results.type = Float::kF32;
-    p.results.runs = 1;
-    p.results.apart = s.rows * s.depth * 4;
-    p.results.copies = (uint32_t)c.splits;
+  p->up = up.data;
+  p->up_stride0 = up.stride0;
+  p->lhs_second = s.pitch;  // (half of a row's bytes)
+  p->depth = (uint32_t)s.cols;
+  p->results = results_of(a, layout_of(a.lhs_grad_stride0, a.M0, a.K, a.K0), a.lhs_grad, nullptr, a.lhs_grad_stride0, 0, s.rows, a.M, false);
+  *c = choose_lhs_grad(s);
+  if (c->splits > 1) {  // (the depth is a multiple of eight)
+    GradResults& r = p->results;
+    r.out[0] = a.workspace + grads_bytes(s);
+    r.at = layout_of(s.depth, 1, s.depth, 1);
+    r.stride0[0] = s.depth;
+    r.type = Float::kF32;
+    r.runs = 1;
+    r.apart = s.rows * s.depth * 4;
+    r.copies = (uint32_t)c->splits;
   }
-  *e = f16 ? launch_lhs_grad_f16(p, c.tile, stream) : launch_lhs_grad_bf16(p, c.tile, stream);
-  if (c.splits == 1 || *e != hipSuccess) return true;
+  return c->tile >= 0;
+}
+hipError_t launch_sums(const GatedBackwardArgs& a, const Sizes& s, int splits, hipStream_t stream) {
   SumArgs g;
   g.parts = (const float*)(a.workspace + grads_bytes(s));
   g.out = a.lhs_grad;
-  g.at = at;
+  g.at = layout_of(a.lhs_grad_stride0, a.M0, a.K, a.K0);
   g.cols = (uint32_t)s.depth;
   g.fours = g.cols / 4;
   g.results = s.rows * g.fours;
   g.apart = s.rows * s.depth;
-  g.splits = c.splits;
+  g.splits = splits;
   const int size = float_bytes(a.out_type);
-  g.runs = runs_of(at, a.lhs_grad, a.M, size, 4, 4 * size);
+  g.runs = runs_of(g.at, a.lhs_grad, a.M, size, 4, 4 * size);
   g.type = a.out_type;
   const int64_t groups = (g.results + kThreads - 1) / kThreads;
-  *e = launch_kernel(f16 ? gated_lhs_grad_sums<Float::kF16> : gated_lhs_grad_sums<Float::kBf16>, (unsigned)(groups < (1 << 22) ? groups : 1 << 22),
-                     kThreads, 0, stream, g);
-  return true;
+  return launch_kernel(a.type == Float::kF16 ? gated_lhs_grad_sums<Float::kF16> : gated_lhs_grad_sums<Float::kBf16>,
+                       (unsigned)(groups < (1 << 22) ? groups : 1 << 22), kThreads, 0, stream, g);
 }
-bool launch_weight_grads(const GatedBackwardArgs& a, const Sizes& s, hipStream_t stream, hipError_t* e) {
-  WeightGradProduct p;
+bool as_weight_grads(const GatedBackwardArgs& a, const Sizes& s, WeightGradProduct* p, Choice* c) {
   if (s.rows == 0 || s.cols == 0 || s.rows > 0x7FFFFFFF || s.cols > 0x7FFFFFFF - 512) return false;
   const uint8_t* const grads = a.workspace + (a.gate_grad ? 0 : s.pitch);
   // (As many columns of dg as there are with the zeros that fill up an eight.)
-  if (!as_strided16(grads, s.pitch, s.rows, 1, s.pitch / 2, 1, &p.grads) || !as_strided16(a.lhs, a.lhs_stride0, a.M, a.M0, a.K, a.K0, &p.lhs))
+  if (!as_strided16(grads, s.pitch, s.rows, 1, s.pitch / 2, 1, &p->grads) || !as_strided16(a.lhs, a.lhs_stride0, a.M, a.M0, a.K, a.K0, &p->lhs))
     return false;
-  p.lhs_second = s.pitch;
-  p.depth = (uint32_t)s.rows;
+  p->lhs_second = s.pitch;
+  p->depth = (uint32_t)s.rows;
   uint8_t* const first = a.gate_grad ? a.gate_grad : a.up_grad;
   uint8_t* const second = a.gate_grad ? a.up_grad : nullptr;
   const int64_t stride0 = a.gate_grad ? a.gate_grad_stride0 : a.up_grad_stride0;
-  p.results = results_of(a, layout_of(stride0, a.N0, a.K, a.K0), first, second, stride0, a.up_grad_stride0, s.cols, a.N, a.accumulate);
-  const Choice c = choose(kWeightGradTimes, s.cols, s.depth, (s.rows + 31) / 32, p.results.copies, 1);
-  if (c.tile < 0) return false;
-  *e = a.type == Float::kF16 ? launch_weight_grad_f16(p, c.tile, stream) : launch_weight_grad_bf16(p, c.tile, stream);
-  return true;
+  p->results = results_of(a, layout_of(stride0, a.N0, a.K, a.K0), first, second, stride0, a.up_grad_stride0, s.cols, a.N, a.accumulate);
+  *c = choose(kWeightGradTimes, s.cols, s.depth, (s.rows + 31) / 32, p->results.copies, 1);
+  return c->tile >= 0;
 }
 
 bool launch_first(const GatedBackwardArgs& a, const Sizes& s, hipStream_t stream, hipError_t* e) {
@@ -350,9 +343,23 @@ hipError_t launch_gated_backward(const GatedBackwardArgs& a, hipStream_t stream,
   hipError_t e = hipSuccess;
   if (!launch_first(a, s, stream, &e))
     e = launch_over(gated_backward_generic<Float::kF16>, gated_backward_generic<Float::kBf16>, g, s.rows * (s.pitch / 2), stream);
-  if (e == hipSuccess && a.lhs_grad && !launch_lhs_grad(a, s, stream, &e))
+  if (e != hipSuccess) return e;
+  LhsGradProduct lhs;
+  WeightGradProduct weights;
+  Choice of_lhs = {-1, 1}, of_weights = {-1, 1};
+  const bool any_weights = a.gate_grad || a.up_grad, f16 = a.type == Float::kF16;
+  const bool lhs_fast = a.lhs_grad && as_lhs_grad(a, s, &lhs, &of_lhs), weights_fast = any_weights && as_weight_grads(a, s, &weights, &of_weights);
+  if (lhs_fast && weights_fast && of_lhs.tile == kSmallestGradTile && of_weights.tile == kSmallestGradTile) {
+    e = f16 ? launch_both_grads_f16(lhs, weights, stream) : launch_both_grads_bf16(lhs, weights, stream);
+  } else {
+    if (lhs_fast) e = f16 ? launch_lhs_grad_f16(lhs, of_lhs.tile, stream) : launch_lhs_grad_bf16(lhs, of_lhs.tile, stream);
+    if (e == hipSuccess && weights_fast)
+      e = f16 ? launch_weight_grad_f16(weights, of_weights.tile, stream) : launch_weight_grad_bf16(weights, of_weights.tile, stream);
+  }
+  if (e == hipSuccess && lhs_fast && of_lhs.splits > 1) e = launch_sums(a, s, of_lhs.splits, stream);
+  if (e == hipSuccess && a.lhs_grad && !lhs_fast)
     e = launch_over(gated_lhs_grad_generic<Float::kF16>, gated_lhs_grad_generic<Float::kBf16>, g, s.rows * s.depth, stream);
-  if (e == hipSuccess && (a.gate_grad || a.up_grad) && !launch_weight_grads(a, s, stream, &e))
+  if (e == hipSuccess && any_weights && !weights_fast)
     e = launch_over(gated_weight_grad_generic<Float::kF16>, gated_weight_grad_generic<Float::kBf16>, g, s.cols * s.depth, stream);
   return e;
 }

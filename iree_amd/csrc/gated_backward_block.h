@@ -24,8 +24,7 @@ hipError_t launch_grad_tile(const P& p, int tile, hipStream_t stream) {
   return hipErrorInvalidValue;
 }
 
-template <Float T>
-hipError_t launch_lhs_grad(const LhsGradProduct& g, int tile, hipStream_t stream) {
+inline BlockProduct<LhsGrad, Operand16, Strided16> as_block_product(const LhsGradProduct& g) {
   BlockProduct<LhsGrad, Operand16, Strided16> p;
   p.lhs = g.grads;
   p.rhs = g.gate;
@@ -34,10 +33,9 @@ hipError_t launch_lhs_grad(const LhsGradProduct& g, int tile, hipStream_t stream
   p.lhs_second = g.lhs_second;
   p.depth = g.depth;
   (GradResults&)p.epilogue = g.results;
-  return launch_grad_tile<T>(p, tile, stream);
+  return p;
 }
-template <Float T>
-hipError_t launch_weight_grad(const WeightGradProduct& g, int tile, hipStream_t stream) {
+inline BlockProduct<WeightGrads, Strided16, Strided16> as_block_product(const WeightGradProduct& g) {
   BlockProduct<WeightGrads, Strided16, Strided16> p;
   p.lhs = g.grads;
   p.rhs = g.lhs;
@@ -46,7 +44,28 @@ hipError_t launch_weight_grad(const WeightGradProduct& g, int tile, hipStream_t 
   p.lhs_second = g.lhs_second;
   p.depth = g.depth;
   (GradResults&)p.epilogue = g.results;
-  return launch_grad_tile<T>(p, tile, stream);
+  return p;
+}
+
+// Both products' workgroups in one launch, 64x64 tiles of each.
+struct BothGrads {
+  BlockProduct<LhsGrad, Operand16, Strided16> lhs;
+  BlockProduct<WeightGrads, Strided16, Strided16> weights;
+  uint32_t of_lhs;  // workgroups, a multiple of 8
+};
+template <Float T>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void both_grads_kernel(const BothGrads p) {
+  if (blockIdx.x < p.of_lhs) product16_block<T, 1, 1, 8, false>(p.lhs, blockIdx.x);
+  else product16_block<T, 1, 1, 8, false>(p.weights, blockIdx.x - p.of_lhs);
+}
+template <Float T>
+hipError_t launch_both_grads(const LhsGradProduct& lhs, const WeightGradProduct& weights, hipStream_t stream) {
+  constexpr int LDS = block_lds_bytes(1, 1, 8);
+  static_assert(LDS <= 64 * 1024, "LDS");
+  BothGrads p{as_block_product(lhs), as_block_product(weights), 0};
+  p.of_lhs = lay_out_tiles<1, 1>(p.lhs);
+  const unsigned of_weights = lay_out_tiles<1, 1>(p.weights);
+  return launch_kernel(both_grads_kernel<T>, p.of_lhs + of_weights, 256, LDS, stream, p);
 }
 
 }  // namespace

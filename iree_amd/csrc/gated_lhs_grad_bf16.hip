@@ -1,5 +1,7 @@
 #include "gated_backward_block.h"
 
 namespace uk {
-hipError_t launch_lhs_grad_bf16(const LhsGradProduct& p, int tile, hipStream_t stream) { return launch_lhs_grad<Float::kBf16>(p, tile, stream); }
+hipError_t launch_lhs_grad_bf16(const LhsGradProduct& p, int tile, hipStream_t stream) {
+  return launch_grad_tile<Float::kBf16>(as_block_product(p), tile, stream);
+}
 }  // namespace uk

@@ -189,9 +189,11 @@ __device__ __forceinline__ void read_piece(const Strided16&, const uint8_t* side
 
 constexpr int block_lds_bytes(int am, int bn, int stages) { return stages * 64 * (am + bn) * 64; }
 
+constexpr bool two_fit(int am, int bn, int stages) { return am * bn <= 8 && block_lds_bytes(am, bn, stages) <= 80 * 1024; }
+
+// Workgroup `number` of a product's.
 template <Float T, int AM, int BN, int STAGES, bool STREAM, typename E, typename A, typename B>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(AM * BN <= 8 && block_lds_bytes(AM, BN, STAGES) <= 80 * 1024 ? 2 : 1, 2)))
-void product16_block_kernel(const BlockProduct<E, A, B> p) {
+__device__ __forceinline__ void product16_block(const BlockProduct<E, A, B>& p, uint32_t number) {
   constexpr bool PAIRED = E::kPaired, IN_TURN = E::kInTurn;
   constexpr int ROWS = 64 * AM, COLS = 64 * BN, RESULTS = PAIRED ? COLS / 2 : COLS;
   constexpr int A_BYTES = ROWS * 64, STAGE = A_BYTES + COLS * 64;
@@ -199,8 +201,8 @@ void product16_block_kernel(const BlockProduct<E, A, B> p) {
   static_assert(STAGES >= 3 && (STAGES - 1) * LOADS <= 63, "ring depth");
 
   const uint32_t tiles = p.tile_rows * p.tile_cols, per_xcd = (tiles + 7) >> 3;
-  const uint32_t linear = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= per_xcd || linear >= tiles) return;
+  const uint32_t linear = (number & 7) * per_xcd + (number >> 3);
+  if ((number >> 3) >= per_xcd || linear >= tiles) return;
   int tile_row, tile_col;
   tile_of_number(linear, p.tile_rows, p.tile_cols, p.band_reciprocal, &tile_row, &tile_col);
   // (An epilogue's copies: a second result's tiles, or another part of K's, come behind those of the first.)
@@ -379,10 +381,16 @@ void product16_block_kernel(const BlockProduct<E, A, B> p) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <Float T, int AM, int BN, int STAGES, bool STREAM = false, typename E, typename A, typename B>
-hipError_t launch_block_tile(BlockProduct<E, A, B> p, hipStream_t stream) {
-  constexpr int RESULTS = E::kPaired ? 32 * BN : 64 * BN, LDS = block_lds_bytes(AM, BN, STAGES);
-  static_assert(LDS <= 160 * 1024, "LDS");
+template <Float T, int AM, int BN, int STAGES, bool STREAM, typename E, typename A, typename B>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(two_fit(AM, BN, STAGES) ? 2 : 1, 2)))
+void product16_block_kernel(const BlockProduct<E, A, B> p) {
+  product16_block<T, AM, BN, STAGES, STREAM>(p, blockIdx.x);
+}
+
+// Fills in what a kernel of these tiles needs of the grid, and returns its workgroups, a multiple of 8.
+template <int AM, int BN, typename E, typename A, typename B>
+unsigned lay_out_tiles(BlockProduct<E, A, B>& p) {
+  constexpr int RESULTS = E::kPaired ? 32 * BN : 64 * BN;
   p.tile_rows = (p.lhs.rows + 64 * AM - 1) / (64 * AM);
   if constexpr (E::kCopies) {
     p.epilogue.tile_rows_of_copy = p.tile_rows;
@@ -391,11 +399,18 @@ hipError_t launch_block_tile(BlockProduct<E, A, B> p, hipStream_t stream) {
   }
   p.tile_cols = (p.rhs.rows + RESULTS - 1) / RESULTS;
   p.band_reciprocal = band_reciprocal(p.tile_cols);
-  const unsigned tiles = p.tile_rows * p.tile_cols;
+  return (p.tile_rows * p.tile_cols + 7) / 8 * 8;
+}
+
+template <Float T, int AM, int BN, int STAGES, bool STREAM = false, typename E, typename A, typename B>
+hipError_t launch_block_tile(BlockProduct<E, A, B> p, hipStream_t stream) {
+  constexpr int LDS = block_lds_bytes(AM, BN, STAGES);
+  static_assert(LDS <= 160 * 1024, "LDS");
+  const unsigned groups = lay_out_tiles<AM, BN>(p);
   void (*kernel)(const BlockProduct<E, A, B>) = product16_block_kernel<T, AM, BN, STAGES, STREAM, E, A, B>;
   const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (e != hipSuccess) return e;
-  return launch_kernel(kernel, (tiles + 7) / 8 * 8, 256, LDS, stream, p);
+  return launch_kernel(kernel, groups, 256, LDS, stream, p);
 }
 
 }  // namespace
