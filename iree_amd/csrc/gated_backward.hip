@@ -163,10 +163,11 @@ GradResults results_of(const GatedBackwardArgs& a, const Layout& at, uint8_t* fi
 // in 28 parts and 188 in one, 100 x 12176 x 3504 45 and 125, 508 x 9526 x 325 33 and 105, 2048 x 8192 x 4096 245 in two and 283 in one
 // (of smaller tiles). tile -1: none can.
 struct Times { float start, one, two, start_again, busy; };  // two = 0: one workgroup on a compute unit
-struct Choice { int tile, splits; };
+struct Choice { int tile, splits; float cost; };
+// The parts of sums are written and read, in a launch more.
+float parts_time(int64_t rows, int64_t cols, int64_t splits) { return splits == 1 ? 0 : 2 + (float)splits * (float)(rows * cols) * 1.5e-6f; }
 Choice choose(const Times* times, int64_t rows, int64_t cols, int64_t chunks, int64_t copies, int64_t most_splits) {
-  Choice best = {-1, 1};
-  float least = 0;
+  Choice best = {-1, 1, 0};
   for (int i = 0; i < (int)(sizeof kGradTiles / sizeof kGradTiles[0]); ++i) {
     const GradTile& t = kGradTiles[i];
     const int64_t of_one = (rows + t.rows - 1) / t.rows * ((cols + t.cols - 1) / t.cols) * copies;
@@ -174,15 +175,10 @@ Choice choose(const Times* times, int64_t rows, int64_t cols, int64_t chunks, in
     for (int64_t splits = 1; splits <= most_splits; ++splits) {
       const int64_t tiles = of_one * splits, rounds = (tiles + 255) / 256;
       if (tiles > (1 << 23)) continue;  // (a grid has fewer than 2^32 threads)
-      // (The parts of sums are written and read, in a launch more.)
-      const float parts = splits == 1 ? 0 : 2 + (float)splits * (float)(rows * cols) * 1.5e-6f;
       const float in_turn = (float)chunks / (float)splits * (of.two == 0 ? rounds * of.one : (rounds >> 1) * of.two + (rounds & 1) * of.one);
       const float busy = (float)of_one * (float)chunks / 256 * of.busy, steps = in_turn > busy ? in_turn : busy;
-      const float cost = of.start + (rounds - 1) * of.start_again + steps + parts;
-      if (best.tile < 0 || cost < least) {
-        least = cost;
-        best = {i, (int)splits};
-      }
+      const float cost = of.start + (rounds - 1) * of.start_again + steps + parts_time(rows, cols, splits);
+      if (best.tile < 0 || cost < best.cost) best = {i, (int)splits, cost};
     }
   }
   return best;
@@ -195,12 +191,44 @@ constexpr Times kWeightGradTimes[] = {{17.3f, .522f, 0, 15.6f, .92f},   {11.9f, 
                                       {6.3f, .141f, .210f, 1.1f, .12f}};
 
 // lhs_grad's. A split has sixteen chunks at least, and all of them 64 MiB of sums at most.
-Choice choose_lhs_grad(const Sizes& s) {
-  if (s.rows < 1 || s.cols < 1 || s.depth < 1 || s.rows > INT32_MAX || s.cols > INT32_MAX || s.depth > INT32_MAX) return {-1, 1};
+int64_t most_splits(const Sizes& s) {
   const int64_t whole = 2 * (s.cols / 32), of_sums = s.rows > (1 << 24) / s.depth ? 1 : (1 << 24) / (s.rows * s.depth);
   const int64_t most = whole / 16 < of_sums ? whole / 16 : of_sums;
-  return choose(kLhsGradTimes, s.rows, s.depth, 2 * ((s.cols + 31) / 32), 1, most < 1 ? 1 : most > 32 ? 32 : most);
+  return most < 1 ? 1 : most > 32 ? 32 : most;
 }
+bool choosable(const Sizes& s) {
+  return s.rows > 0 && s.cols > 0 && s.depth > 0 && s.rows <= INT32_MAX && s.cols <= INT32_MAX && s.depth <= INT32_MAX;
+}
+Choice choose_lhs_grad(const Sizes& s) {
+  if (!choosable(s)) return {-1, 1, 0};
+  return choose(kLhsGradTimes, s.rows, s.depth, 2 * ((s.cols + 31) / 32), 1, most_splits(s));
+}
+// Both products in one launch of 64x64 tiles: the longer of them, or all chunks of all tiles, as many as the machine has at a time. Over
+// 120 problems of 1 to 2048 rows, 64 to 12000 columns, K of 64 to 6000 a backward pass takes 1.23 times less in the mean where this is
+// chosen for the less time (130 x 1000 x 500 15.5 us and not 20, 37 x 1338 x 1001 13.8 and 18.9; but 30 x 8567 x 3462 94 and 68 apart); what is
+// chosen is slower than the better by 0.1 % in the mean.
+constexpr float kBothStart = 5.6f, kBothOne = .150f, kBothTwo = .155f, kBothAgain = 2.34f, kBothBusy = .15f;
+Choice choose_both(const Sizes& s, int64_t copies) {
+  Choice best = {-1, 1, 0};
+  if (!choosable(s)) return best;
+  const int64_t of_lhs = (s.rows + 63) / 64 * ((s.depth + 63) / 64), of_weights = (s.cols + 63) / 64 * ((s.depth + 63) / 64) * copies;
+  const int64_t lhs_chunks = 2 * ((s.cols + 31) / 32), weight_chunks = (s.rows + 31) / 32, most = most_splits(s);
+  if (of_lhs * most + of_weights > (1 << 23)) return best;
+  const float all = ((float)of_lhs * (float)lhs_chunks + (float)of_weights * (float)weight_chunks) / 256 * kBothBusy;
+  for (int64_t splits = 1; splits <= most; ++splits) {
+    const int64_t tiles = of_lhs * splits + of_weights;
+    const float longer = lhs_chunks > splits * weight_chunks ? (float)lhs_chunks / (float)splits : (float)weight_chunks;
+    const float in_turn = longer * (tiles > 256 ? kBothTwo : kBothOne), steps = in_turn > all ? in_turn : all;
+    const float cost = kBothStart + (float)((tiles + 511) / 512 - 1) * kBothAgain + steps + parts_time(s.rows, s.depth, splits);
+    if (best.tile < 0 || cost < best.cost) best = {kSmallestGradTile, (int)splits, cost};
+  }
+  return best;
+}
+Choice choose_weight_grads(const Sizes& s, int64_t copies) {
+  if (!choosable(s)) return {-1, 1, 0};
+  return choose(kWeightGradTimes, s.cols, s.depth, (s.rows + 31) / 32, copies, 1);
+}
+int64_t copies_of(const GatedBackwardArgs& a) { return (a.gate_grad != nullptr) + (a.up_grad != nullptr); }
 int64_t grads_bytes(const Sizes& s) { return (s.rows * s.pitch * 2 + 255) / 256 * 256; }
 
 // The sums of lhs_grad's splits, in their order: a thread for four of a row. (2048 x 4096 in two parts: 15 us, 84 MB at 5.6 TB/s.)
@@ -238,7 +266,7 @@ __global__ __launch_bounds__(kThreads) void gated_lhs_grad_sums(const SumArgs p)
 }
 
 // false: the general kernel takes it.
-bool as_lhs_grad(const GatedBackwardArgs& a, const Sizes& s, LhsGradProduct* p, Choice* c) {
+bool as_lhs_grad(const GatedBackwardArgs& a, const Sizes& s, LhsGradProduct* p) {
   Strided16 up;
   if (s.rows == 0 || s.cols == 0 || s.cols > 0x7FFFFFFF - 512) return false;
   if (!as_operand16(a.workspace, s.pitch, s.rows, 1, s.cols, 1, &p->grads) || !near16(p->grads, 256) ||
@@ -249,18 +277,17 @@ bool as_lhs_grad(const GatedBackwardArgs& a, const Sizes& s, LhsGradProduct* p, 
   p->lhs_second = s.pitch;  // (half of a row's bytes)
   p->depth = (uint32_t)s.cols;
   p->results = results_of(a, layout_of(a.lhs_grad_stride0, a.M0, a.K, a.K0), a.lhs_grad, nullptr, a.lhs_grad_stride0, 0, s.rows, a.M, false);
-  *c = choose_lhs_grad(s);
-  if (c->splits > 1) {  // (the depth is a multiple of eight)
-    GradResults& r = p->results;
-    r.out[0] = a.workspace + grads_bytes(s);
-    r.at = layout_of(s.depth, 1, s.depth, 1);
-    r.stride0[0] = s.depth;
-    r.type = Float::kF32;
-    r.runs = 1;
-    r.apart = s.rows * s.depth * 4;
-    r.copies = (uint32_t)c->splits;
-  }
-  return c->tile >= 0;
+  return true;
+}
+// (The depth is a multiple of eight.)
+void split_sums(const GatedBackwardArgs& a, const Sizes& s, int splits, GradResults* r) {
+  r->out[0] = a.workspace + grads_bytes(s);
+  r->at = layout_of(s.depth, 1, s.depth, 1);
+  r->stride0[0] = s.depth;
+  r->type = Float::kF32;
+  r->runs = 1;
+  r->apart = s.rows * s.depth * 4;
+  r->copies = (uint32_t)splits;
 }
 hipError_t launch_sums(const GatedBackwardArgs& a, const Sizes& s, int splits, hipStream_t stream) {
   SumArgs g;
@@ -279,7 +306,7 @@ hipError_t launch_sums(const GatedBackwardArgs& a, const Sizes& s, int splits, h
   return launch_kernel(a.type == Float::kF16 ? gated_lhs_grad_sums<Float::kF16> : gated_lhs_grad_sums<Float::kBf16>,
                        (unsigned)(groups < (1 << 22) ? groups : 1 << 22), kThreads, 0, stream, g);
 }
-bool as_weight_grads(const GatedBackwardArgs& a, const Sizes& s, WeightGradProduct* p, Choice* c) {
+bool as_weight_grads(const GatedBackwardArgs& a, const Sizes& s, WeightGradProduct* p) {
   if (s.rows == 0 || s.cols == 0 || s.rows > 0x7FFFFFFF || s.cols > 0x7FFFFFFF - 512) return false;
   const uint8_t* const grads = a.workspace + (a.gate_grad ? 0 : s.pitch);
   // (As many columns of dg as there are with the zeros that fill up an eight.)
@@ -291,8 +318,7 @@ bool as_weight_grads(const GatedBackwardArgs& a, const Sizes& s, WeightGradProdu
   uint8_t* const second = a.gate_grad ? a.up_grad : nullptr;
   const int64_t stride0 = a.gate_grad ? a.gate_grad_stride0 : a.up_grad_stride0;
   p->results = results_of(a, layout_of(stride0, a.N0, a.K, a.K0), first, second, stride0, a.up_grad_stride0, s.cols, a.N, a.accumulate);
-  *c = choose(kWeightGradTimes, s.cols, s.depth, (s.rows + 31) / 32, p->results.copies, 1);
-  return c->tile >= 0;
+  return true;
 }
 
 bool launch_first(const GatedBackwardArgs& a, const Sizes& s, hipStream_t stream, hipError_t* e) {
@@ -327,7 +353,11 @@ int64_t gated_backward_workspace(const GatedBackwardArgs& a) {
   if (__builtin_mul_overflow(s.rows, 2 * s.pitch, &bytes) || bytes > INT64_MAX - (1ll << 30)) return -1;
   bytes = grads_bytes(s);
   if (a.lhs_grad) {
-    const int splits = choose_lhs_grad(s).splits;
+    int splits = choose_lhs_grad(s).splits;
+    if (const int64_t copies = copies_of(a)) {
+      const int both = choose_both(s, copies).splits;
+      splits = splits < both ? both : splits;
+    }
     if (splits > 1) bytes += splits * s.rows * s.depth * 4;
   }
   return bytes;
@@ -346,20 +376,28 @@ hipError_t launch_gated_backward(const GatedBackwardArgs& a, hipStream_t stream,
   if (e != hipSuccess) return e;
   LhsGradProduct lhs;
   WeightGradProduct weights;
-  Choice of_lhs = {-1, 1}, of_weights = {-1, 1};
-  const bool any_weights = a.gate_grad || a.up_grad, f16 = a.type == Float::kF16;
-  const bool lhs_fast = a.lhs_grad && as_lhs_grad(a, s, &lhs, &of_lhs), weights_fast = any_weights && as_weight_grads(a, s, &weights, &of_weights);
-  if (lhs_fast && weights_fast && of_lhs.tile == kSmallestGradTile && of_weights.tile == kSmallestGradTile) {
+  const int64_t copies = copies_of(a);
+  const bool f16 = a.type == Float::kF16;
+  bool lhs_fast = a.lhs_grad && as_lhs_grad(a, s, &lhs), weights_fast = copies && as_weight_grads(a, s, &weights);
+  Choice of_lhs = lhs_fast ? choose_lhs_grad(s) : Choice{-1, 1, 0};
+  const Choice of_weights = weights_fast ? choose_weight_grads(s, copies) : Choice{-1, 1, 0};
+  lhs_fast = of_lhs.tile >= 0;
+  weights_fast = of_weights.tile >= 0;
+  const Choice both = lhs_fast && weights_fast ? choose_both(s, copies) : Choice{-1, 1, 0};
+  const bool together = both.tile >= 0 && both.cost < of_lhs.cost + of_weights.cost;
+  if (together) of_lhs = both;
+  if (of_lhs.splits > 1) split_sums(a, s, of_lhs.splits, &lhs.results);
+  if (together) {
     e = f16 ? launch_both_grads_f16(lhs, weights, stream) : launch_both_grads_bf16(lhs, weights, stream);
   } else {
     if (lhs_fast) e = f16 ? launch_lhs_grad_f16(lhs, of_lhs.tile, stream) : launch_lhs_grad_bf16(lhs, of_lhs.tile, stream);
     if (e == hipSuccess && weights_fast)
       e = f16 ? launch_weight_grad_f16(weights, of_weights.tile, stream) : launch_weight_grad_bf16(weights, of_weights.tile, stream);
   }
-  if (e == hipSuccess && lhs_fast && of_lhs.splits > 1) e = launch_sums(a, s, of_lhs.splits, stream);
+  if (e == hipSuccess && of_lhs.splits > 1) e = launch_sums(a, s, of_lhs.splits, stream);
   if (e == hipSuccess && a.lhs_grad && !lhs_fast)
     e = launch_over(gated_lhs_grad_generic<Float::kF16>, gated_lhs_grad_generic<Float::kBf16>, g, s.rows * s.depth, stream);
-  if (e == hipSuccess && any_weights && !weights_fast)
+  if (e == hipSuccess && copies && !weights_fast)
     e = launch_over(gated_weight_grad_generic<Float::kF16>, gated_weight_grad_generic<Float::kBf16>, g, s.cols * s.depth, stream);
   return e;
 }

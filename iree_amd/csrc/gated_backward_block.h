@@ -47,7 +47,7 @@ inline BlockProduct<WeightGrads, Strided16, Strided16> as_block_product(const We
   return p;
 }
 
-// Both products' workgroups in one launch, 64x64 tiles of each.
+// Both products' workgroups in one launch, 64x64 tiles of each: small gradients, which launches and starts bound.
 struct BothGrads {
   BlockProduct<LhsGrad, Operand16, Strided16> lhs;
   BlockProduct<WeightGrads, Strided16, Strided16> weights;

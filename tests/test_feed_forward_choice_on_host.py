@@ -9,7 +9,7 @@ from feed_forward_reference import up
 from host_launches import recorder  # noqa: F401
 from iree_amd import abi
 from test_gpu_adapter_mmt4d import PROBLEMS as ADAPTERS
-from test_gpu_gated_backward import SPLIT
+from test_gpu_gated_backward import PROBLEMS as BACKWARD, SPLIT
 
 GIB = 1 << 30
 F32, SAME = {"f16": 1, "bf16": 3}, {"f16": 2, "bf16": 4}
@@ -72,6 +72,26 @@ def test_what_is_picked_is_near_the_fastest(recorder):  # noqa: F811
         slower["weights"].append(times[picked] / min(times.values()))
     for of, x in slower.items():
         assert sum(x) / len(x) < 1.05 and max(x) < 1.2, (of, x)
+
+
+def all_gradients(recorder, m, n, k, tile):  # noqa: F811
+    given = [("lhs", "m"), ("gate", "n"), ("up", "n"), ("gate_pre", "o"), ("up_pre", "o"), ("out_grad", "o")]
+    p = filled(abi.GatedMmt4dBackwardParams(), m, n, k, tile, given + [("lhs_grad", "m"), ("gate_grad", "n"), ("up_grad", "n")], SAME["bf16"] | abi.GATED_MMT4D_SILU)
+    p.workspace_buffer, p.workspace_size = 512 * GIB, 256 * GIB
+    kernel = recorder.call("iree_uk_mi355x_gated_mmt4d_backward_p", p)[0]
+    return next((x for x in ("both_grads", "11WeightGrads", "gated_lhs_grad_sums") if x in kernel), None)
+
+
+# Both products in one launch, the parts of lhs_grad's sums behind it; or one after the other.
+@pytest.mark.parametrize("m,n,k,last", [(130, 1000, 512, "gated_lhs_grad_sums"), (206, 353, 749, "both_grads"), (16, 256, 128, "both_grads"),
+                                        (4096, 11008, 4096, "11WeightGrads"),
+                                        (30, 8567, 3462, "gated_lhs_grad_sums")])
+def test_small_gradients_in_one_launch(recorder, m, n, k, last):  # noqa: F811
+    assert all_gradients(recorder, m, n, k, (1, 16, 16)) == last
+
+
+def test_both_products_in_one_launch_are_tested(recorder):  # noqa: F811
+    assert sum(all_gradients(recorder, m, n, k, tile) == "both_grads" for m, n, k, tile in BACKWARD) > 5
 
 
 def test_split_sums_are_tested(recorder):  # noqa: F811
