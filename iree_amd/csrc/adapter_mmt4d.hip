@@ -460,8 +460,9 @@ int64_t pitch_of(int64_t rank) { return (rank + 31) / 32 * 32; }
 
 bool multiple(const void* p, int64_t to) { return (uintptr_t)p % to == 0; }
 
-// Fragments of columns of a wavefront's turn, and turns: as many as leave some 4096 wavefronts, sixteen to a compute unit. (64 rows of 64
-// adapters, rank 16, and 2000 rows of 12, rank 64: 14.0 and 22.9 us; twice as many wavefronts 19.5 and 24.7; half as many, the latter 28.8.)
+// Fragments of columns of a wavefront's turn, and turns: as many as leave some 4096 wavefronts, sixteen to a compute unit. (Both launches
+// with 2048, 4096 and 8192 wavefronts: 64 rows of 64 adapters x 14336, rank 16, 18.0, 19.3, 24.4 us; 2000 rows of 12 in runs x 4096, rank 64,
+// 37.9, 33.7, 33.9; 256 of 40 x 8192, rank 32, 38.2, 34.0, 36.7; 40 of 16 x 11008, rank 16, 13.7, 13.4, 15.0.)
 int up_fragments(int64_t rank) { return rank <= 32 ? 4 : 2; }
 uint32_t turns_of(int64_t rows, int64_t slots, int64_t cols, int64_t rank) {
   const int64_t across = (cols + 16 * up_fragments(rank) - 1) / (16 * up_fragments(rank)), t = (rows + 15) / 16 * slots * across / 4096;
