@@ -72,6 +72,10 @@ hipError_t launch_over(void (*f16)(const AdapterKernelArgs), void (*bf16)(const 
 // Sixteen rows at a time, and of these all that one adapter has: the tile's adapters are numbered in the order of their first
 // rows, and a workgroup takes every SLOTS-th of them. A row has one adapter, so nobody else writes its results; what the matrix
 // instructions compute of the other rows is thrown away, and what is not finite there stays there.
+//
+// Many rows of few adapters are put in order first: a tile is then sixteen rows of one adapter, wherever they are, and each adapter is
+// read once for every sixteen of its rows whatever the order of rows. (Which of an adapter's rows share a tile is up to atomics, and does
+// not matter: a row's results do not depend on the others.)
 
 constexpr int kFragments = 4;  // of 16 columns that a wavefront multiplies by `up`, and of 16 ranks by `down`, at most
 
@@ -87,33 +91,124 @@ struct AdapterProduct {
   Float out_type;
   uint32_t depth, rank, count, cols, pitch, splits;
   uint32_t turns;           // blocks of columns that a wavefront multiplies by `up`, one after the other
-  uint32_t slots, units;    // of a launch: workgroups' pieces of work
+  uint32_t tiles, slots, units;  // of a launch: workgroups' pieces of work
+  const uint4* heads;       // rows in order: of each tile its adapter (count: none), its first row's place in the order, its rows
+  const uint32_t* ids;      // and the sixteen rows; else null
   uint32_t parts, parts_reciprocal, slots_reciprocal;
   int32_t accumulate, runs;
 };
 
-// f(adapter, which of the sixteen rows have it) for every `slots`-th adapter of the rows from `first` on. -> The rows that have none.
-template <typename F>
-__device__ __forceinline__ uint32_t of_adapters(const AdapterProduct& p, uint32_t first, uint32_t slot, int lane, F f) {
-  const uint32_t row = first + (lane & 15);
-  const int32_t named = row < p.lhs.rows ? p.index[row] : -1;
-  const uint32_t with = (uint32_t)__builtin_amdgcn_ballot_w64(named >= 0 && (uint32_t)named < p.count) & 0xFFFF;
-  // The first rows of adapters: nobody before has the same. (Lanes compare with the fifteen in front of them; -1 where there is none, and such a row has no adapter.)
-  bool again = false;
-  int32_t before = named;
+// f(adapter, which of the tile's sixteen rows have it, the row of lane % 16, the first one's place among the sums) for every `slots`-th
+// adapter of a tile. zeros(which of the rows have none, the row of lane % 16), by the first slot.
+template <typename F, typename Z>
+__device__ __forceinline__ void of_adapters(const AdapterProduct& p, uint32_t tile, uint32_t slot, int lane, F f, Z zeros) {
+  const uint32_t at = tile * 16 + (lane & 15);
+  uint32_t row, first = tile * 16, without, todo;  // todo: a bit for each adapter left, that of its first row
+  int32_t named;
+  if (p.heads) {
+    const uint32_t id = p.ids[at];
+    const uint4 head = p.heads[tile];
+    const uint32_t rows = (uint32_t)__builtin_amdgcn_readfirstlane((int)head.z), mask = (1u << rows) - 1;
+    named = (uint32_t)(lane & 15) < rows && head.x < p.count ? (int32_t)head.x : -1;
+    // (Read by all lanes: as an operand of the choice only those lanes would read it that have no row, and the first of them.)
+    const uint32_t first_id = (uint32_t)__builtin_amdgcn_readfirstlane((int)id);
+    row = (uint32_t)(lane & 15) < rows ? id : first_id;
+    first = (uint32_t)__builtin_amdgcn_readfirstlane((int)head.y);
+    const bool any = (uint32_t)__builtin_amdgcn_readfirstlane((int)head.x) < p.count;
+    todo = any && rows != 0 ? 1 : 0;
+    without = any ? 0 : mask;
+  } else {
+    row = at < p.lhs.rows ? at : p.lhs.rows - 1;
+    named = at < p.lhs.rows ? p.index[at] : -1;
+    const uint32_t with = (uint32_t)__builtin_amdgcn_ballot_w64(named >= 0 && (uint32_t)named < p.count) & 0xFFFF;
+    // The first rows of adapters: nobody before has the same. (Lanes compare with the fifteen in front of them; -1 where there is none, and such a row has no adapter.)
+    bool again = false;
+    int32_t before = named;
 #pragma unroll
-  for (int back = 1; back < 16; ++back) {
-    before = __builtin_amdgcn_update_dpp(-1, before, 0x111, 0xF, 0xF, false);  // (of the lane in front, within sixteen)
-    again |= before == named;
+    for (int back = 1; back < 16; ++back) {
+      before = __builtin_amdgcn_update_dpp(-1, before, 0x111, 0xF, 0xF, false);  // (of the lane in front, within sixteen)
+      again |= before == named;
+    }
+    todo = (uint32_t)__builtin_amdgcn_ballot_w64(!again) & with;
+    for (uint32_t i = slot; i != 0 && todo != 0; --i) todo &= todo - 1;
+    without = slot == 0 ? ~with & (p.lhs.rows - first < 16 ? (1u << (p.lhs.rows - first)) - 1 : 0xFFFF) : 0;
   }
-  uint32_t firsts = (uint32_t)__builtin_amdgcn_ballot_w64(!again) & with;
-  for (; slot != 0 && firsts != 0; --slot) firsts &= firsts - 1;
-  while (firsts != 0) {
-    const int32_t of = __builtin_amdgcn_readlane(named, __builtin_ctz(firsts));
-    f((uint32_t)of, (uint32_t)__builtin_amdgcn_ballot_w64(named == of) & with);
-    for (uint32_t i = 0; i < p.slots && firsts != 0; ++i) firsts &= firsts - 1;
+  while (todo != 0) {
+    const int32_t of = __builtin_amdgcn_readlane(named, __builtin_ctz(todo));
+    f((uint32_t)of, (uint32_t)__builtin_amdgcn_ballot_w64(named == of) & 0xFFFF, row, first);
+    for (uint32_t i = 0; i < p.slots && todo != 0; ++i) todo &= todo - 1;
   }
-  return ~with & 0xFFFF;
+  zeros(without, row);
+}
+
+// Rows in the order of their adapters, those without one behind them, and the tiles that this makes, by one workgroup: how many rows each
+// adapter has, where its first one and its first tile come, then each row to its place. Adapters' numbers are in LDS.
+constexpr uint32_t kMostOrdered = 2047, kOrderThreads = 1024;
+struct OrderArgs {
+  const int32_t* index;
+  uint4* heads;
+  uint32_t* ids;
+  uint32_t rows, count, tiles;  // tiles: as many as there may be
+};
+__global__ __launch_bounds__(kOrderThreads) void adapter_order_kernel(const OrderArgs p) {
+  __shared__ uint32_t rows_of[kMostOrdered + 1], taken[kMostOrdered + 1], first_row[kMostOrdered + 1], first_tile[kMostOrdered + 1];
+  __shared__ uint32_t wave_rows[kOrderThreads / 64], wave_tiles[kOrderThreads / 64];
+  const uint32_t thread = threadIdx.x, lane = thread & 63, wave = thread >> 6, entries = p.count + 1;
+  auto adapter_of = [&](uint32_t row) {
+    const int32_t i = p.index[row];
+    return i < 0 || (uint32_t)i >= p.count ? p.count : (uint32_t)i;
+  };
+  for (uint32_t a = thread; a < entries; a += kOrderThreads) rows_of[a] = taken[a] = 0;
+  __syncthreads();
+  for (uint32_t row = thread; row < p.rows; row += kOrderThreads) atomicAdd(&rows_of[adapter_of(row)], 1u);
+  __syncthreads();
+  // Two adapters a thread; sums over the threads in front of it.
+  constexpr uint32_t EACH = (kMostOrdered + 1) / kOrderThreads;
+  uint32_t rows[EACH], own_rows = 0, own_tiles = 0;
+#pragma unroll
+  for (uint32_t e = 0; e < EACH; ++e) {
+    rows[e] = EACH * thread + e < entries ? rows_of[EACH * thread + e] : 0;
+    own_rows += rows[e];
+    own_tiles += (rows[e] + 15) >> 4;
+  }
+  uint32_t rows_here = own_rows, tiles_here = own_tiles;
+#pragma unroll
+  for (int by = 1; by < 64; by *= 2) {
+    const uint32_t r = __shfl_up(rows_here, by), t = __shfl_up(tiles_here, by);
+    if (lane >= (uint32_t)by) {
+      rows_here += r;
+      tiles_here += t;
+    }
+  }
+  if (lane == 63) {
+    wave_rows[wave] = rows_here;
+    wave_tiles[wave] = tiles_here;
+  }
+  __syncthreads();
+  uint32_t row_at = rows_here - own_rows, tile_at = tiles_here - own_tiles, all_tiles = 0;
+  for (uint32_t w = 0; w < kOrderThreads / 64; ++w) {
+    if (w < wave) {
+      row_at += wave_rows[w];
+      tile_at += wave_tiles[w];
+    }
+    all_tiles += wave_tiles[w];
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < EACH; ++e) {
+    if (EACH * thread + e < entries) {
+      first_row[EACH * thread + e] = row_at;
+      first_tile[EACH * thread + e] = tile_at;
+    }
+    row_at += rows[e];
+    tile_at += (rows[e] + 15) >> 4;
+  }
+  __syncthreads();
+  for (uint32_t row = thread; row < p.rows; row += kOrderThreads) {
+    const uint32_t a = adapter_of(row), n = atomicAdd(&taken[a], 1u), tile = first_tile[a] + (n >> 4);
+    p.ids[tile * 16 + (n & 15)] = row;
+    if ((n & 15) == 0) p.heads[tile] = make_uint4(a, first_row[a] + n, rows_of[a] - n < 16 ? rows_of[a] - n : 16, 0);
+  }
+  for (uint32_t tile = all_tiles + thread; tile < p.tiles; tile += kOrderThreads) p.heads[tile] = make_uint4(0, 0, 0, 0);
 }
 
 extern __shared__ uint4 staged[];
@@ -149,17 +244,20 @@ __global__ __launch_bounds__(64 * kWaves<RT>) void adapter_down_kernel(const Ada
     const uint32_t upper = divide(unit, p.parts, p.parts_reciprocal), part = unit - upper * p.parts;
     const uint32_t tile = divide(upper, p.slots, p.slots_reciprocal), slot = upper - tile * p.slots;
     const uint32_t block = part / p.splits, split = part - block * p.splits;
-    const uint32_t first = tile * 16, first_rank = block * (16 * RT);
+    const uint32_t first_rank = block * (16 * RT);
     // (Splits begin with whole fours.)
     const uint32_t fours = (full + 3) / 4;
     const uint32_t from = (uint32_t)((uint64_t)fours * split / p.splits), to = (uint32_t)((uint64_t)fours * (split + 1) / p.splits);
     auto lhs_row = [&](uint32_t row) {
-      row = row < p.lhs.rows ? row : p.lhs.rows - 1;
       const uint32_t panel = divide(row, p.lhs.tile_rows, p.lhs.tile_reciprocal);
       return p.lhs.data + (int64_t)panel * p.lhs.stride0 + (row - panel * p.lhs.tile_rows) * p.lhs.row_bytes;
     };
     const int64_t lhs_step = 64 * (int64_t)p.lhs.tile_rows;
-    of_adapters(p, first, slot, lane, [&](uint32_t of, uint32_t same) {
+    auto no_zeros = [](uint32_t, uint32_t) {};
+    of_adapters(p, tile, slot, lane, [&](uint32_t of, uint32_t same, uint32_t row, uint32_t first) {
+      const uint8_t* rows[4];  // of the lane's loads
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rows[i] = lhs_row((uint32_t)__shfl((int)row, 4 * i + g));
       auto down_row = [&](uint32_t rank) {
         return p.down + of * p.down_stride0 + (int64_t)(rank < p.rank ? rank : p.rank - 1) * p.down_stride1;
       };
@@ -169,7 +267,7 @@ __global__ __launch_bounds__(64 * kWaves<RT>) void adapter_down_kernel(const Ada
         for (int i = 0; i < 4; ++i) {
           const uint32_t of_sixteen = 4 * i + g, piece = (uint32_t)r ^ of_sixteen;
           const uint32_t chunk = 4 * four + (piece >> 2) < full ? 4 * four + (piece >> 2) : full - 1;
-          load_pieces(lds0 + i * 1024, lhs_row(first + of_sixteen) + chunk * lhs_step + (piece & 1) * p.lhs.piece1 + (piece >> 1 & 1) * p.lhs.piece2);
+          load_pieces(lds0 + i * 1024, rows[i] + chunk * lhs_step + (piece & 1) * p.lhs.piece1 + (piece >> 1 & 1) * p.lhs.piece2);
 #pragma unroll
           for (int j = 0; j < RT; ++j)
             load_pieces(lds0 + (1 + j) * 4096 + i * 1024, down_row(first_rank + 16 * j + of_sixteen) + (int64_t)chunk * 64 + (piece & 3) * 16);
@@ -188,7 +286,7 @@ __global__ __launch_bounds__(64 * kWaves<RT>) void adapter_down_kernel(const Ada
       // What K has behind its last whole chunk, zeros behind it.
       if (rest != 0 && split == p.splits - 1 && wave == (int)((to - from) % WAVES)) {
         const int exist = (int)rest - 8 * g;
-        const uint4 a = last_piece(lhs_row(first + r) + full * lhs_step + (g & 1) * p.lhs.piece1 + (g >> 1) * p.lhs.piece2, exist);
+        const uint4 a = last_piece(lhs_row(row) + full * lhs_step + (g & 1) * p.lhs.piece1 + (g >> 1) * p.lhs.piece2, exist);
 #pragma unroll
         for (int j = 0; j < RT; ++j)
           acc[j] = mfma16_16<T>(last_piece(down_row(first_rank + 16 * j + r) + (int64_t)full * 64 + 16 * g, exist), a, acc[j]);
@@ -207,7 +305,7 @@ __global__ __launch_bounds__(64 * kWaves<RT>) void adapter_down_kernel(const Ada
         if ((same >> r & 1) != 0 && rank < p.pitch) *(p16_v4f32*)(p.sums + ((int64_t)split * p.lhs.rows + first + r) * p.pitch + rank) = v;
       }
       __syncthreads();
-    });
+    }, no_zeros);
   }
 }
 
@@ -262,30 +360,28 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterProduct p)
     // unit = (tile * slots + slot) * parts + block of columns
     const uint32_t upper = divide(unit, p.parts, p.parts_reciprocal), part = unit - upper * p.parts;
     const uint32_t tile = divide(upper, p.slots, p.slots_reciprocal), slot = upper - tile * p.slots;
-    const uint32_t first = tile * 16, first_col = (part * 4 + wave) * (16 * F * p.turns);
+    const uint32_t first_col = (part * 4 + wave) * (16 * F * p.turns);
     const uint32_t end_col = first_col + 16 * F * p.turns < p.cols ? first_col + 16 * F * p.turns : p.cols;
-    const uint32_t row = first + r < p.lhs.rows ? first + r : p.lhs.rows - 1;
-    uint8_t* const out = p.out + layout_row(p.out_at, first) * SIZE;
-    const uint32_t out_row = (uint32_t)(layout_row(p.out_at, row) - layout_row(p.out_at, first));  // elements
-    // Four results, of the fragment at `col`, as they lie in memory.
+    // Four results of a row, of the fragment at `col`, as they lie in memory.
     typedef uint32_t Words __attribute__((ext_vector_type(SIZE)));
-    auto four_at = [&](uint32_t col) {
-      uint8_t* const fragment = out + layout_col(p.out_at, col) * SIZE;
-      return (Words*)__builtin_assume_aligned(fragment + (out_row + 4 * g) * SIZE, 4 * SIZE);
+    auto results_of = [&](uint32_t row) { return p.out + (layout_row(p.out_at, row) + 4 * g) * SIZE; };
+    auto four_at = [&](uint8_t* results, uint32_t col) {
+      return (Words*)__builtin_assume_aligned(results + layout_col(p.out_at, col) * SIZE, 4 * SIZE);
     };
-    auto store_one_by_one = [&](uint32_t from, p16_v4f32 v) {
+    auto store_one_by_one = [&](uint32_t row, uint32_t from, p16_v4f32 v) {
 #pragma unroll 1
       for (int e = 0; e < 4; ++e) {
         const uint32_t col = from + 4 * g + e;
         if (col >= p.cols) continue;
-        const int64_t at = out_row + layout_col(p.out_at, col);
-        const float x = v[e] + (p.accumulate ? element<OUT>(out, at) : 0);
-        if constexpr (OUT == Float::kF32) ((float*)out)[at] = x;
-        else ((uint16_t*)out)[at] = mx_narrow<OUT>(x);
+        const int64_t at = layout_row(p.out_at, row) + layout_col(p.out_at, col);
+        const float x = v[e] + (p.accumulate ? element<OUT>(p.out, at) : 0);
+        if constexpr (OUT == Float::kF32) ((float*)p.out)[at] = x;
+        else ((uint16_t*)p.out)[at] = mx_narrow<OUT>(x);
       }
     };
-    const uint32_t without = of_adapters(p, first, slot, lane, [&](uint32_t of, uint32_t same) {
+    auto add = [&](uint32_t of, uint32_t same, uint32_t row, uint32_t first) {
       const bool mine = (same >> r & 1) != 0;
+      uint8_t* const results = results_of(row);
       const uint8_t* const up = p.up + of * p.up_stride0;
       uint4 w[CHUNKS][F], t[PARTS];
       Words old[F] = {};
@@ -310,7 +406,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterProduct p)
       auto load_old = [&](Words (&to)[F], uint32_t col0) {
 #pragma unroll
         for (int f = 0; f < F; ++f)
-          if (FAST && p.accumulate && mine && col0 + 16 * f < end_col) to[f] = *four_at(col0 + 16 * f);
+          if (FAST && p.accumulate && mine && col0 + 16 * f < end_col) to[f] = *four_at(results, col0 + 16 * f);
       };
       // The sums of ranks from rank0 on, as operands.
       auto take_sums = [&](uint32_t rank0) {
@@ -423,40 +519,57 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterProduct p)
             if (col >= end_col) continue;
             p16_v4f32 v = acc[f] * (MANY ? scale : unit_of_row * scale);
             if constexpr (!FAST) {
-              store_one_by_one(col, v);
+              store_one_by_one(row, col, v);
             } else if constexpr (OUT == Float::kF32) {
               v += __builtin_bit_cast(p16_v4f32, old[f]);
-              *four_at(col) = __builtin_bit_cast(Words, v);
+              *four_at(results, col) = __builtin_bit_cast(Words, v);
             } else {
               float x[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) x[e] = v[e] + mx_widen<OUT>((uint16_t)(old[f][e / 2] >> (16 * (e & 1))));
-              *four_at(col) = Words{mx_narrow_pair<OUT>(x[0], x[1]), mx_narrow_pair<OUT>(x[2], x[3])};
+              *four_at(results, col) = Words{mx_narrow_pair<OUT>(x[0], x[1]), mx_narrow_pair<OUT>(x[2], x[3])};
             }
           }
           if (turn + 1 < p.turns) load_old(old, col0 + 16 * F);
         }
       }
-    });
-    if (!p.accumulate && slot == 0 && (without >> r & 1) != 0 && first + r < p.lhs.rows) {
+    };
+    of_adapters(p, tile, slot, lane, add, [&](uint32_t without, uint32_t row) {
+      if (p.accumulate || (without >> r & 1) == 0) return;
+      uint8_t* const results = results_of(row);
       for (uint32_t col = first_col; col < end_col; col += 16) {
-        if constexpr (!FAST) store_one_by_one(col, p16_v4f32{0, 0, 0, 0});
-        else *four_at(col) = Words(0);
+        if constexpr (!FAST) store_one_by_one(row, col, p16_v4f32{0, 0, 0, 0});
+        else *four_at(results, col) = Words(0);
       }
-    }
+    });
   }
 }
 
+// Whether rows are put in order, and tiles: what adapters of sixteen rows in any order have to be read, less what each adapter's own tiles
+// have, is 48 MiB and more, some 8 us; the launch takes 4 more (of which rows in runs have nothing: no host knows their order).
+struct Tiles { int64_t most; bool ordered; };
+Tiles tiles_of(int64_t rows, int64_t count, int64_t depth, int64_t cols, int64_t rank) {
+  const int64_t sixteens = (rows + 15) / 16, own = rows / 16 + (count + 1 < rows ? count + 1 : rows);
+  if (rows <= 16 || rows > 65536 || count < 2 || count > kMostOrdered) return {sixteens, false};
+  // (Of `count` adapters sixteen rows have count (1 - (1 - 1 / count)^16) in the mean.)
+  double others = 1;
+  for (int i = 0; i < 16; ++i) others *= 1 - 1 / (double)count;
+  const double saved = (double)sixteens * (double)count * (1 - others) - (double)own;
+  if (saved * 2 * (double)rank * (double)(depth + cols) < (double)(48 << 20)) return {sixteens, false};
+  return {own, true};
+}
 // How many parts K is split into: as many as leave every wavefront four chunks, while two workgroups, as many as a compute unit's LDS
 // holds, come to each. (2000 rows, rank 64, K 4096: 3 parts 14.9 us, 4 12.6, 6 15.3.)
-uint32_t splits_of(int64_t rows, int64_t depth, int64_t rank) {
+uint32_t splits_of(int64_t rows_of_tiles, int64_t depth, int64_t rank) {
   const int waves = rank > 32 ? kWaves<kFragments> : kWaves<1>;
-  const int64_t tiles = (rows + 15) / 16 * ((rank + 16 * kFragments - 1) / (16 * kFragments));
+  const int64_t tiles = rows_of_tiles * ((rank + 16 * kFragments - 1) / (16 * kFragments));
   const int64_t most = depth / 32 / (4 * waves), wanted = 512 / tiles;
   const int64_t s = most < wanted ? most : wanted;
   return (uint32_t)(s < 1 ? 1 : s);
 }
 int64_t pitch_of(int64_t rank) { return (rank + 31) / 32 * 32; }
+// (Fewer than 2^31 rows, and 2^15 ranks; few splits where there are many.)
+int64_t sums_bytes(int64_t rows, int64_t rank, int64_t splits) { return (rows * pitch_of(rank) * 4 * splits + 255) / 256 * 256; }
 
 bool multiple(const void* p, int64_t to) { return (uintptr_t)p % to == 0; }
 
@@ -464,8 +577,8 @@ bool multiple(const void* p, int64_t to) { return (uintptr_t)p % to == 0; }
 // with 2048, 4096 and 8192 wavefronts: 64 rows of 64 adapters x 14336, rank 16, 18.0, 19.3, 24.4 us; 2000 rows of 12 in runs x 4096, rank 64,
 // 37.9, 33.7, 33.9; 256 of 40 x 8192, rank 32, 38.2, 34.0, 36.7; 40 of 16 x 11008, rank 16, 13.7, 13.4, 15.0.)
 int up_fragments(int64_t rank) { return rank <= 32 ? 4 : 2; }
-uint32_t turns_of(int64_t rows, int64_t slots, int64_t cols, int64_t rank) {
-  const int64_t across = (cols + 16 * up_fragments(rank) - 1) / (16 * up_fragments(rank)), t = (rows + 15) / 16 * slots * across / 4096;
+uint32_t turns_of(int64_t tiles, int64_t slots, int64_t cols, int64_t rank) {
+  const int64_t across = (cols + 16 * up_fragments(rank) - 1) / (16 * up_fragments(rank)), t = tiles * slots * across / 4096;
   return (uint32_t)(t < 1 ? 1 : t > 8 ? 8 : t);
 }
 int64_t column_parts(const AdapterProduct& p) {
@@ -479,7 +592,9 @@ bool as_product(const AdapterArgs& a, AdapterProduct* p) {
   if (a.count == 0 || depth > 0x7FFFFFFF || cols > 0x7FFFFFFF - 512) return false;
   if (!as_operand16(a.lhs, a.lhs_stride0, a.M, a.M0, a.K, a.K0, &p->lhs)) return false;
   if (!multiple(a.down, 16) || (a.count > 1 && a.down_stride0 % 8 != 0) || (a.rank > 1 && a.down_stride1 % 8 != 0)) return false;
-  const int64_t rows = a.M * a.M0, tiles = (rows + 15) / 16;
+  const int64_t rows = a.M * a.M0;
+  const Tiles t = tiles_of(rows, a.count, depth, cols, a.rank);
+  p->tiles = (uint32_t)t.most;
   p->down = a.down; p->up = a.up;
   p->down_stride0 = 2 * a.down_stride0; p->down_stride1 = 2 * a.down_stride1;
   p->up_stride0 = 2 * a.up_stride0; p->up_stride1 = 2 * a.up_stride1;
@@ -491,26 +606,28 @@ bool as_product(const AdapterArgs& a, AdapterProduct* p) {
   p->out_type = a.out_type;
   p->depth = (uint32_t)depth; p->rank = (uint32_t)a.rank; p->count = (uint32_t)a.count; p->cols = (uint32_t)cols;
   p->pitch = (uint32_t)pitch_of(a.rank);
-  p->splits = splits_of(rows, depth, a.rank);
+  p->splits = splits_of(t.most, depth, a.rank);
+  const int64_t sums = sums_bytes(rows, a.rank, p->splits);
+  p->heads = t.ordered ? (const uint4*)(a.workspace + sums) : nullptr;
+  p->ids = t.ordered ? (const uint32_t*)(a.workspace + sums + 16 * t.most) : nullptr;
   p->accumulate = a.accumulate;
   const int e = float_bytes(a.out_type);
   p->runs = runs_of(p->out_at, a.out, a.M, e, 16, 4 * e);
-  // (32 bits from an adapter's start to a column of `up`, and from a tile's first result to its last.)
-  if (p->up_stride1 > (1ll << 31) / cols || (a.M > 1 && a.out_stride0 > (1ll << 28) / 17) || (int64_t)p->out_at.tile * a.N > (1ll << 28)) return false;
+  // (32 bits from an adapter's start to a column of `up`.)
+  if (p->up_stride1 > (1ll << 31) / cols) return false;
   // Adapters of a tile side by side where there are few tiles.
-  const int64_t slots = 128 / tiles, most = a.count < 16 ? a.count : 16;
+  const int64_t slots = t.ordered ? 1 : 128 / t.most, most = a.count < 16 ? a.count : 16;
   p->slots = (uint32_t)(slots < 1 ? 1 : slots > most ? most : slots);
   p->slots_reciprocal = reciprocal_of(p->slots);
-  p->turns = turns_of(rows, p->slots, cols, a.rank);
+  p->turns = turns_of(t.most, p->slots, cols, a.rank);
   return true;
 }
 
 // One launch over tiles * slots * parts pieces of work.
 hipError_t launch_units(void (*kernel)(const AdapterProduct), AdapterProduct p, int64_t parts, unsigned threads, unsigned lds, hipStream_t stream) {
-  const int64_t tiles = ((int64_t)p.lhs.rows + 15) / 16;
   p.parts = (uint32_t)parts;
   p.parts_reciprocal = reciprocal_of(p.parts);
-  p.units = (uint32_t)(tiles * p.slots * parts);
+  p.units = (uint32_t)(p.tiles * (int64_t)p.slots * parts);
   return launch_kernel(kernel, p.units < (1u << 22) ? p.units : 1u << 22, threads, lds, stream, p);
 }
 
@@ -548,7 +665,7 @@ hipError_t launch_up(const AdapterProduct& p, hipStream_t stream) {
 
 // Whether the pieces of work of both launches are fewer than 2^31.
 bool countable(const AdapterProduct& p) {
-  const int64_t tiles = ((int64_t)p.lhs.rows + 15) / 16, blocks = (p.rank + 15) / 16, most = (1ll << 31) / (tiles * p.slots);
+  const int64_t blocks = (p.rank + 15) / 16, most = (1ll << 31) / ((int64_t)p.tiles * p.slots);
   return blocks * p.splits < most && column_parts(p) < most;
 }
 
@@ -556,10 +673,10 @@ bool countable(const AdapterProduct& p) {
 
 int64_t adapter_workspace(const AdapterArgs& a) {
   if (a.count == 0) return 0;
-  const int64_t rows = a.M * a.M0;  // fewer than 2^31, and 2^15 ranks
-  int64_t bytes;
-  if (__builtin_mul_overflow(rows * pitch_of(a.rank) * 4, (int64_t)splits_of(rows, a.K * a.K0, a.rank), &bytes) || bytes > INT64_MAX - 256) return -1;
-  return (bytes + 255) / 256 * 256;
+  const int64_t rows = a.M * a.M0, depth = a.K * a.K0, cols = a.N * a.N0;
+  const Tiles t = tiles_of(rows, a.count, depth, cols, a.rank);
+  // The rank sums; of rows in order 16 bytes for a tile's head and 64 for its rows.
+  return sums_bytes(rows, a.rank, splits_of(t.most, depth, a.rank)) + (t.ordered ? (80 * t.most + 255) / 256 * 256 : 0);
 }
 
 hipError_t launch_adapter_mmt4d(const AdapterArgs& a, hipStream_t stream, const char** name) {
@@ -567,6 +684,11 @@ hipError_t launch_adapter_mmt4d(const AdapterArgs& a, hipStream_t stream, const 
   if (as_product(a, &p) && countable(p)) {
     *name = "adapter_mmt4d";
     const bool f16 = a.type == Float::kF16;
+    if (p.heads) {
+      const OrderArgs o = {p.index, (uint4*)p.heads, (uint32_t*)p.ids, p.lhs.rows, p.count, p.tiles};
+      const hipError_t e = launch_kernel(adapter_order_kernel, 1, kOrderThreads, 0, stream, o);
+      if (e != hipSuccess) return e;
+    }
     const hipError_t e = f16 ? launch_down<Float::kF16>(p, stream) : launch_down<Float::kBf16>(p, stream);
     return e != hipSuccess ? e : f16 ? launch_up<Float::kF16>(p, stream) : launch_up<Float::kBf16>(p, stream);
   }

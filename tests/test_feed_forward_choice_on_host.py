@@ -8,7 +8,7 @@ from feed_forward_kernels import GATED, GATED_TIMES, LHS_GRADS, WEIGHT_GRADS, WE
 from feed_forward_reference import up
 from host_launches import recorder  # noqa: F401
 from iree_amd import abi
-from test_gpu_adapter_mmt4d import PROBLEMS as ADAPTERS
+from test_gpu_adapter_mmt4d import ORDERED, PROBLEMS as ADAPTERS
 from test_gpu_gated_backward import PROBLEMS as BACKWARD, SPLIT
 
 GIB = 1 << 30
@@ -128,3 +128,14 @@ def test_every_adapter_kernel_is_tested(recorder, type, out):  # noqa: F811
     forms = {(half, chunks, fast, many) for half, chunks, many in (("1", "1", "0"), ("0", "1", "0"), ("0", "2", "0"), ("0", "2", "1")) for fast in "01"}
     assert forms == {x for x in picked if isinstance(x, tuple)}
     assert any("adapter_up_generic" in x for x in picked)
+
+
+def test_many_rows_of_few_adapters_are_put_in_order(recorder):  # noqa: F811
+    for m, n, k, rank, count, tile, _ in ORDERED:
+        adapters(recorder, m, n, k, rank, count, tile, "bf16", "f32")
+        assert recorder.lib.recorded_launches() == 3, (m, n, k, rank, count, tile)
+    # Few rows, as many adapters as rows, little to read, one adapter, and more than have numbers in LDS.
+    for m, n, k, rank, count in ((16, 14336, 4096, 64, 2), (64, 14336, 4096, 16, 64), (40, 11008, 4096, 16, 16), (300, 300, 300, 16, 3),
+                                 (4096, 4096, 4096, 64, 1), (4096, 4096, 4096, 64, 2048)):
+        adapters(recorder, m, n, k, rank, count, (1, 16, 16), "bf16", "f32")
+        assert recorder.lib.recorded_launches() == 2, (m, n, k, rank, count)

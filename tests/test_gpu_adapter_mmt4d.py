@@ -74,6 +74,35 @@ def test_alone_and_without_scales(gpu_lib, m, n, k, rank, count, tile, order, ou
     check_case(gpu_lib, m, n, k, rank, count, tile, "bf16", "bf16" if out == "same" else out, order, accumulate=False, scaled=False)
 
 
+# Many rows of few adapters, which are put in order first: all sorts of tiles, ranks and columns, rows of one adapter, of few and of many.
+ORDERED = [
+    (1000, 1000, 1024, 64, 12, (1, 16, 16), "mixed"), (905, 520, 2000, 100, 30, (1, 16, 8), "mixed"), (704, 2048, 512, 64, 9, (16, 16, 16), "mixed"),
+    (2100, 300, 1500, 64, 500, (1, 4, 16), "mixed"), (1500, 1040, 2050, 16, 21, (4, 8, 16), "runs"), (6000, 512, 512, 30, 4, (1, 16, 32), "one"),
+    (3000, 400, 3000, 32, 2047, (1, 16, 16), "mixed"), (500, 2000, 3104, 64, 7, (1, 1, 1552), "mixed"),
+]
+
+
+@pytest.mark.parametrize("accumulate", [True, False])
+@pytest.mark.parametrize("type,out", [("bf16", "bf16"), ("f16", "f32"), ("bf16", "f32")])
+@pytest.mark.parametrize("m,n,k,rank,count,tile,order", ORDERED)
+def test_many_rows_of_few_adapters(gpu_lib, m, n, k, rank, count, tile, order, type, out, accumulate):  # noqa: F811
+    check_case(gpu_lib, m, n, k, rank, count, tile, type, out, order, accumulate)
+
+
+def test_rows_in_order_give_the_same_bits_and_strange_indices_name_nobody(gpu_lib):  # noqa: F811
+    rng, x, down, up_, index, scales = inputs(5, 1000, 512, 2048, 64, 12, (1, 16, 16), "bf16", "mixed")
+    run = lambda i: ref.run_adapters(gpu_lib, x, down, up_, i, scales, (1, 16, 16), "bf16", "f32")[0]  # noqa: E731
+    first = run(index)
+    for _ in range(3):
+        np.testing.assert_array_equal(run(index), first)
+    others = index.copy()
+    others[::3] = rng.choice([-2 ** 31, -1, 12, 13, 2 ** 31 - 1], others[::3].size)
+    got = run(others)
+    np.testing.assert_array_equal(got[1::3], first[1::3])
+    assert not got[::3].any()
+    assert not run(np.full_like(index, 12)).any()
+
+
 @pytest.mark.parametrize("gap,offset", [(8, 8), (16, 24), (3, 5)])
 @pytest.mark.parametrize("m,n,k,rank,tile", [(1, 100, 300, 16, (1, 16, 16)), (40, 100, 384, 8, (1, 16, 16)), (48, 80, 384, 12, (16, 16, 16)),
                                              (300, 200, 512, 64, (1, 1, 32))])

@@ -84,7 +84,7 @@ def captured(lib, *calls):
     return graph
 
 
-@pytest.mark.parametrize("m,rank,count", [(1, 16, 3), (50, 16, 7), (300, 64, 5)])
+@pytest.mark.parametrize("m,rank,count", [(1, 16, 3), (50, 16, 7), (300, 64, 5), (2000, 64, 9)])
 def test_a_captured_call_takes_the_adapters_that_rows_have_at_replay(gpu_lib, m, rank, count):  # noqa: F811
     a = Adapters(gpu_lib, m, m, 320, 2048, rank, count)
     graph = captured(gpu_lib, a)
@@ -119,7 +119,7 @@ def test_split_sums_replayed(gpu_lib, m, n, k):  # noqa: F811
 
 
 def test_calls_at_once(gpu_lib):  # noqa: F811
-    calls = [Adapters(gpu_lib, 1, 64, 4096, 2048, 16, 20), Adapters(gpu_lib, 2, 500, 1024, 1024, 64, 5), Backward(gpu_lib, 3, 100, 2048, 512),
+    calls = [Adapters(gpu_lib, 1, 64, 4096, 2048, 16, 20), Adapters(gpu_lib, 2, 500, 1024, 1024, 64, 5), Adapters(gpu_lib, 5, 2000, 1024, 1024, 64, 7), Backward(gpu_lib, 3, 100, 2048, 512),
              Backward(gpu_lib, 4, 700, 512, 512)]
     wants = []
     for call in calls:
