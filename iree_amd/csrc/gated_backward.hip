@@ -173,6 +173,7 @@ Choice choose(const Times* times, int64_t rows, int64_t cols, int64_t chunks, in
     const int64_t of_one = (rows + t.rows - 1) / t.rows * ((cols + t.cols - 1) / t.cols) * copies;
     const Times& of = times[i];
     for (int64_t splits = 1; splits <= most_splits; ++splits) {
+      if (splits > 1 && of_one * (splits - 1) > 512) break;  // (all compute units had two)
       const int64_t tiles = of_one * splits, rounds = (tiles + 255) / 256;
       if (tiles > (1 << 23)) continue;  // (a grid has fewer than 2^32 threads)
       const float in_turn = (float)chunks / (float)splits * (of.two == 0 ? rounds * of.one : (rounds >> 1) * of.two + (rounds & 1) * of.one);
@@ -216,6 +217,7 @@ Choice choose_both(const Sizes& s, int64_t copies) {
   if (of_lhs * most + of_weights > (1 << 23)) return best;
   const float all = ((float)of_lhs * (float)lhs_chunks + (float)of_weights * (float)weight_chunks) / 256 * kBothBusy;
   for (int64_t splits = 1; splits <= most; ++splits) {
+    if (splits > 1 && of_lhs * (splits - 1) + of_weights > 1024) break;
     const int64_t tiles = of_lhs * splits + of_weights;
     const float longer = lhs_chunks > splits * weight_chunks ? (float)lhs_chunks / (float)splits : (float)weight_chunks;
     const float in_turn = longer * (tiles > 256 ? kBothTwo : kBothOne), steps = in_turn > all ? in_turn : all;
