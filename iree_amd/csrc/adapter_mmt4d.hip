@@ -141,26 +141,57 @@ __device__ __forceinline__ void of_adapters(const AdapterProduct& p, uint32_t ti
   zeros(without, row);
 }
 
-// Rows in the order of their adapters, those without one behind them, and the tiles that this makes, by one workgroup: how many rows each
-// adapter has, where its first one and its first tile come, then each row to its place. Adapters' numbers are in LDS.
+// Rows in the order of their adapters, those without one behind them, and the tiles that this makes, by one workgroup: each row takes a
+// number among its adapter's, then where an adapter's first row and first tile come makes that a place. Adapters' counts are in LDS; a
+// wavefront's rows of one adapter take their numbers at once while they are many. The first rows of a thread stay in registers, others'
+// numbers wait in memory. (2000 rows, 12 adapters in runs: 4.9 us; one row at a time, and twice over the indices, 7.3.)
 constexpr uint32_t kMostOrdered = 2047, kOrderThreads = 1024;
 struct OrderArgs {
   const int32_t* index;
   uint4* heads;
   uint32_t* ids;
+  uint32_t* numbers;            // of rows; what the rank sums take later
   uint32_t rows, count, tiles;  // tiles: as many as there may be
 };
 __global__ __launch_bounds__(kOrderThreads) void adapter_order_kernel(const OrderArgs p) {
-  __shared__ uint32_t rows_of[kMostOrdered + 1], taken[kMostOrdered + 1], first_row[kMostOrdered + 1], first_tile[kMostOrdered + 1];
+  __shared__ uint32_t rows_of[kMostOrdered + 1], first_row[kMostOrdered + 1], first_tile[kMostOrdered + 1];
   __shared__ uint32_t wave_rows[kOrderThreads / 64], wave_tiles[kOrderThreads / 64];
+  constexpr uint32_t KEPT = 4;
   const uint32_t thread = threadIdx.x, lane = thread & 63, wave = thread >> 6, entries = p.count + 1;
   auto adapter_of = [&](uint32_t row) {
-    const int32_t i = p.index[row];
+    const int32_t i = p.index[row < p.rows ? row : p.rows - 1];
     return i < 0 || (uint32_t)i >= p.count ? p.count : (uint32_t)i;
   };
-  for (uint32_t a = thread; a < entries; a += kOrderThreads) rows_of[a] = taken[a] = 0;
+  // (By all lanes of a wavefront.)
+  auto number_of = [&](uint32_t adapter, bool is_row) {
+    uint64_t todo = __builtin_amdgcn_ballot_w64(is_row);
+    uint32_t number = 0;
+    for (bool many = true; many && todo != 0;) {
+      const uint32_t leader = (uint32_t)__builtin_ctzll(todo), of = (uint32_t)__builtin_amdgcn_readlane((int)adapter, (int)leader);
+      const bool same = is_row && adapter == of;
+      const uint64_t all = __builtin_amdgcn_ballot_w64(same);
+      uint32_t base = 0;
+      if (lane == leader) base = atomicAdd(&rows_of[of], (uint32_t)__builtin_popcountll(all));
+      base = (uint32_t)__builtin_amdgcn_readlane((int)base, (int)leader);
+      const uint32_t in_front = __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+      number = same ? base + in_front : number;
+      todo &= ~all;
+      many = __builtin_popcountll(all) >= 16;  // (else rows are mixed, and hinder each other little)
+    }
+    if ((todo >> lane & 1) != 0) number = atomicAdd(&rows_of[adapter], 1u);
+    return number;
+  };
+  uint32_t adapters[KEPT], numbers[KEPT];
+#pragma unroll
+  for (uint32_t i = 0; i < KEPT; ++i) adapters[i] = adapter_of(i * kOrderThreads + thread);
+  for (uint32_t a = thread; a < entries; a += kOrderThreads) rows_of[a] = 0;
   __syncthreads();
-  for (uint32_t row = thread; row < p.rows; row += kOrderThreads) atomicAdd(&rows_of[adapter_of(row)], 1u);
+#pragma unroll
+  for (uint32_t i = 0; i < KEPT; ++i) numbers[i] = number_of(adapters[i], i * kOrderThreads + thread < p.rows);
+  for (uint32_t at = KEPT * kOrderThreads; at < p.rows; at += kOrderThreads) {
+    const uint32_t row = at + thread, number = number_of(adapter_of(row), row < p.rows);
+    if (row < p.rows) p.numbers[row] = number;
+  }
   __syncthreads();
   // Two adapters a thread; sums over the threads in front of it.
   constexpr uint32_t EACH = (kMostOrdered + 1) / kOrderThreads;
@@ -203,11 +234,15 @@ __global__ __launch_bounds__(kOrderThreads) void adapter_order_kernel(const Orde
     tile_at += (rows[e] + 15) >> 4;
   }
   __syncthreads();
-  for (uint32_t row = thread; row < p.rows; row += kOrderThreads) {
-    const uint32_t a = adapter_of(row), n = atomicAdd(&taken[a], 1u), tile = first_tile[a] + (n >> 4);
+  auto place = [&](uint32_t row, uint32_t a, uint32_t n) {
+    if (row >= p.rows) return;
+    const uint32_t tile = first_tile[a] + (n >> 4), left = rows_of[a] - n;
     p.ids[tile * 16 + (n & 15)] = row;
-    if ((n & 15) == 0) p.heads[tile] = make_uint4(a, first_row[a] + n, rows_of[a] - n < 16 ? rows_of[a] - n : 16, 0);
-  }
+    if ((n & 15) == 0) p.heads[tile] = make_uint4(a, first_row[a] + n, left < 16 ? left : 16, 0);
+  };
+#pragma unroll
+  for (uint32_t i = 0; i < KEPT; ++i) place(i * kOrderThreads + thread, adapters[i], numbers[i]);
+  for (uint32_t row = KEPT * kOrderThreads + thread; row < p.rows; row += kOrderThreads) place(row, adapter_of(row), p.numbers[row]);
   for (uint32_t tile = all_tiles + thread; tile < p.tiles; tile += kOrderThreads) p.heads[tile] = make_uint4(0, 0, 0, 0);
 }
 
@@ -546,9 +581,9 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterProduct p)
 }
 
 // Whether rows are put in order, and tiles: what adapters of sixteen rows in any order have to be read, less what each adapter's own tiles
-// have, is 16 MiB and more. Rows mixed at random then take what rows in runs do and the launch's 3 us (2000 x 4096 x 4096, 12 adapters, rank 64,
+// have, is 16 MiB and more. Rows mixed at random then take what rows in runs do and 1 to 3 us for the launch (2000 x 4096 x 4096, 12 adapters, rank 64,
 // 159 -> 40 us, 256 x 8192 x 4096, 40 adapters, rank 32, 35 -> 19, 4000 x 11008 x 4096, 30 adapters, rank 32, 487 -> 137); rows that come in
-// runs, and no host knows whether they do, 34 -> 37, 23 -> 17 and 115 -> 112. In 40 problems of 5 to 100 MiB mixed rows take 11 us less in the
+// runs, and no host knows whether they do, 34 -> 35, 23 -> 17 and 115 -> 108. In 40 problems of 5 to 100 MiB mixed rows take 11 us less in the
 // mean from 16 MiB on, and rows in runs 0.2 more; below it is 0.7 less and 1.4 more.
 struct Tiles { int64_t most; bool ordered; };
 Tiles tiles_of(int64_t rows, int64_t count, int64_t depth, int64_t cols, int64_t rank) {
@@ -688,7 +723,7 @@ hipError_t launch_adapter_mmt4d(const AdapterArgs& a, hipStream_t stream, const 
     *name = "adapter_mmt4d";
     const bool f16 = a.type == Float::kF16;
     if (p.heads) {
-      const OrderArgs o = {p.index, (uint4*)p.heads, (uint32_t*)p.ids, p.lhs.rows, p.count, p.tiles};
+      const OrderArgs o = {p.index, (uint4*)p.heads, (uint32_t*)p.ids, (uint32_t*)p.sums, p.lhs.rows, p.count, p.tiles};
       const hipError_t e = launch_kernel(adapter_order_kernel, 1, kOrderThreads, 0, stream, o);
       if (e != hipSuccess) return e;
     }

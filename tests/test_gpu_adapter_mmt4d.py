@@ -79,6 +79,7 @@ ORDERED = [
     (1000, 1000, 1024, 64, 12, (1, 16, 16), "mixed"), (905, 520, 2000, 100, 30, (1, 16, 8), "mixed"), (704, 2048, 512, 64, 9, (16, 16, 16), "mixed"),
     (2100, 300, 1500, 64, 500, (1, 4, 16), "mixed"), (1500, 1040, 2050, 16, 21, (4, 8, 16), "runs"), (6000, 512, 512, 30, 4, (1, 16, 32), "one"),
     (3000, 400, 3000, 32, 2047, (1, 16, 16), "mixed"), (500, 2000, 3104, 64, 7, (1, 1, 1552), "mixed"),
+    (9001, 256, 256, 16, 40, (1, 16, 16), "mixed"), (5000, 256, 256, 16, 5, (1, 16, 16), "runs"),
 ]
 
 
