@@ -3,7 +3,7 @@
 #define IREE_AMD_CSRC_GATED_MMT4D_BLOCK_H_
 
 #include "gated_mmt4d.h"
-#include "product16_block.h"
+#include "product16_lines.h"
 
 namespace uk {
 namespace {
@@ -23,6 +23,14 @@ hipError_t launch_gated_block(const GatedProduct& g, int tile, hipStream_t strea
   // tiles; where other calls have filled the caches in between, 40 x 11008 x 4096 (180 MB) 38.1 -> 35.1, 64 x 14336 x 4096 47.1 -> 43.4 and
   // 128 x 11008 x 4096 53.2 -> 50.2. The same call made again at once finds its weights there: 29 -> 35, 36 -> 43 and 33 -> 49.
   const bool stream_rhs = g.lhs.rows <= 128 && 6 * (int64_t)g.gate.rows * g.depth > (256ll << 20);
+  if (whole_lines(g.lhs, g.depth)) {
+    switch (tile) {
+      case 0: return launch_lines_tile<T, 4, 4>(p, stream);
+      case 1: return launch_lines_tile<T, 4, 3>(p, stream);
+      case 2: return launch_lines_tile<T, 3, 3>(p, stream);
+      case 3: return launch_lines_tile<T, 3, 4>(p, stream);
+    }
+  }
   switch (tile) {  // kGatedTiles
     case 0: return launch_block_tile<T, 4, 4, 4>(p, stream);
     case 1: return launch_block_tile<T, 4, 3, 4>(p, stream);

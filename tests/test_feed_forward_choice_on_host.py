@@ -4,7 +4,7 @@ import re
 
 import pytest
 
-from feed_forward_kernels import GATED, GATED_TIMES, LHS_GRADS, WEIGHT_GRADS, WEIGHT_GRADS_TIMES
+from feed_forward_kernels import GATED, GATED_LINES, GATED_TIMES, LHS_GRADS, WEIGHT_GRADS, WEIGHT_GRADS_TIMES
 from feed_forward_reference import up
 from host_launches import recorder  # noqa: F401
 from iree_amd import abi
@@ -50,6 +50,16 @@ def test_every_gated_kernel_is_picked(recorder, type):  # noqa: F811
         assert gated(recorder, m, n, k, tile, type)[1] == "gated_mmt4d_" + kernel, (m, n, k, tile)
         picked.add(kernel)
     assert len(picked) == 17
+
+
+def test_rows_of_whole_lines(recorder):  # noqa: F811
+    for kernel, m, n, k, tile in GATED_LINES:
+        symbol, name = gated(recorder, m, n, k, tile)
+        assert "product16_lines_kernel" in symbol and name == "gated_mmt4d_" + kernel, (m, n, k, tile)
+    assert len({x[0] for x in GATED_LINES}) == 4
+    # (K not a multiple of 64, and rows in tiles)
+    for m, n, k, tile in ((1371, 3273, 96, (1, 16, 16)), (1371, 3273, 130, (1, 16, 8)), (2048, 4096, 512, (16, 16, 16))):
+        assert "product16_block_kernel" in gated(recorder, m, n, k, tile)[0]
 
 
 @pytest.mark.parametrize("type", ["bf16", "f16"])
@@ -105,7 +115,8 @@ def test_split_sums_are_tested(recorder):  # noqa: F811
 def test_weights_past_the_caches(recorder, m, n, k, streams):  # noqa: F811
     kernel, _ = gated(recorder, m, n, k, (1, 16, 16))
     past = re.search(r"few_kernelILNS_5FloatE\dELi\dELi\dELb(\d)|block_kernelILNS_5FloatE\dELi\dELi\dELi\dELb(\d)", kernel)
-    assert (past[1] or past[2]) == str(int(streams)), kernel
+    assert (past is not None and (past[1] or past[2]) == "1") == streams, kernel
+
 
 
 def adapters(recorder, m, n, k, rank, count, tile, type, out):  # noqa: F811
