@@ -23,12 +23,19 @@ hipError_t launch_gated_block(const GatedProduct& g, int tile, hipStream_t strea
   // tiles; where other calls have filled the caches in between, 40 x 11008 x 4096 (180 MB) 38.1 -> 35.1, 64 x 14336 x 4096 47.1 -> 43.4 and
   // 128 x 11008 x 4096 53.2 -> 50.2. The same call made again at once finds its weights there: 29 -> 35, 36 -> 43 and 33 -> 49.
   const bool stream_rhs = g.lhs.rows <= 128 && 6 * (int64_t)g.gate.rows * g.depth > (256ll << 20);
+  // Row-major rows that are whole cache lines are loaded by whole lines in the four largest tiles, one workgroup of which fits a compute
+  // unit, and in the two others that still fit it twice with the longer ring: 512 x 11008 x 4096 in 256x96 tiles 100 -> 85 us,
+  // 4096 x 11008 x 4096 in 256x128 ones 624 -> 592, 300 x 11008 x 4096 in 192x96 72 -> 65, 128 x 11008 x 4096 in 64x96 50.3 -> 46.1,
+  // 400 x 4096 x 4096 in 128x64 37.2 -> 35.7. 64x64 tiles won 43.8 -> 40.2 for 64 rows but lost 35.2 -> 36.2 for 40 and 23.5 -> 24.3
+  // for 77, 64x32 ones gained nothing where they are taken.
   if (whole_lines(g.lhs, g.depth)) {
     switch (tile) {
       case 0: return launch_lines_tile<T, 4, 4>(p, stream);
       case 1: return launch_lines_tile<T, 4, 3>(p, stream);
       case 2: return launch_lines_tile<T, 3, 3>(p, stream);
       case 3: return launch_lines_tile<T, 3, 4>(p, stream);
+      case 6: return stream_rhs ? launch_lines_tile<T, 2, 2, true>(p, stream) : launch_lines_tile<T, 2, 2>(p, stream);
+      case 8: return stream_rhs ? launch_lines_tile<T, 1, 3, true>(p, stream) : launch_lines_tile<T, 1, 3>(p, stream);
     }
   }
   switch (tile) {  // kGatedTiles
