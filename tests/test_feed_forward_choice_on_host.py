@@ -59,9 +59,10 @@ def test_rows_of_whole_lines(recorder):  # noqa: F811
         form = re.search(r"product16_lines_kernelILNS_5FloatE\dELi\dELi\dELb(\d)", symbol)
         assert form and name == "gated_mmt4d_" + kernel, (m, n, k, tile)
         picked.add((kernel, form[1]))
-    assert len(picked) == 8  # (two of the six with weights past the caches too)
-    # (K not a multiple of 64, and rows in tiles)
-    for m, n, k, tile in ((1371, 3273, 96, (1, 16, 16)), (1371, 3273, 130, (1, 16, 8)), (2048, 4096, 512, (16, 16, 16))):
+    assert len(picked) == 11  # (two of the nine with weights past the caches too)
+    # (K not a multiple of 64, rows in tiles, and two workgroups to a compute unit)
+    for m, n, k, tile in ((1371, 3273, 96, (1, 16, 16)), (1371, 3273, 130, (1, 16, 8)), (2048, 4096, 512, (16, 16, 16)),
+                          (1573, 4882, 128, (1, 16, 16)), (914, 8341, 64, (1, 16, 16)), (314, 12557, 64, (1, 16, 16))):
         assert "product16_block_kernel" in gated(recorder, m, n, k, tile)[0]
 
 
