@@ -612,7 +612,10 @@ void iree_uk_mi355x_gated_mmt4d_p(const iree_uk_mi355x_gated_mmt4d_params_t* par
  * The result's type of the type flag is that of out_grad and of all gradients;
  * with ACCUMULATE the gradients of the weights are added to what they hold. dg
  * and du are rounded to the operands' type in between, which the matrix
- * instructions take; the sums over them are in f32 and rounded once. A gradient
+ * instructions take, whatever the result's type: each is within 2^-8 (bf16) or
+ * 2^-11 (f16) of itself, or in f16 within 2^-39 of the call's largest, which a
+ * power of two brings into f16's range first, however large or small they are.
+ * The sums over them are in f32 and rounded once. A gradient
  * whose buffer is NULL is not computed, and gate and up are not read without
  * lhs_grad, nor lhs without the gradients of the weights. The same call gives
  * the same bits. The fast kernels ask gate and up, for lhs_grad, and lhs, for the
@@ -620,10 +623,11 @@ void iree_uk_mi355x_gated_mmt4d_p(const iree_uk_mi355x_gated_mmt4d_params_t* par
  * row tall: of 8 columns in all), and to be aligned as above.
  *   workspace: device memory of iree_uk_mi355x_gated_mmt4d_backward_workspace()
  *   bytes, 256-byte aligned, which is written before it is read and holds
- *   nothing afterwards: dg and du, and where lhs_grad has few rows parts of its
- *   sums in f32. Calls that may run at the same time, graphs that hold
- *   them included, need workspaces of their own. (In synchronous mode it may be
- *   host memory like any other buffer; it is not touched then.) */
+ *   nothing afterwards: dg and du, in f16 what their largest is, and where
+ *   lhs_grad has few rows parts of its sums in f32. Calls that may run at the
+ *   same time, graphs that hold them included, need workspaces of their own. (In
+ *   synchronous mode it may be host memory like any other buffer; it is not
+ *   touched then.) */
 void iree_uk_mi355x_gated_mmt4d_backward_p(const iree_uk_mi355x_gated_mmt4d_backward_params_t* params);
 /* Bytes of workspace for a call with these sizes, flags and gradients (0 where
  * the call would be refused, which is reported as by the call). */

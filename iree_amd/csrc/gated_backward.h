@@ -15,6 +15,7 @@ struct GradResults {
   int64_t apart;
   Layout at;
   Float type;
+  const float* unit;           // of f16 operands: what dg and du are multiples of, a power of two
   int32_t accumulate;
   int32_t runs;                // eight (f32: four) columns from a multiple of that on lie next to each other, aligned
   uint32_t rows;               // of each
@@ -26,6 +27,7 @@ struct GradResults {
     const int r = lane & 31, half = lane >> 5;
     Layout l = at;
     l.stride0 = of_stride0;
+    const float of_one = T == Float::kF16 ? *unit : 1;
 #pragma unroll
     for (int i = 0; i < AM; ++i) {
       const uint32_t row = row0 + 32 * i + r;
@@ -40,7 +42,7 @@ struct GradResults {
           if (col >= cols) continue;
           float v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = acc[i][j][4 * q + e];
+          for (int e = 0; e < 8; ++e) v[e] = T == Float::kF16 ? acc[i][j][4 * q + e] * of_one : acc[i][j][4 * q + e];
           if (runs && col + 16 <= cols) store_runs<T>(v, to, l, row_at, col, half);
           else store_one_by_one<T>(v, to, l, row_at, col, cols, half);
         }

@@ -7,8 +7,53 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// dg and du of f16 operands are held as multiples of a power of two, the call's `unit`, which brings the largest of them (that is finite)
+// to between 2^14 and 2^15. As they are, 65504 and more would be infinite, which gradients of a scaled loss come to, and 2^-25 and less
+// zero; like this what is 2^-28 of the largest or more has all bits of an f16, and only what is less than 2^-39 of it is zero. A pass over
+// the inputs in front of the first step finds the largest, each of its workgroups one of some; the first step makes the unit of these, and
+// the products' results are multiplied by it in f32. (bf16 has f32's range.) The pass takes 26 us of 2048 x 8192, f16 throughout, 100 MB,
+// where the whole backward pass takes 600, and 4 of 130 x 1000.
+struct Scaling {
+  float* largest;  // [kMostLargest]
+  float* unit;     // or null: there is no dg
+  uint32_t count;  // of the largest
+};
+constexpr int kMostLargest = 8 * kThreads, kScalingBytes = 4 * kMostLargest + 256;
+
+// In the first step, by all of a workgroup: one over the unit.
+__device__ __forceinline__ float one_over_unit(const Scaling& s) {
+  __shared__ float of_wave[kThreads / 64];
+  float v = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kMostLargest / kThreads; ++i) {
+    const uint32_t at = i * kThreads + threadIdx.x;
+    v = __builtin_fmaxf(v, at < s.count ? s.largest[at] : 0);
+  }
+  for (int by = 32; by > 0; by /= 2) v = __builtin_fmaxf(v, __shfl_xor(v, by));
+  if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = v;
+  __syncthreads();
+  for (int w = 0; w < kThreads / 64; ++w) v = __builtin_fmaxf(v, of_wave[w]);
+  // (Of subnormals, and zeros, as large as a float's exponent has it.)
+  const int by = v == 0 ? 0 : 127 + 14 - (int)(__builtin_bit_cast(uint32_t, v) >> 23), power = by < 126 ? by : 126;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *s.unit = __builtin_bit_cast(float, (uint32_t)(127 - power) << 23);
+  return __builtin_bit_cast(float, (uint32_t)(127 + power) << 23);
+}
+// In the pass in front of it: the larger one.
+__device__ __forceinline__ float larger(float largest, float v) {
+  v = __builtin_fabsf(v);
+  return v < __builtin_inff() && v > largest ? v : largest;
+}
+__device__ __forceinline__ void put_largest(const Scaling& s, float v) {
+  __shared__ float of_wave[kThreads / 64];
+  for (int by = 32; by > 0; by /= 2) v = __builtin_fmaxf(v, __shfl_xor(v, by));
+  if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = v;
+  __syncthreads();
+  for (int w = 0; w < kThreads / 64; ++w) v = __builtin_fmaxf(v, of_wave[w]);
+  if (threadIdx.x == 0) s.largest[blockIdx.x] = v;
+}
+
 // The workspace: [rows][2 * cols] of the operands' type, a row's dg then its du, each filled up with zeros to a multiple of eight;
-// behind it, where lhs_grad's sums over the columns are split, [splits][rows][depth] of f32.
+// behind it, of f16, what Scaling has, and where lhs_grad's sums over the columns are split, [splits][rows][depth] of f32.
 struct Sizes {
   int64_t rows, cols, depth, pitch;
   explicit Sizes(const GatedBackwardArgs& a)
@@ -18,13 +63,17 @@ struct Sizes {
 struct BackwardArgs {
   GatedBackwardArgs p;
   Curve curve;
+  Scaling scaling;
   int64_t rows, cols, depth, pitch, results;
 };
 
-template <Float T>
+// LARGEST: the pass in front that finds it.
+template <Float T, bool LARGEST>
 __global__ __launch_bounds__(kThreads) void gated_backward_generic(const BackwardArgs g) {
   const GatedBackwardArgs& a = g.p;
   const int64_t half = g.pitch / 2;
+  const float times = T == Float::kF16 && !LARGEST ? one_over_unit(g.scaling) : 1;
+  float largest = 0;
   for (int64_t n = (int64_t)blockIdx.x * kThreads + threadIdx.x; n < g.results; n += (int64_t)gridDim.x * kThreads) {
     const int64_t row = n / half, col = n % half;
     float dg = 0, du = 0;
@@ -36,10 +85,20 @@ __global__ __launch_bounds__(kThreads) void gated_backward_generic(const Backwar
       du = grad * activated_and_slope(g.curve, element(a.pre_type, a.gate_pre, i * a.gate_pre_stride0 + in_row), &slope);
       dg = grad * u * slope;
     }
+    if constexpr (LARGEST) {
+      largest = larger(larger(largest, dg), du);
+      continue;
+    }
     uint16_t* to = (uint16_t*)a.workspace + row * g.pitch + col;
-    to[0] = mx_narrow<T>(dg);
-    to[half] = mx_narrow<T>(du);
+    to[0] = mx_narrow<T>(dg * times);
+    to[half] = mx_narrow<T>(du * times);
   }
+  if constexpr (LARGEST) put_largest(g.scaling, largest);
+}
+
+template <Float T>
+__device__ __forceinline__ float unit_of(const Scaling& s) {
+  return T == Float::kF16 && s.unit ? *s.unit : 1;
 }
 
 // lhs_grad: a thread for each result, which goes over the columns.
@@ -57,7 +116,8 @@ __global__ __launch_bounds__(kThreads) void gated_lhs_grad_generic(const Backwar
         sum += mx_widen<T>(from[g.pitch / 2 + col]) * element<T>(a.up, j * a.up_stride0 + at);
       }
     }
-    put_element(a.out_type, a.lhs_grad, row / a.M0 * a.lhs_grad_stride0 + (k / a.K0 * a.M0 + row % a.M0) * a.K0 + k % a.K0, sum);
+    put_element(a.out_type, a.lhs_grad, row / a.M0 * a.lhs_grad_stride0 + (k / a.K0 * a.M0 + row % a.M0) * a.K0 + k % a.K0,
+                sum * unit_of<T>(g.scaling));
   }
 }
 
@@ -74,6 +134,8 @@ __global__ __launch_bounds__(kThreads) void gated_weight_grad_generic(const Back
       sum_g += mx_widen<T>(from[0]) * x;
       sum_u += mx_widen<T>(from[g.pitch / 2]) * x;
     }
+    sum_g *= unit_of<T>(g.scaling);
+    sum_u *= unit_of<T>(g.scaling);
     const int64_t panel = col / a.N0, in_panel = (k / a.K0 * a.N0 + col % a.N0) * a.K0 + k % a.K0;
     if (a.gate_grad) {
       const int64_t at = panel * a.gate_grad_stride0 + in_panel;
@@ -95,13 +157,16 @@ struct FirstStep {
   uint8_t* grads;
   Layout gate_at, up_at, out_at;
   Curve curve;
+  Scaling scaling;
   int64_t results;  // eights
   uint32_t half, half_reciprocal;  // eights of a row's dg
   int64_t pitch;
   Float pre_type, out_type;
 };
-template <Float T>
+template <Float T, bool LARGEST>
 __global__ __launch_bounds__(kThreads) void gated_backward_first(const FirstStep p) {
+  const float times = T == Float::kF16 && !LARGEST ? one_over_unit(p.scaling) : 1;
+  float largest = 0;
   for (int64_t n = (int64_t)blockIdx.x * kThreads + threadIdx.x; n < p.results; n += (int64_t)gridDim.x * kThreads) {
     const uint32_t row = p.results < (1ll << 32) ? divide((uint32_t)n, p.half, p.half_reciprocal) : (uint32_t)(n / p.half);
     const uint32_t col = 8 * (uint32_t)(n - (int64_t)row * p.half);
@@ -120,11 +185,19 @@ __global__ __launch_bounds__(kThreads) void gated_backward_first(const FirstStep
       const float value = activated_and_slope(p.curve, g[e], &slope);
       g[e] = grad[e] * u[e] * slope;
       u[e] = grad[e] * value;
+      if constexpr (LARGEST) {
+        largest = larger(larger(largest, g[e]), u[e]);
+      } else {
+        g[e] *= times;
+        u[e] *= times;
+      }
     }
+    if constexpr (LARGEST) continue;
     const int64_t to = (int64_t)row * p.pitch + col;
     store_run<T, 8>(p.grads, to, g);
     store_run<T, 8>(p.grads, to + p.pitch / 2, u);
   }
+  if constexpr (LARGEST) put_largest(p.scaling, largest);
 }
 
 hipError_t launch_over(void (*f16)(const BackwardArgs), void (*bf16)(const BackwardArgs), BackwardArgs& g, int64_t results, hipStream_t stream) {
@@ -135,13 +208,26 @@ hipError_t launch_over(void (*f16)(const BackwardArgs), void (*bf16)(const Backw
   return launch_kernel(g.p.type == Float::kF16 ? f16 : bf16, grid, kThreads, 0, stream, g);
 }
 
+// The first step, of f16 behind the pass that finds the largest.
+template <typename P>
+hipError_t launch_step(void (*largest)(const P), void (*f16)(const P), void (*bf16)(const P), Float type, const P& p, hipStream_t stream) {
+  if (p.results == 0) return hipSuccess;
+  const int64_t groups = (p.results + kThreads - 1) / kThreads;
+  if (type == Float::kF16) {
+    const hipError_t e = launch_kernel(largest, p.scaling.count, kThreads, 0, stream, p);
+    if (e != hipSuccess) return e;
+  }
+  return launch_kernel(type == Float::kF16 ? f16 : bf16, (unsigned)(groups < (1 << 22) ? groups : 1 << 22), kThreads, 0, stream, p);
+}
+
 GradResults results_of(const GatedBackwardArgs& a, const Layout& at, uint8_t* first, uint8_t* second, int64_t stride0, int64_t stride1,
-                       int64_t rows, int64_t panels, bool accumulate) {
+                       int64_t rows, int64_t panels, const float* unit, bool accumulate) {
   GradResults r;
   r.out[0] = first; r.out[1] = second;
   r.stride0[0] = stride0; r.stride0[1] = stride1;
   r.at = at;
   r.type = a.out_type;
+  r.unit = unit;
   r.accumulate = accumulate;
   const int e = float_bytes(a.out_type);
   Layout other = at;
@@ -232,6 +318,15 @@ Choice choose_weight_grads(const Sizes& s, int64_t copies) {
 }
 int64_t copies_of(const GatedBackwardArgs& a) { return (a.gate_grad != nullptr) + (a.up_grad != nullptr); }
 int64_t grads_bytes(const Sizes& s) { return (s.rows * s.pitch * 2 + 255) / 256 * 256; }
+// Where the parts of sums begin.
+int64_t sums_at(const Sizes& s, Float type) { return grads_bytes(s) + (type == Float::kF16 && s.rows > 0 && s.cols > 0 ? kScalingBytes : 0); }
+// Of a first step of so many pieces of work, a thread for each or more.
+Scaling scaling_of(const GatedBackwardArgs& a, const Sizes& s, int64_t results) {
+  if (a.type != Float::kF16 || s.rows == 0 || s.cols == 0) return {nullptr, nullptr, 0};
+  float* const largest = (float*)(a.workspace + grads_bytes(s));
+  const int64_t groups = (results + kThreads - 1) / kThreads;
+  return {largest, largest + kMostLargest, (uint32_t)(groups < kMostLargest ? groups : kMostLargest)};
+}
 
 // The sums of lhs_grad's splits, in their order: a thread for four of a row. (2048 x 4096 in two parts: 15 us, 84 MB at 5.6 TB/s.)
 struct SumArgs {
@@ -278,12 +373,13 @@ bool as_lhs_grad(const GatedBackwardArgs& a, const Sizes& s, LhsGradProduct* p) 
   p->up_stride0 = up.stride0;
   p->lhs_second = s.pitch;  // (half of a row's bytes)
   p->depth = (uint32_t)s.cols;
-  p->results = results_of(a, layout_of(a.lhs_grad_stride0, a.M0, a.K, a.K0), a.lhs_grad, nullptr, a.lhs_grad_stride0, 0, s.rows, a.M, false);
+  p->results = results_of(a, layout_of(a.lhs_grad_stride0, a.M0, a.K, a.K0), a.lhs_grad, nullptr, a.lhs_grad_stride0, 0, s.rows, a.M,
+                          scaling_of(a, s, 0).unit, false);
   return true;
 }
 // (The depth is a multiple of eight.)
 void split_sums(const GatedBackwardArgs& a, const Sizes& s, int splits, GradResults* r) {
-  r->out[0] = a.workspace + grads_bytes(s);
+  r->out[0] = a.workspace + sums_at(s, a.type);
   r->at = layout_of(s.depth, 1, s.depth, 1);
   r->stride0[0] = s.depth;
   r->type = Float::kF32;
@@ -293,7 +389,7 @@ void split_sums(const GatedBackwardArgs& a, const Sizes& s, int splits, GradResu
 }
 hipError_t launch_sums(const GatedBackwardArgs& a, const Sizes& s, int splits, hipStream_t stream) {
   SumArgs g;
-  g.parts = (const float*)(a.workspace + grads_bytes(s));
+  g.parts = (const float*)(a.workspace + sums_at(s, a.type));
   g.out = a.lhs_grad;
   g.at = layout_of(a.lhs_grad_stride0, a.M0, a.K, a.K0);
   g.cols = (uint32_t)s.depth;
@@ -319,7 +415,8 @@ bool as_weight_grads(const GatedBackwardArgs& a, const Sizes& s, WeightGradProdu
   uint8_t* const first = a.gate_grad ? a.gate_grad : a.up_grad;
   uint8_t* const second = a.gate_grad ? a.up_grad : nullptr;
   const int64_t stride0 = a.gate_grad ? a.gate_grad_stride0 : a.up_grad_stride0;
-  p->results = results_of(a, layout_of(stride0, a.N0, a.K, a.K0), first, second, stride0, a.up_grad_stride0, s.cols, a.N, a.accumulate);
+  p->results = results_of(a, layout_of(stride0, a.N0, a.K, a.K0), first, second, stride0, a.up_grad_stride0, s.cols, a.N,
+                          scaling_of(a, s, 0).unit, a.accumulate);
   return true;
 }
 
@@ -341,9 +438,9 @@ bool launch_first(const GatedBackwardArgs& a, const Sizes& s, hipStream_t stream
   p.results = s.rows * p.half;
   p.pitch = s.pitch;
   p.pre_type = a.pre_type; p.out_type = a.out_type;
-  const int64_t groups = (p.results + kThreads - 1) / kThreads;
-  *e = launch_kernel(a.type == Float::kF16 ? gated_backward_first<Float::kF16> : gated_backward_first<Float::kBf16>,
-                     (unsigned)(groups < (1 << 22) ? groups : 1 << 22), kThreads, 0, stream, p);
+  p.scaling = scaling_of(a, s, p.results);
+  *e = launch_step(gated_backward_first<Float::kF16, true>, gated_backward_first<Float::kF16, false>, gated_backward_first<Float::kBf16, false>,
+                   a.type, p, stream);
   return true;
 }
 
@@ -353,7 +450,7 @@ int64_t gated_backward_workspace(const GatedBackwardArgs& a) {
   const Sizes s(a);
   int64_t bytes;
   if (__builtin_mul_overflow(s.rows, 2 * s.pitch, &bytes) || bytes > INT64_MAX - (1ll << 30)) return -1;
-  bytes = grads_bytes(s);
+  bytes = sums_at(s, a.type);
   if (a.lhs_grad) {
     int splits = choose_lhs_grad(s).splits;
     if (const int64_t copies = copies_of(a)) {
@@ -373,8 +470,11 @@ hipError_t launch_gated_backward(const GatedBackwardArgs& a, hipStream_t stream,
   g.rows = s.rows; g.cols = s.cols; g.depth = s.depth; g.pitch = s.pitch;
   *name = "gated_backward";
   hipError_t e = hipSuccess;
+  g.results = s.rows * (s.pitch / 2);
+  g.scaling = scaling_of(a, s, g.results);
   if (!launch_first(a, s, stream, &e))
-    e = launch_over(gated_backward_generic<Float::kF16>, gated_backward_generic<Float::kBf16>, g, s.rows * (s.pitch / 2), stream);
+    e = launch_step(gated_backward_generic<Float::kF16, true>, gated_backward_generic<Float::kF16, false>,
+                    gated_backward_generic<Float::kBf16, false>, a.type, g, stream);
   if (e != hipSuccess) return e;
   LhsGradProduct lhs;
   WeightGradProduct weights;
