@@ -474,16 +474,17 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterProduct p)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               v[c][e + i] = four[i];
-              largest = __builtin_fmaxf(largest, __builtin_fabsf(four[i]));
+              const float size = __builtin_fabsf(four[i]);
+              largest = size < __builtin_inff() && size > largest ? size : largest;
             }
           }
         __syncthreads();
         if constexpr (T == Float::kF16) {
-          // To below 2^15, with the row's other ranks. (What is not finite, and zeros, as they are.)
+          // To below 2^15, with the row's other ranks that are finite. (Zeros, and what is not finite, stay what they are.)
           largest = __builtin_fmaxf(largest, __shfl_xor(largest, 16));
           largest = __builtin_fmaxf(largest, __shfl_xor(largest, 32));
           const int field = (int)(__builtin_bit_cast(uint32_t, largest) >> 23);
-          const int by = field == 255 || field < 24 ? 0 : 127 + 14 - field;
+          const int by = field < 24 ? 0 : 127 + 14 - field;
           unit_of_row = ldexpf(1.0f, -by);
 #pragma unroll
           for (int c = 0; c < CHUNKS; ++c)
