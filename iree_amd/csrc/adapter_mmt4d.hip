@@ -375,14 +375,16 @@ __device__ __forceinline__ void split_sum(float v, uint16_t (&part)[3]) {
 // MANY: more ranks than that, whose sums are taken anew in every turn.
 //
 // The splits' sums are added on their way into LDS, where a workgroup's four wavefronts have them from; only those of rows that have the
-// adapter are read. The next turn's `up` and results are on their way while one's are multiplied.
+// adapter are read. A turn's `up` is asked for when the one before it has been multiplied, and its results when that one's are stored.
 //
 // 64 rows of 64 adapters x 14336, rank 16, take 14.0 us, 36 MB at 2.6 TB/s: a wavefront waits for its index, then for its sums, then has
-// three turns to make up for it. 2000 rows in runs x 4096, rank 64, take 23 us, of which the f32
+// three turns to make up for it. 2000 rows in runs x 4096, rank 64, take 20 to 23 us, of which the f32
 // results, read and written, are 65 MB. Results turned in LDS, so that four lanes have 64 bytes of a row, gained 4 % there and lost 10 % here.
 //
 // FAST: columns come in whole sixteens that lie next to each other, aligned, and an adapter's row of `up` in whole eights, aligned. (As
-// two branches of one kernel the slow one's registers halved the number of wavefronts on a compute unit.)
+// two branches of one kernel the slow one's registers halved the number of wavefronts on a compute unit.) Without it results go one by
+// one, also where only `up` is in the way: both launches of 64 rows of 64 adapters x 14336 x 4096 into f32 take 54 us with rank 4, 62
+// with 7 and 69 with 30, where 8 takes 19, 16 20 and 32 24; of 2000 rows in runs x 4096 x 4096 50, 52 and 57, and 26, 27 and 31.
 template <Float T, Float OUT, bool HALF, int CHUNKS, int F, bool FAST, bool MANY>
 __global__ __launch_bounds__(256) void adapter_up_kernel(const AdapterProduct p) {
   constexpr int SIZE = OUT == Float::kF32 ? 4 : 2, GROUP = HALF ? 16 : 32 * CHUNKS, PITCH = GROUP + 4;  // (rows 4 banks apart)
@@ -597,8 +599,8 @@ Tiles tiles_of(int64_t rows, int64_t count, int64_t depth, int64_t cols, int64_t
   if (saved * 2 * (double)rank * (double)(depth + cols) < (double)(16 << 20)) return {sixteens, false};
   return {own, true};
 }
-// How many parts K is split into: as many as leave every wavefront four chunks, while two workgroups, as many as a compute unit's LDS
-// holds, come to each. (2000 rows, rank 64, K 4096: 3 parts 14.9 us, 4 12.6, 6 15.3.)
+// How many parts K is split into: as many as leave every wavefront four chunks, while two workgroups come to a compute unit, which its LDS
+// holds of 16 ranks (64 KiB) and of more than 32 (80), but of 17 to 32 (96) one. (2000 rows, rank 64, K 4096: 3 parts 14.9 us, 4 12.6, 6 15.3.)
 uint32_t splits_of(int64_t rows_of_tiles, int64_t depth, int64_t rank) {
   const int waves = rank > 32 ? kWaves<kFragments> : kWaves<1>;
   const int64_t tiles = rows_of_tiles * ((rank + 16 * kFragments - 1) / (16 * kFragments));

@@ -104,7 +104,10 @@ bool block_covers(const GatedProduct& p) {
 // more than 16 rows the block kernels, which read the lhs less often, are left to decide.
 //
 // Fitted to the times of every kernel in 530 problems drawn from 1 to 4096 rows, 64 to 28672 columns, K of 64 to 14336, row-major and
-// tiled; over these the kernel taken is slower than the best one by 2.7 % in the mean, by more than 15 % in one of twenty.
+// tiled; over these the kernel taken is slower than the best one by 2.7 % in the mean, by more than 15 % in one of twenty. Those are times
+// of product16_block.h's loop in every tile. Where rows of the lhs are whole cache lines nine of the tiles run product16_lines.h's, which
+// is 2 to 13 % faster, each by another share: in 300 other problems like that, of 1 to 4096 rows, the kernel taken is slower than the best
+// one by 3.8 % in the mean, by more than 15 % in one of twelve.
 struct Choice {
   enum { kGeneric, kFew, kBlock } kernel;
   int number;

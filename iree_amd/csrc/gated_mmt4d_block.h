@@ -24,12 +24,12 @@ hipError_t launch_gated_block(const GatedProduct& g, int tile, hipStream_t strea
   // 128 x 11008 x 4096 53.2 -> 50.2. The same call made again at once finds its weights there: 29 -> 35, 36 -> 43 and 33 -> 49.
   const bool stream_rhs = g.lhs.rows <= 128 && 6 * (int64_t)g.gate.rows * g.depth > (256ll << 20);
   // Row-major rows that are whole cache lines are loaded by whole lines in the four largest tiles, one workgroup of which fits a compute
-  // unit, and in two others that still fit it twice with the longer ring: 512 x 11008 x 4096 in 256x96 tiles 100 -> 85 us,
-  // 4096 x 11008 x 4096 in 256x128 ones 624 -> 592, 300 x 11008 x 4096 in 192x96 72 -> 65, 128 x 11008 x 4096 in 64x96 50.3 -> 46.1,
-  // 400 x 4096 x 4096 in 128x64 37.2 -> 35.7. 64x64 tiles won 43.8 -> 40.2 for 64 rows but lost 35.2 -> 36.2 for 40 and 23.5 -> 24.3
+  // unit, and in two others that still fit it twice with the longer ring: 512 x 11008 x 4096 in 256x96 tiles 102 -> 90 us,
+  // 4096 x 11008 x 4096 in 256x128 ones 678 -> 654, 300 x 11008 x 4096 in 192x96 75.7 -> 72.4, 128 x 11008 x 4096 in 64x96 50.4 -> 46.6,
+  // 400 x 4096 x 4096 in 128x64 38.6 -> 37.3 (weights from memory, clocks settled, both in turn). 64x64 tiles won 43.8 -> 40.2 for 64 rows but lost 35.2 -> 36.2 for 40 and 23.5 -> 24.3
   // for 77, 64x32 ones gained nothing where they are taken. The other three would fit once and not twice, and so take it where there is
-  // a tile at most for a compute unit: 256 x 11008 x 4096 in 230 of 128x96 69.9 -> 59.8, 200 x 14336 x 4096 in 224 of 128x128
-  // 76.5 -> 67.7, 1024 x 4096 x 4096 in 256 62.9 -> 59.8, 400 x 4096 x 4096 in 224 of 64x128 38.6 -> 35.9; more tiles lost, 700 x 5632 x
+  // a tile at most for a compute unit: 256 x 11008 x 4096 in 230 of 128x96 70.3 -> 61.5, 200 x 14336 x 4096 in 224 of 128x128
+  // 77.6 -> 70.2, 1024 x 4096 x 4096 in 256 67.0 -> 65.2, 400 x 4096 x 4096 in 224 of 64x128 38.6 -> 35.9; more tiles lost, 700 x 5632 x
   // 2048 in 264 of 128x128 50.0 -> 56.7.
   const GatedTile& shape = kGatedTiles[tile];
   const bool one_each = ((int64_t)g.lhs.rows + shape.rows - 1) / shape.rows * (((int64_t)g.gate.rows + shape.cols - 1) / shape.cols) <= 256;

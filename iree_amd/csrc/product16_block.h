@@ -21,10 +21,10 @@
 // first) or, in turn, for another part of K.
 //
 // What bounds it. (Figures of row-major rows are those of product16_lines.h where their K allows.) Large products the board's power: 4096 x
-// 11008 x 4096, gate and up in 256x128 tiles, 592 us with row-major rows, 1.25 PFLOP/s (6 rounds of 256 tiles where 5.4 would do), 2048 x
-// 8192 x 4096, two whole rounds, 223 us, 1.23, where a library's plain product of 8192^3 reaches 1.35; with fewer compute units at work a
-// chunk takes 0.5 us and not 0.8. Some hundred rows the tiles' number: 512 x 11008 x 4096 in 230 tiles of 256x96 80 us from the caches and
-// 85 from memory (87 with the rows in tiles, 100 by half lines). Few rows the weights: 40 x 11008 x 4096 35 us, 180 MB at 5.2 TB/s, and
+// 11008 x 4096, gate and up in 256x128 tiles, 611 us with row-major rows, 1.21 PFLOP/s (6 rounds of 256 tiles where 5.4 would do), 2048 x
+// 8192 x 4096, two whole rounds, 220 us, 1.25, where a library's plain product of 8192^3 reaches 1.35; with fewer compute units at work a
+// chunk takes 0.5 us and not 0.8. Some hundred rows the tiles' number: 512 x 11008 x 4096 in 230 tiles of 256x96 81 us from the caches and
+// 90 from memory (87 with the rows in tiles, 102 by half lines). Few rows the weights: 40 x 11008 x 4096 35 us, 180 MB at 5.2 TB/s, and
 // short of that LDS, which 64 rows of chunks go into and come out of twice: 64x32 tiles take 0.12 us a chunk however few there are. Neither
 // deeper rings, nor touching all of the lhs first, nor columns in two launches (whole rounds, then the rest) gained.
 #ifndef IREE_AMD_CSRC_PRODUCT16_BLOCK_H_
