@@ -653,8 +653,9 @@ iree_uk_index_t iree_uk_mi355x_gated_mmt4d_backward_workspace(
  * floats of its type that add up to it (of f16 within 2^-24 of it, or 2^-39 of
  * the row's largest finite one), so that an infinite value of `up` gives
  * infinities or NaN. They take an lhs as above and a `down` whose address and
- * strides are multiples of 16 bytes; `up` may lie anywhere, and is read faster
- * aligned like that.
+ * strides are multiples of 16 bytes; `up` may lie anywhere, but takes two to
+ * three times as long where it is not aligned like that or rank is no multiple
+ * of 8.
  *   workspace: as above, of iree_uk_mi355x_adapter_mmt4d_workspace() bytes; it
  *   holds rank sums in f32 and, where rows are put in order, that. */
 void iree_uk_mi355x_adapter_mmt4d_p(const iree_uk_mi355x_adapter_mmt4d_params_t* params);

@@ -7,7 +7,7 @@
 //
 // What it saves is the L2's requests: 512 x 11008 x 4096, gate and up from memory, makes 11.0 million by half lines, 7.0 with the rows in
 // tiles, where a chunk's pieces lie together, and takes 102, 87 and, by whole lines, 90 us (1.03 PFLOP/s, 2.2 TB/s) once the clocks have
-// settled; in the first millisecond under load 85. 4096 x 11008 x 4096 takes 611 to 654 us by the box, 1.13 to 1.21 PFLOP/s, which the
+// settled; in the first millisecond under load 85. 4096 x 11008 x 4096 takes 611 to 654 us from card to card, 1.13 to 1.21 PFLOP/s, which the
 // board's power bounds.
 #ifndef IREE_AMD_CSRC_PRODUCT16_LINES_H_
 #define IREE_AMD_CSRC_PRODUCT16_LINES_H_

@@ -13,12 +13,12 @@ pytestmark = pytest.mark.gpu
 NAMES = ("lhs", "gate", "up", "gate_pre", "up_pre", "out_grad", "lhs_grad", "gate_grad", "up_grad")
 
 
-def bits(x, t0, t1):
-    """[rows][cols] -> panels of tiles of bf16, a row each."""
-    return torch.from_numpy(ref.raw(ref.tiled(x, t0, t1), "bf16").view(np.int16).reshape(x.shape[0] // t0, -1)).cuda()
+def bits(x, t0, t1, type="bf16"):
+    """[rows][cols] -> panels of tiles, a row each."""
+    return torch.from_numpy(ref.raw(ref.tiled(x, t0, t1), type).view(np.int16).reshape(x.shape[0] // t0, -1)).cuda()
 
 
-def call(lib, m, n, k, tile, held, stride={}):
+def call(lib, m, n, k, tile, held, stride={}, type="bf16"):
     p = abi.GatedMmt4dBackwardParams()
     ref.tiles_into(p, m, n, k, tile)
     m0, n0, _ = tile
@@ -26,22 +26,22 @@ def call(lib, m, n, k, tile, held, stride={}):
     for name in NAMES:
         setattr(p, name + "_buffer", held[name].data_ptr())
         setattr(p, name + "_stride0", stride.get(name, panel.get(name, m0 * n)))
-    p.flags = abi.GATED_MMT4D_TYPE_BF16BF16BF16 | abi.GATED_MMT4D_SILU
+    p.flags = ref.type_flag("GATED_MMT4D", type, type) | abi.GATED_MMT4D_SILU
     keep, size = ref.workspace(lib, "gated_mmt4d_backward", p)
     ref.call(lib, "gated_mmt4d_backward", p)
     assert bool((keep[size:] == 0xFF).all())
     return size
 
 
-def problem(seed, m, n, k):
+def problem(seed, m, n, k, type="bf16"):
     rng = np.random.default_rng(seed)
-    return dict(x=values(rng, m, k, "bf16"), gate=values(rng, n, k, "bf16", 0.2), up_=values(rng, n, k, "bf16", 0.2),
-                g=values(rng, m, n, "bf16", 1.5), u=values(rng, m, n, "bf16", 1.5), grad=values(rng, m, n, "bf16"))
+    return dict(x=values(rng, m, k, type), gate=values(rng, n, k, type, 0.2), up_=values(rng, n, k, type, 0.2),
+                g=values(rng, m, n, type, 1.5), u=values(rng, m, n, type, 1.5), grad=values(rng, m, n, type))
 
 
-def matrix_of(panels, t0, t1):
+def matrix_of(panels, t0, t1, type="bf16"):
     """Panels of tiles in device memory -> [rows][cols]"""
-    x = panels.view(torch.bfloat16).float().cpu().numpy().astype(np.float64)
+    x = panels.view(torch.float16 if type == "f16" else torch.bfloat16).float().cpu().numpy().astype(np.float64)
     return ref.untiled(x.reshape(x.shape[0], -1, t0, t1))
 
 
@@ -51,25 +51,25 @@ def all_zero(panels):
 
 # The gradient of out is zero but in the last 48 rows: those of lhs_grad are not zero, and the weights' gradients are sums over them.
 @pytest.mark.parametrize("n,k", [(8192, 64), (64, 16384)])
-@pytest.mark.parametrize("m0", [1, 16])
-def test_many_rows(gpu_lib, m0, n, k):  # noqa: F811
+@pytest.mark.parametrize("m0,type", [(1, "bf16"), (16, "bf16"), (16, "f16")])
+def test_many_rows(gpu_lib, m0, type, n, k):  # noqa: F811
     m, last, tile = 139264, 48, (m0, 16, 16)
     assert m * max(2 * n, k) > 2 ** 31
-    given = problem(n, last, n, k)
+    given = problem(n, last, n, k, type)
     held = {name: torch.full((m // m0, m0 * cols), 0x3F80, dtype=torch.int16, device="cuda")
             for name, cols in (("lhs", k), ("lhs_grad", k), ("gate_pre", n), ("up_pre", n), ("out_grad", n))}
     held["out_grad"].zero_()
     for name, of, t1 in (("lhs", "x", 16), ("gate_pre", "g", 16), ("up_pre", "u", 16), ("out_grad", "grad", 16)):
-        held[name][-last // m0:] = bits(given[of], m0, t1)
+        held[name][-last // m0:] = bits(given[of], m0, t1, type)
     for name, of in (("gate", "gate"), ("up", "up_")):
-        held[name], held[name + "_grad"] = bits(given[of], 16, 16), torch.full((n // 16, 16 * k), 0x3F80, dtype=torch.int16, device="cuda")
-    assert call(gpu_lib, m, n, k, tile, held) >= 4 * m * n
-    want, off = ref.backward(activation="silu", type="bf16", **given)
+        held[name], held[name + "_grad"] = bits(given[of], 16, 16, type), torch.full((n // 16, 16 * k), 0x3F80, dtype=torch.int16, device="cuda")
+    assert call(gpu_lib, m, n, k, tile, held, type=type) >= 4 * m * n
+    want, off = ref.backward(activation="silu", type=type, **given)
     assert all_zero(held["lhs_grad"][:-last // m0])
-    check(matrix_of(held["lhs_grad"][-last // m0:], m0, 16), want[0], off[0], "bf16")
+    check(matrix_of(held["lhs_grad"][-last // m0:], m0, 16, type), want[0], off[0], type)
     # (Rows of zeros add nothing, exactly.)
-    check(matrix_of(held["gate_grad"], 16, 16), want[1], off[1], "bf16")
-    check(matrix_of(held["up_grad"], 16, 16), want[2], off[2], "bf16")
+    check(matrix_of(held["gate_grad"], 16, 16, type), want[1], off[1], type)
+    check(matrix_of(held["up_grad"], 16, 16, type), want[2], off[2], type)
 
 
 # The gradient of out is zero but in the last 64 columns: only theirs of the weights' gradients are not zero.

@@ -76,6 +76,14 @@ def test_nothing_but_zeros(gpu_lib):  # noqa: F811
         assert (x == 0).all()
 
 
+@pytest.mark.parametrize("m,n", [(0, 32), (8, 0)])
+def test_sums_over_nothing(gpu_lib, m, n):  # noqa: F811
+    given, _ = inputs(1, m, n, 48, (1, 16, 16), "f16", "f32", "f32")
+    got, _ = ref.run_backward(gpu_lib, activation="silu", tile=(1, 16, 16), type="f16", out="f32", pre_type="f32", **given)
+    for x in got:
+        assert (x == 0).all()
+
+
 @pytest.mark.parametrize("strange", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("power", [0, 30, -30])
 def test_values_that_are_not_finite_are_not_the_largest(gpu_lib, strange, power):  # noqa: F811
